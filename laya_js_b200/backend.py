@@ -30,7 +30,7 @@ _MODE = {"symmetric": 0, "affine": 1}
 class CudaTensor:
     """An opaque device tensor handle (index.ts:75-78 Tensor: shape + dtype)."""
 
-    __slots__ = ("handle", "shape", "dtype", "disposed", "_backend", "__weakref__")
+    __slots__ = ("handle", "shape", "dtype", "disposed", "keep", "_backend", "__weakref__")  # keep: owner of borrowed memory
 
     def __init__(self, backend: "CudaBackend", handle: int):
         self._backend = backend

@@ -1,0 +1,423 @@
+// Low-rank adapters of many requests beside a shared projection, and their
+// gradients (include/laya_cuda_adapters.h).
+//
+// Three products make both directions, because the banks keep their long axis
+// contiguous (A [n, r, K], B [n, r, N]) and enter symmetrically:
+//   shrink  Q[t, :] = s_a · P_a · X[t]             u (X = x, P = A), g (X = dy, P = B)
+//   expand  Y[t, :] = W-product of X[t] + P_aᵀ·Q[t] y (P = B), dx (P = A, W read transposed)
+//   outer   dP_a    = Σ_{t in a} Q[t] ⊗ X[t]       dA (Q = g, X = x), dB (Q = u, X = dy)
+// Q holds f32.
+//
+// The kernels of this file take every dtype, size and rank: one thread block
+// per tile, f32 sums in registers.
+#include "lc_adapters.h"
+#include "lc_api.h"
+#include "laya_cuda_adapters.h"
+
+#include <algorithm>
+#include <cmath>
+#include <memory>
+#include <unordered_set>
+#include <vector>
+
+namespace {
+using namespace lc;
+
+// ------------------------------------------------------------- the plan
+
+std::unordered_set<AdapterPlan*>& plans() {
+  static std::unordered_set<AdapterPlan*> s;
+  return s;
+}
+
+AdapterPlan* check_plan(uint64_t h) {
+  AdapterPlan* p = reinterpret_cast<AdapterPlan*>(h);
+  LC_CHECK(h && plans().count(p), "adapters: invalid or freed plan handle");
+  return p;
+}
+
+// The plan's arrays are written once, by the copy that builds it: a use on
+// another stream waits for that copy.
+void plan_enter(AdapterPlan* p) {
+  cudaStream_t st = stream();
+  if (st == p->built_on) return;
+  p->shared = true;
+  if (p->settled || (p->settled = cudaEventQuery(p->built) == cudaSuccess)) return;
+  cudaGetLastError();
+  // a capturing stream cannot wait for an event recorded outside the capture
+  if (capturing()) CUDA_OK(cudaEventSynchronize(p->built));
+  else CUDA_OK(cudaStreamWaitEvent(st, p->built, 0));
+}
+
+void plan_release(AdapterPlan* p) {
+  if (p->shared && !capturing()) cudaDeviceSynchronize();  // the memory is freed in the order of one stream
+  if (p->dev) dfree(p->dev);
+  if (p->built) cudaEventDestroy(p->built);
+  delete p;
+}
+
+// ------------------------------------------------------------- kernels for every dtype and size
+
+// Q[t, j] = s_a · Σ_k X[t, k]·P[a, j, k]; rows without an adapter get zeros.
+// A block per row, a warp per rank row j.
+template <typename T>
+__global__ void __launch_bounds__(128) k_shrink_any(const T* __restrict__ X, const T* __restrict__ P, const float* __restrict__ scales,
+                                                    const int32_t* __restrict__ row_adapter, float* __restrict__ Q, int C, int r) {
+  const int64_t t = blockIdx.x;
+  const int a = row_adapter[t], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float s = a >= 0 ? (scales ? scales[a] : 1.f) : 0.f;
+  const T* x = X + t * C;
+  for (int j = warp; j < r; j += 4) {
+    float acc = 0.f;
+    if (a >= 0) {
+      const T* p = P + ((int64_t)a * r + j) * C;
+      for (int k = lane; k < C; k += 32) acc = fmaf(to_f<T>(x[k]), to_f<T>(p[k]), acc);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    }
+    if (lane == 0) Q[t * r + j] = a >= 0 ? s * acc : 0.f;
+  }
+}
+
+// Y[m, n] = Σ_k X[m, k]·W(n, k) (+ bias[n]) + Σ_j Q[m, j]·P[a(m), j, n], with
+// W(n, k) = W[n·swn + k·swk]. 64 x 64 tiles, 4 x 4 outputs per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) k_expand_any(const T* __restrict__ X, const T* __restrict__ W, int64_t swn, int64_t swk,
+                                                    const char* bias, int bias_dtype, const float* __restrict__ Q,
+                                                    const T* __restrict__ P, const int32_t* __restrict__ row_adapter, T* __restrict__ Y,
+                                                    int64_t M, int N, int K, int r) {
+  __shared__ float xs[16][64 + 4], ws[16][64 + 4];
+  const int64_t m0 = (int64_t)blockIdx.x * 64;
+  const int n0 = blockIdx.y * 64, tid = threadIdx.x, tm = (tid >> 4) * 4, tn = (tid & 15) * 4;
+  float acc[4][4] = {};
+  if (W)
+    for (int k0 = 0; k0 < K; k0 += 16) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int e = tid + 256 * i;
+        {
+          const int m = e >> 4, k = e & 15;
+          xs[k][m] = (m0 + m < M && k0 + k < K) ? to_f<T>(X[(m0 + m) * K + k0 + k]) : 0.f;
+        }
+        // the fast index of the load follows W's contiguous axis
+        const int n = swk == 1 ? e >> 4 : e & 63, k = swk == 1 ? e & 15 : e >> 6;
+        ws[k][n] = (n0 + n < N && k0 + k < K) ? to_f<T>(W[(n0 + n) * swn + (k0 + k) * swk]) : 0.f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 16; k++) {
+        const float4 xv = *(const float4*)&xs[k][tm], wv = *(const float4*)&ws[k][tn];
+        const float xa[4] = {xv.x, xv.y, xv.z, xv.w}, wa[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) acc[i][j] = fmaf(xa[i], wa[j], acc[i][j]);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int64_t m = m0 + tm + i;
+    if (m >= M) break;
+    const int a = row_adapter[m];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int n = n0 + tn + j;
+      if (n >= N) break;
+      float v = acc[i][j];
+      if (bias) v += ld_as<float>(bias, bias_dtype, n);
+      if (a >= 0) {
+        const T* p = P + (int64_t)a * r * N + n;
+        const float* q = Q + m * r;
+        float d = 0.f;
+        for (int l = 0; l < r; l++) d = fmaf(q[l], to_f<T>(p[(int64_t)l * N]), d);
+        v += d;
+      }
+      Y[m * N + n] = from_f<T>(v);
+    }
+  }
+}
+
+// dP[a, j, c] = Σ_{t in a} Q[t, j]·X[t, c]: a block per adapter, 8 rank rows
+// and 128 columns; rows in order, in groups of 64 so that a long sum loses no
+// more than a short one.
+template <typename T>
+__global__ void __launch_bounds__(128) k_outer_any(const float* __restrict__ Q, const T* __restrict__ X, const int2* __restrict__ spans,
+                                                   const int32_t* __restrict__ span_ptr, T* __restrict__ dP, int C, int r) {
+  const int a = blockIdx.z, j0 = blockIdx.y * 8, c = blockIdx.x * 128 + threadIdx.x;
+  const int nj = min(8, r - j0);
+  float acc[8] = {}, part[8] = {};
+  int n = 0;
+  for (int s = span_ptr[a]; s < span_ptr[a + 1]; s++) {
+    const int2 rows = spans[s];
+    for (int t = rows.x; t < rows.y; t++) {
+      const float x = c < C ? to_f<T>(X[(int64_t)t * C + c]) : 0.f;
+      const float* q = Q + (int64_t)t * r + j0;
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (j < nj) part[j] = fmaf(q[j], x, part[j]);
+      if (++n == 64) {
+        n = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc[j] += part[j], part[j] = 0.f;
+      }
+    }
+  }
+  if (c < C)
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (j < nj) dP[((int64_t)a * r + j0 + j) * C + c] = from_f<T>(acc[j] + part[j]);
+}
+
+// ------------------------------------------------------------- operands
+
+struct Held {  // tensors made inside an op, released when it returns or throws
+  std::vector<LcTensor*> ts;
+  std::vector<void*> mem;
+  ~Held() {
+    for (auto* t : ts) release(t);
+    for (void* p : mem) dfree(p);
+  }
+  LcTensor* dense(LcTensor* t) {
+    LcTensor* c = contiguous(t);
+    if (c != t) ts.push_back(c);
+    return c;
+  }
+  LcTensor* made(LcTensor* t) {
+    ts.push_back(t);
+    return t;
+  }
+  void* scratch(size_t bytes) {
+    mem.push_back(nullptr);
+    return mem.back() = dmalloc(bytes);
+  }
+  LcTensor* keep(LcTensor* t) {  // handed to the caller: no longer released here
+    ts.erase(std::find(ts.begin(), ts.end(), t));
+    return t;
+  }
+};
+
+struct Operands {
+  AdapterPlan* plan = nullptr;
+  LcTensor *x = nullptr, *dy = nullptr, *w = nullptr, *bias = nullptr, *a = nullptr, *b = nullptr, *scales = nullptr;
+  int64_t T = 0, K = 0, N = 0;
+  int r = 0, n = 0, dtype = 0;
+  const float* scale_ptr() const { return scales ? (const float*)scales->data() : nullptr; }
+};
+
+Operands operands(const char* op, lc_tensor xh, lc_tensor dyh, lc_tensor wh, lc_tensor biash, lc_tensor ah, lc_tensor bh, lc_tensor sh,
+                  uint64_t planh, Held& held) {
+  const std::string name(op);
+  Operands o;
+  o.plan = check_plan(planh);
+  LcTensor* x = check(xh, op);
+  LcTensor* a = check(ah, op);
+  LcTensor* b = check(bh, op);
+  LcTensor* w = wh ? check(wh, op) : nullptr;
+  LcTensor* dy = dyh ? check(dyh, op) : nullptr;
+  LcTensor* bias = biash ? check(biash, op) : nullptr;
+  LcTensor* s = sh ? check(sh, op) : nullptr;
+  o.dtype = x->dtype;
+  LC_CHECK(o.dtype == LC_F32 || is_half(o.dtype), name + ": x must be f32, f16 or bf16, got " + dtype_name(o.dtype));
+  LC_CHECK(x->ndim >= 1, name + ": x [..., in] expected");
+  LC_CHECK(a->ndim == 3 && b->ndim == 3, name + ": a [n, r, in] and b [n, r, out] expected");
+  for (LcTensor* t : {a, b, w, dy})
+    if (t) LC_CHECK(t->dtype == o.dtype, name + ": x, w, a, b (and dy) must share a dtype, got " + dtype_name(o.dtype) + " and " + dtype_name(t->dtype));
+  o.K = x->shape[x->ndim - 1];
+  o.N = b->shape[2];
+  const int64_t rows = o.K ? x->numel() / o.K : 0;
+  LC_CHECK(o.K >= 1 && o.N >= 1, name + ": in and out must be at least 1");
+  LC_CHECK(o.K <= INT32_MAX / 8 && o.N <= INT32_MAX / 8, name + ": in or out is too large");
+  LC_CHECK(a->shape[2] == o.K, name + ": x " + shape_str(x->dims()) + " vs a " + shape_str(a->dims()));
+  LC_CHECK(a->shape[0] == b->shape[0] && a->shape[1] == b->shape[1], name + ": a " + shape_str(a->dims()) + " vs b " + shape_str(b->dims()));
+  LC_CHECK(a->shape[0] == o.plan->n_adapters,
+           name + ": the plan was made for " + std::to_string(o.plan->n_adapters) + " adapters, a " + shape_str(a->dims()));
+  LC_CHECK(a->shape[1] >= 1 && a->shape[1] <= kAdapterMaxRank, name + ": rank must be 1 to " + std::to_string(kAdapterMaxRank));
+  LC_CHECK(rows == o.plan->rows, name + ": x has " + std::to_string(rows) + " rows, the plan " + std::to_string(o.plan->rows));
+  if (w) LC_CHECK(w->ndim == 2 && w->shape[0] == o.N && w->shape[1] == o.K,
+                  name + ": w " + shape_str(w->dims()) + ", expected [" + std::to_string(o.N) + "," + std::to_string(o.K) + "]");
+  if (bias) LC_CHECK(bias->numel() == o.N && (bias->dtype == LC_F32 || is_half(bias->dtype)), name + ": bias must hold out f32, f16 or bf16 values");
+  if (s) LC_CHECK(s->dtype == LC_F32 && s->ndim == 1 && s->shape[0] == a->shape[0], name + ": scales must be f32 [n]");
+  if (dy) {
+    std::vector<int64_t> want = x->dims();
+    want.back() = o.N;
+    LC_CHECK(dy->dims() == want, name + ": dy " + shape_str(dy->dims()) + ", expected " + shape_str(want));
+  }
+  o.T = rows;
+  o.r = (int)a->shape[1];
+  o.n = (int)a->shape[0];
+  o.x = held.dense(x);
+  o.a = held.dense(a);
+  o.b = held.dense(b);
+  if (w) o.w = held.dense(w);
+  if (dy) o.dy = held.dense(dy);
+  if (bias) o.bias = held.dense(bias);
+  if (s) o.scales = held.dense(s);
+  plan_enter(o.plan);
+  return o;
+}
+
+#define LC_FLOAT_SWITCH(dtype, ...)                                        \
+  switch (dtype) {                                                         \
+    case LC_F32: { using T = float; __VA_ARGS__; } break;                  \
+    case LC_F16: { using T = __half; __VA_ARGS__; } break;                 \
+    default: { using T = __nv_bfloat16; __VA_ARGS__; } break;              \
+  }
+
+void shrink(const Operands& o, const LcTensor* X, const LcTensor* P, int64_t C, float* Q) {
+  if (!o.T) return;
+  LC_FLOAT_SWITCH(o.dtype, launch_chain(k_shrink_any<T>, dim3((unsigned)o.T), dim3(128), 0, stream(), (const T*)X->data(), (const T*)P->data(),
+                                        o.scale_ptr(), (const int32_t*)o.plan->row_adapter, Q, (int)C, o.r));
+  LC_LAUNCHED(1);
+}
+
+// y (transposed = false: w [N, K], C_in = K) or dx (transposed = true: C_in = N)
+void expand(const Operands& o, const LcTensor* X, const LcTensor* P, const float* Q, bool transposed, LcTensor* Y) {
+  if (!o.T) return;
+  const int64_t in = transposed ? o.N : o.K, out = transposed ? o.K : o.N;
+  const LcTensor* bias = transposed ? nullptr : o.bias;
+  dim3 grid((unsigned)((o.T + 63) / 64), (unsigned)((out + 63) / 64));
+  LC_CHECK(grid.y <= 65535, "adapters: too many output columns");
+  LC_FLOAT_SWITCH(o.dtype, launch_chain(k_expand_any<T>, grid, dim3(256), 0, stream(), (const T*)X->data(), o.w ? (const T*)o.w->data() : (const T*)nullptr,
+                                        transposed ? (int64_t)1 : o.K, transposed ? o.K : (int64_t)1, bias ? (const char*)bias->data() : (const char*)nullptr,
+                                        bias ? bias->dtype : 0, Q, (const T*)P->data(), (const int32_t*)o.plan->row_adapter, (T*)Y->data(), o.T,
+                                        (int)out, (int)in, o.r));
+  LC_LAUNCHED(1);
+}
+
+void outer(const Operands& o, const float* Q, const LcTensor* X, int64_t C, LcTensor* dP) {
+  if (!o.n) return;
+  dim3 grid((unsigned)((C + 127) / 128), (unsigned)((o.r + 7) / 8), (unsigned)o.n);
+  LC_CHECK(grid.z <= 65535, "adapters: more than 65535 adapters");
+  LC_FLOAT_SWITCH(o.dtype, launch_chain(k_outer_any<T>, grid, dim3(128), 0, stream(), Q, (const T*)X->data(), (const int2*)o.plan->spans,
+                                        (const int32_t*)o.plan->span_ptr, (T*)dP->data(), (int)C, o.r));
+  LC_LAUNCHED(1);
+}
+
+}  // namespace
+
+void lc_adapters_destroy() {
+  for (auto* p : plans()) plan_release(p);
+  plans().clear();
+}
+
+extern "C" {
+
+int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t* adapters, int nseg, int n_adapters) {
+  LC_API_BEGIN
+  cudaStream_t st = stream();
+  LC_CHECK(st, "liblaya_cuda: lc_init(device) was not called");
+  LC_CHECK(nseg >= 0 && cu_rows && (adapters || !nseg), "adapter plan: cu_rows and adapters are required");
+  LC_CHECK(n_adapters >= 0, "adapter plan: n_adapters must be >= 0");
+  LC_CHECK(!capturing(), "adapter plan: cannot be created while capturing");
+  LC_CHECK(cu_rows[0] == 0, "adapter plan: cu_rows must start at 0");
+  for (int i = 0; i < nseg; i++) {
+    LC_CHECK(cu_rows[i + 1] >= cu_rows[i], "adapter plan: cu_rows must not decrease (request " + std::to_string(i) + ")");
+    LC_CHECK(adapters[i] >= -1 && adapters[i] < n_adapters,
+             "adapter plan: request " + std::to_string(i) + " uses adapter " + std::to_string(adapters[i]) + " of " + std::to_string(n_adapters));
+  }
+  const int T = cu_rows[nseg];
+  // the requests that have rows and an adapter; neighbours with the same adapter become one
+  struct Seg { int lo, hi, a; };
+  std::vector<Seg> segs;
+  for (int i = 0; i < nseg; i++) {
+    if (adapters[i] < 0 || cu_rows[i + 1] == cu_rows[i]) continue;
+    if (!segs.empty() && segs.back().a == adapters[i] && segs.back().hi == cu_rows[i]) segs.back().hi = cu_rows[i + 1];
+    else segs.push_back({cu_rows[i], cu_rows[i + 1], adapters[i]});
+  }
+  // device image: adapter of each row | spans by adapter | where each adapter's spans start
+  const size_t S = segs.size();
+  std::vector<int32_t> span_ptr(n_adapters + 1, 0);
+  for (auto& s : segs) span_ptr[s.a + 1]++;
+  for (int a = 0; a < n_adapters; a++) span_ptr[a + 1] += span_ptr[a];
+  std::vector<int32_t> at(span_ptr.begin(), span_ptr.end() - 1), spans(2 * S);
+  for (auto& s : segs) {
+    const int k = at[s.a]++;
+    spans[2 * k] = s.lo;
+    spans[2 * k + 1] = s.hi;
+  }
+  std::vector<int32_t> row_adapter(T, -1);
+  for (auto& s : segs) std::fill(row_adapter.begin() + s.lo, row_adapter.begin() + s.hi, s.a);
+  std::vector<int32_t> image;
+  auto put = [&](const std::vector<int32_t>& v) {
+    const size_t off = image.size();
+    image.insert(image.end(), v.begin(), v.end());
+    image.resize((image.size() + 63) / 64 * 64);
+    return off;
+  };
+  const size_t o_rows = put(row_adapter), o_spans = put(spans), o_ptr = put(span_ptr);
+  struct Guard {
+    AdapterPlan* p;
+    ~Guard() { if (p) plan_release(p); }
+  } g{new AdapterPlan()};
+  AdapterPlan* p = g.p;
+  p->rows = T;
+  p->n_adapters = n_adapters;
+  p->nspans = (int)S;
+  p->built_on = st;
+  CUDA_OK(cudaEventCreateWithFlags(&p->built, cudaEventDisableTiming));
+  p->dev = (int32_t*)dmalloc(image.size() * 4);
+  // pageable source: staged when the call returns
+  CUDA_OK(cudaMemcpyAsync(p->dev, image.data(), image.size() * 4, cudaMemcpyHostToDevice, st));
+  CUDA_OK(cudaEventRecord(p->built, st));
+  p->row_adapter = p->dev + o_rows;
+  p->spans = (int2*)(p->dev + o_spans);
+  p->span_ptr = p->dev + o_ptr;
+  plans().insert(p);
+  g.p = nullptr;
+  *out = reinterpret_cast<uint64_t>(p);
+  LC_API_END
+}
+
+int lc_adapter_plan_free(uint64_t h) {
+  LC_API_BEGIN
+  AdapterPlan* p = check_plan(h);
+  plan_enter(p);
+  plans().erase(p);
+  plan_release(p);
+  LC_API_END
+}
+
+int lc_adapter_linear(lc_tensor* out, lc_tensor xh, lc_tensor wh, lc_tensor biash, lc_tensor ah, lc_tensor bh, lc_tensor sh, uint64_t plan) {
+  LC_API_BEGIN
+  Held held;
+  LC_CHECK(out, "adapter_linear: out is required");
+  Operands o = operands("adapter_linear", xh, 0, wh, biash, ah, bh, sh, plan, held);
+  std::vector<int64_t> shape = check(xh, "adapter_linear")->dims();
+  shape.back() = o.N;
+  LcTensor* y = held.made(alloc(o.dtype, shape));
+  float* u = (float*)held.scratch((size_t)o.T * o.r * 4);
+  shrink(o, o.x, o.a, o.K, u);
+  expand(o, o.x, o.b, u, false, y);
+  *out = handle(held.keep(y));
+  LC_API_END
+}
+
+int lc_adapter_linear_grad(lc_tensor* dxo, lc_tensor* dao, lc_tensor* dbo, lc_tensor dyh, lc_tensor xh, lc_tensor wh, lc_tensor ah, lc_tensor bh,
+                           lc_tensor sh, uint64_t plan) {
+  LC_API_BEGIN
+  Held held;
+  LC_CHECK(dyh, "adapter_linear_grad: dy is required");
+  Operands o = operands("adapter_linear_grad", xh, dyh, wh, 0, ah, bh, sh, plan, held);
+  LcTensor *dx = nullptr, *da = nullptr, *db = nullptr;
+  if (dxo) dx = held.made(alloc(o.dtype, check(xh, "adapter_linear_grad")->dims()));
+  if (dao) da = held.made(alloc(o.dtype, o.a->dims()));
+  if (dbo) db = held.made(alloc(o.dtype, o.b->dims()));
+  if (dx || da) {
+    float* g = (float*)held.scratch((size_t)o.T * o.r * 4);
+    shrink(o, o.dy, o.b, o.N, g);
+    if (dx) expand(o, o.dy, o.a, g, true, dx);
+    if (da) outer(o, g, o.x, o.K, da);
+  }
+  if (db) {
+    float* u = (float*)held.scratch((size_t)o.T * o.r * 4);
+    shrink(o, o.x, o.a, o.K, u);
+    outer(o, u, o.dy, o.N, db);
+  }
+  if (dx) *dxo = handle(held.keep(dx));
+  if (da) *dao = handle(held.keep(da));
+  if (db) *dbo = handle(held.keep(db));
+  LC_API_END
+}
+
+}  // extern "C"

@@ -4,6 +4,7 @@
 // tcgen05 GEMM does not take (packages/tensor-backend/src/index.ts:208-243).
 #include "lc_api.h"
 #include "lc_gelu.cuh"
+#include "lc_adapters.h"
 #include "lc_gemm.h"
 
 #include <cmath>
@@ -483,6 +484,7 @@ void lc_internal_destroy_caches() {
   for (float* d : rope_retired()) cudaFree(d);
   rope_retired().clear();
   lc_gemm_destroy_caches();
+  lc_adapters_destroy();
 }
 
 // ------------------------------------------------------------- sdpa (generic)
