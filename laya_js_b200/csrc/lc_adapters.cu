@@ -6,12 +6,14 @@
 //   shrink  Q[t, :] = s_a · P_a · X[t]             u (X = x, P = A), g (X = dy, P = B)
 //   expand  Y[t, :] = W-product of X[t] + P_aᵀ·Q[t] y (P = B), dx (P = A, W read transposed)
 //   outer   dP_a    = Σ_{t in a} Q[t] ⊗ X[t]       dA (Q = g, X = x), dB (Q = u, X = dy)
-// Q holds f32.
 //
-// The kernels of this file take every dtype, size and rank: one thread block
-// per tile, f32 sums in registers.
+// f16 and bf16 run on the tensor cores (lc_adapters_tc.cu, gemm_adapted in
+// lc_gemm.cu), which read 16-byte aligned rows: operands with other widths or
+// addresses are copied into padded rows first. The kernels of this file serve
+// f32: one thread block per tile, f32 sums in registers, Q in f32.
 #include "lc_adapters.h"
 #include "lc_api.h"
+#include "lc_gemm.h"
 #include "laya_cuda_adapters.h"
 
 #include <algorithm>
@@ -56,22 +58,23 @@ void plan_release(AdapterPlan* p) {
   delete p;
 }
 
-// ------------------------------------------------------------- kernels for every dtype and size
+// ------------------------------------------------------------- f32
 
 // Q[t, j] = s_a · Σ_k X[t, k]·P[a, j, k]; rows without an adapter get zeros.
 // A block per row, a warp per rank row j.
-template <typename T>
-__global__ void __launch_bounds__(128) k_shrink_any(const T* __restrict__ X, const T* __restrict__ P, const float* __restrict__ scales,
+__global__ void __launch_bounds__(128) k_shrink_f32(const float* __restrict__ X, const float* __restrict__ P, const float* __restrict__ scales,
                                                     const int32_t* __restrict__ row_adapter, float* __restrict__ Q, int C, int r) {
+  pdl_trigger();
+  pdl_wait();
   const int64_t t = blockIdx.x;
   const int a = row_adapter[t], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float s = a >= 0 ? (scales ? scales[a] : 1.f) : 0.f;
-  const T* x = X + t * C;
+  const float* x = X + t * C;
   for (int j = warp; j < r; j += 4) {
     float acc = 0.f;
     if (a >= 0) {
-      const T* p = P + ((int64_t)a * r + j) * C;
-      for (int k = lane; k < C; k += 32) acc = fmaf(to_f<T>(x[k]), to_f<T>(p[k]), acc);
+      const float* p = P + ((int64_t)a * r + j) * C;
+      for (int k = lane; k < C; k += 32) acc = fmaf(x[k], p[k], acc);
 #pragma unroll
       for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     }
@@ -81,11 +84,12 @@ __global__ void __launch_bounds__(128) k_shrink_any(const T* __restrict__ X, con
 
 // Y[m, n] = Σ_k X[m, k]·W(n, k) (+ bias[n]) + Σ_j Q[m, j]·P[a(m), j, n], with
 // W(n, k) = W[n·swn + k·swk]. 64 x 64 tiles, 4 x 4 outputs per thread.
-template <typename T>
-__global__ void __launch_bounds__(256) k_expand_any(const T* __restrict__ X, const T* __restrict__ W, int64_t swn, int64_t swk,
+__global__ void __launch_bounds__(256) k_expand_f32(const float* __restrict__ X, const float* __restrict__ W, int64_t swn, int64_t swk,
                                                     const char* bias, int bias_dtype, const float* __restrict__ Q,
-                                                    const T* __restrict__ P, const int32_t* __restrict__ row_adapter, T* __restrict__ Y,
+                                                    const float* __restrict__ P, const int32_t* __restrict__ row_adapter, float* __restrict__ Y,
                                                     int64_t M, int N, int K, int r) {
+  pdl_trigger();
+  pdl_wait();
   __shared__ float xs[16][64 + 4], ws[16][64 + 4];
   const int64_t m0 = (int64_t)blockIdx.x * 64;
   const int n0 = blockIdx.y * 64, tid = threadIdx.x, tm = (tid >> 4) * 4, tn = (tid & 15) * 4;
@@ -97,11 +101,11 @@ __global__ void __launch_bounds__(256) k_expand_any(const T* __restrict__ X, con
         const int e = tid + 256 * i;
         {
           const int m = e >> 4, k = e & 15;
-          xs[k][m] = (m0 + m < M && k0 + k < K) ? to_f<T>(X[(m0 + m) * K + k0 + k]) : 0.f;
+          xs[k][m] = (m0 + m < M && k0 + k < K) ? X[(m0 + m) * K + k0 + k] : 0.f;
         }
         // the fast index of the load follows W's contiguous axis
         const int n = swk == 1 ? e >> 4 : e & 63, k = swk == 1 ? e & 15 : e >> 6;
-        ws[k][n] = (n0 + n < N && k0 + k < K) ? to_f<T>(W[(n0 + n) * swn + (k0 + k) * swk]) : 0.f;
+        ws[k][n] = (n0 + n < N && k0 + k < K) ? W[(n0 + n) * swn + (k0 + k) * swk] : 0.f;
       }
       __syncthreads();
 #pragma unroll
@@ -127,13 +131,13 @@ __global__ void __launch_bounds__(256) k_expand_any(const T* __restrict__ X, con
       float v = acc[i][j];
       if (bias) v += ld_as<float>(bias, bias_dtype, n);
       if (a >= 0) {
-        const T* p = P + (int64_t)a * r * N + n;
+        const float* p = P + (int64_t)a * r * N + n;
         const float* q = Q + m * r;
         float d = 0.f;
-        for (int l = 0; l < r; l++) d = fmaf(q[l], to_f<T>(p[(int64_t)l * N]), d);
+        for (int l = 0; l < r; l++) d = fmaf(q[l], p[(int64_t)l * N], d);
         v += d;
       }
-      Y[m * N + n] = from_f<T>(v);
+      Y[m * N + n] = v;
     }
   }
 }
@@ -141,9 +145,10 @@ __global__ void __launch_bounds__(256) k_expand_any(const T* __restrict__ X, con
 // dP[a, j, c] = Σ_{t in a} Q[t, j]·X[t, c]: a block per adapter, 8 rank rows
 // and 128 columns; rows in order, in groups of 64 so that a long sum loses no
 // more than a short one.
-template <typename T>
-__global__ void __launch_bounds__(128) k_outer_any(const float* __restrict__ Q, const T* __restrict__ X, const int2* __restrict__ spans,
-                                                   const int32_t* __restrict__ span_ptr, T* __restrict__ dP, int C, int r) {
+__global__ void __launch_bounds__(128) k_outer_f32(const float* __restrict__ Q, const float* __restrict__ X, const int2* __restrict__ spans,
+                                                   const int32_t* __restrict__ span_ptr, float* __restrict__ dP, int C, int r) {
+  pdl_trigger();
+  pdl_wait();
   const int a = blockIdx.z, j0 = blockIdx.y * 8, c = blockIdx.x * 128 + threadIdx.x;
   const int nj = min(8, r - j0);
   float acc[8] = {}, part[8] = {};
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(128) k_outer_any(const float* __restrict__ Q, 
   for (int s = span_ptr[a]; s < span_ptr[a + 1]; s++) {
     const int2 rows = spans[s];
     for (int t = rows.x; t < rows.y; t++) {
-      const float x = c < C ? to_f<T>(X[(int64_t)t * C + c]) : 0.f;
+      const float x = c < C ? X[(int64_t)t * C + c] : 0.f;
       const float* q = Q + (int64_t)t * r + j0;
 #pragma unroll
       for (int j = 0; j < 8; j++)
@@ -166,7 +171,7 @@ __global__ void __launch_bounds__(128) k_outer_any(const float* __restrict__ Q, 
   if (c < C)
 #pragma unroll
     for (int j = 0; j < 8; j++)
-      if (j < nj) dP[((int64_t)a * r + j0 + j) * C + c] = from_f<T>(acc[j] + part[j]);
+      if (j < nj) dP[((int64_t)a * r + j0 + j) * C + c] = acc[j] + part[j];
 }
 
 // ------------------------------------------------------------- operands
@@ -257,41 +262,193 @@ Operands operands(const char* op, lc_tensor xh, lc_tensor dyh, lc_tensor wh, lc_
   return o;
 }
 
-#define LC_FLOAT_SWITCH(dtype, ...)                                        \
-  switch (dtype) {                                                         \
-    case LC_F32: { using T = float; __VA_ARGS__; } break;                  \
-    case LC_F16: { using T = __half; __VA_ARGS__; } break;                 \
-    default: { using T = __nv_bfloat16; __VA_ARGS__; } break;              \
-  }
+// ------------------------------------------------------------- f32 forms
 
-void shrink(const Operands& o, const LcTensor* X, const LcTensor* P, int64_t C, float* Q) {
-  if (!o.T) return;
-  LC_FLOAT_SWITCH(o.dtype, launch_chain(k_shrink_any<T>, dim3((unsigned)o.T), dim3(128), 0, stream(), (const T*)X->data(), (const T*)P->data(),
-                                        o.scale_ptr(), (const int32_t*)o.plan->row_adapter, Q, (int)C, o.r));
+void shrink_f32(const Operands& o, const LcTensor* X, const LcTensor* P, int64_t C, float* Q) {
+  launch_chain(k_shrink_f32, dim3((unsigned)o.T), dim3(128), 0, stream(), (const float*)X->data(), (const float*)P->data(), o.scale_ptr(),
+               (const int32_t*)o.plan->row_adapter, Q, (int)C, o.r);
   LC_LAUNCHED(1);
 }
 
-// y (transposed = false: w [N, K], C_in = K) or dx (transposed = true: C_in = N)
-void expand(const Operands& o, const LcTensor* X, const LcTensor* P, const float* Q, bool transposed, LcTensor* Y) {
-  if (!o.T) return;
+// y (transposed = false) or dx (transposed = true)
+void expand_f32(const Operands& o, const LcTensor* X, const LcTensor* P, const float* Q, bool transposed, LcTensor* Y) {
   const int64_t in = transposed ? o.N : o.K, out = transposed ? o.K : o.N;
   const LcTensor* bias = transposed ? nullptr : o.bias;
   dim3 grid((unsigned)((o.T + 63) / 64), (unsigned)((out + 63) / 64));
   LC_CHECK(grid.y <= 65535, "adapters: too many output columns");
-  LC_FLOAT_SWITCH(o.dtype, launch_chain(k_expand_any<T>, grid, dim3(256), 0, stream(), (const T*)X->data(), o.w ? (const T*)o.w->data() : (const T*)nullptr,
-                                        transposed ? (int64_t)1 : o.K, transposed ? o.K : (int64_t)1, bias ? (const char*)bias->data() : (const char*)nullptr,
-                                        bias ? bias->dtype : 0, Q, (const T*)P->data(), (const int32_t*)o.plan->row_adapter, (T*)Y->data(), o.T,
-                                        (int)out, (int)in, o.r));
+  launch_chain(k_expand_f32, grid, dim3(256), 0, stream(), (const float*)X->data(), o.w ? (const float*)o.w->data() : (const float*)nullptr,
+               transposed ? (int64_t)1 : o.K, transposed ? o.K : (int64_t)1, bias ? (const char*)bias->data() : (const char*)nullptr,
+               bias ? bias->dtype : 0, Q, (const float*)P->data(), (const int32_t*)o.plan->row_adapter, (float*)Y->data(), o.T, (int)out,
+               (int)in, o.r);
   LC_LAUNCHED(1);
 }
 
-void outer(const Operands& o, const float* Q, const LcTensor* X, int64_t C, LcTensor* dP) {
-  if (!o.n) return;
+void outer_f32(const Operands& o, const float* Q, const LcTensor* X, int64_t C, LcTensor* dP) {
   dim3 grid((unsigned)((C + 127) / 128), (unsigned)((o.r + 7) / 8), (unsigned)o.n);
   LC_CHECK(grid.z <= 65535, "adapters: more than 65535 adapters");
-  LC_FLOAT_SWITCH(o.dtype, launch_chain(k_outer_any<T>, grid, dim3(128), 0, stream(), Q, (const T*)X->data(), (const int2*)o.plan->spans,
-                                        (const int32_t*)o.plan->span_ptr, (T*)dP->data(), (int)C, o.r));
+  launch_chain(k_outer_f32, grid, dim3(128), 0, stream(), Q, (const float*)X->data(), (const int2*)o.plan->spans,
+               (const int32_t*)o.plan->span_ptr, (float*)dP->data(), (int)C, o.r);
   LC_LAUNCHED(1);
+}
+
+// ------------------------------------------------------------- 16-bit forms
+
+// A row-major matrix (or a stack of them) whose rows TMA can read.
+struct Rows {
+  const void* p = nullptr;
+  int64_t ld = 0;
+};
+
+// Copies rows of `cols` values into rows of `ld` (a multiple of 8), zeros after them.
+struct PadJob {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t rows, cols, ld;
+};
+struct PadJobs {
+  int n;
+  PadJob j[5];
+};
+__global__ void __launch_bounds__(256) k_pad_rows(const __grid_constant__ PadJobs jobs) {
+  pdl_trigger();
+  pdl_wait();
+  for (int k = 0; k < jobs.n; k++) {
+    const PadJob& j = jobs.j[k];
+    const int64_t vecs = j.ld / 8, total = j.rows * vecs;
+    LC_GRID_STRIDE(i, total) {
+      const int64_t row = i / vecs, c = (i % vecs) * 8;
+      const uint16_t* s = j.src + row * j.cols + c;
+      uint16_t v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = c + e < j.cols ? s[e] : (uint16_t)0;
+      *(uint4*)(j.dst + row * j.ld + c) = *(const uint4*)v;
+    }
+  }
+}
+
+struct Padder {
+  Held& held;
+  PadJobs jobs{};
+  int64_t work = 0;
+  Rows of(const LcTensor* t, int64_t rows, int64_t cols) {
+    if (!t) return {};
+    if (cols % 8 == 0 && ((uintptr_t)t->data() & 15) == 0) return {t->data(), cols};
+    const int64_t ld = (cols + 7) / 8 * 8;
+    void* d = held.scratch((size_t)(rows * ld) * 2);
+    jobs.j[jobs.n++] = {(const uint16_t*)t->data(), (uint16_t*)d, rows, cols, ld};
+    work = std::max(work, rows * ld / 8);
+    return {d, ld};
+  }
+  void run() {
+    if (!jobs.n || !work) return;
+    launch_chain(k_pad_rows, dim3(blocks_for(work, 256)), dim3(256), 0, stream(), jobs);
+    LC_LAUNCHED(1);
+  }
+};
+
+void* shrink_tc(const Operands& o, const Rows& X, const Rows& P, int64_t C, Held& held) {
+  void* Q = held.scratch((size_t)o.T * adapter_u_cols(o.r) * 2);
+  AdapterShrink c;
+  c.X = X.p;
+  c.P = P.p;
+  c.C = C;
+  c.ld = X.ld;
+  c.ldp = P.ld;
+  c.n = o.n;
+  c.rank = o.r;
+  c.scales = o.scale_ptr();
+  c.Q = Q;
+  adapter_shrink_tc(c, *o.plan, o.dtype, stream());
+  return Q;
+}
+
+void expand_tc(const Operands& o, const Rows& X, const Rows& W, const Rows& P, const void* Q, bool transposed, LcTensor* Y) {
+  GemmAdaptedCall c;
+  c.x = X.p;
+  c.M = o.T;
+  c.K = transposed ? o.N : o.K;
+  c.ldx = X.ld;
+  c.w = W.p;
+  c.ldw = W.ld;
+  c.N = transposed ? o.K : o.N;
+  c.transposed = transposed;
+  if (o.bias && !transposed) {
+    c.bias = o.bias->data();
+    c.bias_dtype = o.bias->dtype;
+  }
+  c.y = Y->data();
+  c.ldy = c.N;
+  c.share.u = Q;
+  c.share.u_cols = adapter_u_cols(o.r);
+  c.share.bank = P.p;
+  c.share.n = o.n;
+  c.share.rank = o.r;
+  c.share.ld = P.ld;
+  c.share.segs = o.plan->segs;
+  c.share.tile_first = o.plan->tile_first;
+  c.share.nsegs = o.plan->nsegs;
+  gemm_adapted(c, o.dtype, stream());
+}
+
+void outer_tc(const Operands& o, const void* Q, const Rows& X, int64_t C, LcTensor* dP) {
+  AdapterOuter c;
+  c.X = X.p;
+  c.Q = Q;
+  c.C = C;
+  c.ld = X.ld;
+  c.rank = o.r;
+  c.dP = dP->data();
+  adapter_outer_tc(c, *o.plan, o.dtype, stream());
+}
+
+void linear(const Operands& o, LcTensor* y, Held& held) {
+  if (!o.T) return;
+  if (o.dtype == LC_F32) {
+    float* u = (float*)held.scratch((size_t)o.T * o.r * 4);
+    shrink_f32(o, o.x, o.a, o.K, u);
+    expand_f32(o, o.x, o.b, u, false, y);
+    return;
+  }
+  Padder pad{held};
+  const Rows x = pad.of(o.x, o.T, o.K), w = pad.of(o.w, o.N, o.K), a = pad.of(o.a, (int64_t)o.n * o.r, o.K),
+             b = pad.of(o.b, (int64_t)o.n * o.r, o.N);
+  pad.run();
+  void* u = shrink_tc(o, x, a, o.K, held);
+  expand_tc(o, x, w, b, u, false, y);
+}
+
+void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held& held) {
+  if (!o.T) {
+    for (LcTensor* t : {da, db})
+      if (t && t->numel()) CUDA_OK(cudaMemsetAsync(t->data(), 0, t->numel() * dtype_size(o.dtype), stream()));
+    return;
+  }
+  if (o.dtype == LC_F32) {
+    float* q = (float*)held.scratch((size_t)o.T * o.r * 4);
+    if (dx || da) {
+      shrink_f32(o, o.dy, o.b, o.N, q);
+      if (dx) expand_f32(o, o.dy, o.a, q, true, dx);
+      if (da && o.n) outer_f32(o, q, o.x, o.K, da);
+    }
+    if (db && o.n) {
+      shrink_f32(o, o.x, o.a, o.K, q);
+      outer_f32(o, q, o.dy, o.N, db);
+    }
+    return;
+  }
+  Padder pad{held};
+  const Rows dy = pad.of(o.dy, o.T, o.N), x = da || db ? pad.of(o.x, o.T, o.K) : Rows{}, w = dx ? pad.of(o.w, o.N, o.K) : Rows{},
+             a = dx || db ? pad.of(o.a, (int64_t)o.n * o.r, o.K) : Rows{}, b = dx || da ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : Rows{};
+  pad.run();
+  if (dx || da) {
+    void* g = shrink_tc(o, dy, b, o.N, held);
+    if (dx) expand_tc(o, dy, w, a, g, true, dx);
+    if (da) outer_tc(o, g, x, o.K, da);
+  }
+  if (db) {
+    void* u = shrink_tc(o, x, a, o.K, held);
+    outer_tc(o, u, dy, o.N, db);
+  }
 }
 
 }  // namespace
@@ -325,7 +482,7 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
     if (!segs.empty() && segs.back().a == adapters[i] && segs.back().hi == cu_rows[i]) segs.back().hi = cu_rows[i + 1];
     else segs.push_back({cu_rows[i], cu_rows[i + 1], adapters[i]});
   }
-  // device image: adapter of each row | spans by adapter | where each adapter's spans start
+  // the arrays of AdapterPlan in one device allocation
   const size_t S = segs.size();
   std::vector<int32_t> span_ptr(n_adapters + 1, 0);
   for (auto& s : segs) span_ptr[s.a + 1]++;
@@ -338,6 +495,19 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   }
   std::vector<int32_t> row_adapter(T, -1);
   for (auto& s : segs) std::fill(row_adapter.begin() + s.lo, row_adapter.begin() + s.hi, s.a);
+  std::vector<int32_t> seg4, tile_first((T + 127) / 128);
+  for (auto& g : segs) seg4.insert(seg4.end(), {g.lo, g.hi, g.a, 0});
+  for (size_t i = 0, k = 0; i < tile_first.size(); i++) {
+    while (k < S && segs[k].hi <= (int64_t)i * 128) k++;
+    tile_first[i] = (int32_t)k;
+  }
+  std::vector<int32_t> chunks, chunk_ptr(n_adapters + 1, 0);
+  for (int a = 0; a < n_adapters; a++) {
+    for (int k = span_ptr[a]; k < span_ptr[a + 1]; k++)
+      for (int64_t t = spans[2 * k]; t < spans[2 * k + 1]; t += 64)
+        chunks.insert(chunks.end(), {(int32_t)t, (int32_t)std::min<int64_t>(64, spans[2 * k + 1] - t), a, 0});
+    chunk_ptr[a + 1] = (int32_t)(chunks.size() / 4);
+  }
   std::vector<int32_t> image;
   auto put = [&](const std::vector<int32_t>& v) {
     const size_t off = image.size();
@@ -345,7 +515,8 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
     image.resize((image.size() + 63) / 64 * 64);
     return off;
   };
-  const size_t o_rows = put(row_adapter), o_spans = put(spans), o_ptr = put(span_ptr);
+  const size_t o_rows = put(row_adapter), o_spans = put(spans), o_ptr = put(span_ptr), o_segs = put(seg4), o_first = put(tile_first),
+               o_chunks = put(chunks), o_chunk_ptr = put(chunk_ptr);
   struct Guard {
     AdapterPlan* p;
     ~Guard() { if (p) plan_release(p); }
@@ -353,7 +524,8 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   AdapterPlan* p = g.p;
   p->rows = T;
   p->n_adapters = n_adapters;
-  p->nspans = (int)S;
+  p->nsegs = (int)S;
+  p->nchunks = (int)(chunks.size() / 4);
   p->built_on = st;
   CUDA_OK(cudaEventCreateWithFlags(&p->built, cudaEventDisableTiming));
   p->dev = (int32_t*)dmalloc(image.size() * 4);
@@ -363,6 +535,10 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   p->row_adapter = p->dev + o_rows;
   p->spans = (int2*)(p->dev + o_spans);
   p->span_ptr = p->dev + o_ptr;
+  p->segs = (int4*)(p->dev + o_segs);
+  p->tile_first = p->dev + o_first;
+  p->chunks = (int4*)(p->dev + o_chunks);
+  p->chunk_ptr = p->dev + o_chunk_ptr;
   plans().insert(p);
   g.p = nullptr;
   *out = reinterpret_cast<uint64_t>(p);
@@ -386,9 +562,7 @@ int lc_adapter_linear(lc_tensor* out, lc_tensor xh, lc_tensor wh, lc_tensor bias
   std::vector<int64_t> shape = check(xh, "adapter_linear")->dims();
   shape.back() = o.N;
   LcTensor* y = held.made(alloc(o.dtype, shape));
-  float* u = (float*)held.scratch((size_t)o.T * o.r * 4);
-  shrink(o, o.x, o.a, o.K, u);
-  expand(o, o.x, o.b, u, false, y);
+  linear(o, y, held);
   *out = handle(held.keep(y));
   LC_API_END
 }
@@ -403,17 +577,7 @@ int lc_adapter_linear_grad(lc_tensor* dxo, lc_tensor* dao, lc_tensor* dbo, lc_te
   if (dxo) dx = held.made(alloc(o.dtype, check(xh, "adapter_linear_grad")->dims()));
   if (dao) da = held.made(alloc(o.dtype, o.a->dims()));
   if (dbo) db = held.made(alloc(o.dtype, o.b->dims()));
-  if (dx || da) {
-    float* g = (float*)held.scratch((size_t)o.T * o.r * 4);
-    shrink(o, o.dy, o.b, o.N, g);
-    if (dx) expand(o, o.dy, o.a, g, true, dx);
-    if (da) outer(o, g, o.x, o.K, da);
-  }
-  if (db) {
-    float* u = (float*)held.scratch((size_t)o.T * o.r * 4);
-    shrink(o, o.x, o.a, o.K, u);
-    outer(o, u, o.dy, o.N, db);
-  }
+  gradients(o, dx, da, db, held);
   if (dx) *dxo = handle(held.keep(dx));
   if (da) *dao = handle(held.keep(da));
   if (db) *dbo = handle(held.keep(db));

@@ -6,15 +6,43 @@ constexpr int kAdapterMaxRank = 256;
 
 // Rows and adapters of one batch on the device (lc_adapter_plan_create).
 struct AdapterPlan {
-  int rows = 0, n_adapters = 0, nspans = 0;
+  int rows = 0, n_adapters = 0, nsegs = 0, nchunks = 0;
   int32_t* dev = nullptr;          // one allocation behind the arrays below
   int32_t* row_adapter = nullptr;  // [rows]: the adapter of each row, -1 = none
-  int2* spans = nullptr;           // [nspans]: row ranges, adapter by adapter, ascending within one
+  int4* segs = nullptr;            // [nsegs]: row ranges with an adapter, ascending: lo, hi, adapter
+  int32_t* tile_first = nullptr;   // per 128 rows: the first segment that ends after the first of them
+  int2* spans = nullptr;           // [nsegs]: the row ranges adapter by adapter, ascending within one
   int32_t* span_ptr = nullptr;     // [n_adapters + 1]: where each adapter's spans start
+  int4* chunks = nullptr;          // [nchunks]: the spans in blocks of at most 64 rows: row, rows, adapter
+  int32_t* chunk_ptr = nullptr;    // [n_adapters + 1]: where each adapter's blocks start
   cudaStream_t built_on = nullptr;
   cudaEvent_t built = nullptr;     // the arrays are on the device
   bool settled = false;            // `built` has been seen complete
   bool shared = false;             // used on another stream than built_on
 };
+
+// 16-bit columns of a row of Q (lc_adapters_tc.cu): two parts of the rank
+// rounded up to 16, or to 64 above 32, where a part fills whole 128-byte rows.
+inline int adapter_u_cols(int rank) { return 2 * (rank <= 32 ? (rank + 15) / 16 * 16 : (rank + 63) / 64 * 64); }
+
+// Q[t] = s_a·P_a·X[t] for X [rows, C] and P [n, rank, C] (row strides ld, ldp: multiples of 8; 16-byte aligned).
+struct AdapterShrink {
+  const void *X = nullptr, *P = nullptr;
+  int64_t C = 0, ld = 0, ldp = 0;
+  int n = 0, rank = 0;
+  const float* scales = nullptr;
+  void* Q = nullptr;
+};
+// dP[a] = Σ_{t in a} Q[t] ⊗ X[t], [n, rank, C] dense.
+struct AdapterOuter {
+  const void *X = nullptr, *Q = nullptr;
+  int64_t C = 0, ld = 0;
+  int rank = 0;
+  void* dP = nullptr;
+};
+namespace lc {
+void adapter_shrink_tc(const AdapterShrink& c, const AdapterPlan& p, int dtype, cudaStream_t st);
+void adapter_outer_tc(const AdapterOuter& c, const AdapterPlan& p, int dtype, cudaStream_t st);
+}  // namespace lc
 
 void lc_adapters_destroy();

@@ -896,6 +896,7 @@ int lc_copy_into(lc_tensor dsth, lc_tensor srch) {
 void lc_internal_wait_limit_gemm(unsigned long long ns);
 void lc_internal_wait_limit_attention(unsigned long long ns);
 void lc_internal_wait_limit_encoder(unsigned long long ns);
+void lc_internal_wait_limit_adapters(unsigned long long ns);
 void lc_internal_launch_wait_probe();
 
 extern "C" {
@@ -907,6 +908,7 @@ int lc_debug_set_wait_limit(uint64_t ns) {
   lc_internal_wait_limit_gemm(v);
   lc_internal_wait_limit_attention(v);
   lc_internal_wait_limit_encoder(v);
+  lc_internal_wait_limit_adapters(v);
   LC_API_END
 }
 

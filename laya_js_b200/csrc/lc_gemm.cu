@@ -55,6 +55,36 @@ struct GemmArgs {
   GemmQuantB q;  // QB: the packed weight (tmB maps its bytes)
 };
 
+// What a GEMM accumulates after its main loop. GemmPlain: nothing.
+struct GemmPlain {
+  static constexpr bool kOn = false, kWT = false;
+  static constexpr int kb_off = 0;
+};
+// The adapters' share of a projection: for each segment of rows [lo, hi) with
+// adapter a that meets the tile, D[rows] += U·P_a, U [M, 64·nchunks] and P_a
+// [r, N]. U rides as the A operand (the tile's rows, 64 columns per block of
+// the ring) and P_a, whose rows run along N, as an MN-major B operand; the MMA
+// leaves the rows outside the segment alone (TMEM lanes switched off), so a
+// row never meets another request's adapter, not even multiplied by zero.
+// U holds each value as a 16-bit high part and the 16-bit remainder, which
+// meet the same rows of P_a: the sum is as exact as an f32 u.
+// WT: the shared projection is read transposed, D = X·W for W [K, N] (the
+// gradient with respect to the input): an MN-major B operand as well.
+template <bool WT>
+struct GemmAdapted {
+  static constexpr bool kOn = true, kWT = WT;
+  CUtensorMap tmU, tmP;
+  const int4* segs;           // lo, hi, adapter
+  const int32_t* tile_first;  // per 128 rows: the first segment that ends after the first of them
+  int nsegs;
+  int nchunks;                // 64-column blocks of U
+  int ksteps;                 // 16-column steps used per block
+  int half;                   // steps after which P's rows start over (high and low part in one block), else ksteps
+  int pgroups;                // 64-row blocks of P_a
+  int prows;                  // rows of P_a per block (box height of tmP)
+  int kb_off;                 // added to the K block of the main loop's loads (past the operands' end: zeros)
+};
+
 __device__ __forceinline__ float gelu_exact(float x) { return 0.5f * x * (1.0f + erff(x * 0.7071067811865476f)); }
 
 template <typename T>
@@ -860,10 +890,13 @@ __device__ __forceinline__ void epilogue_split(const GemmArgs& args, const CUten
 // conv[stage], which the MMA issuer waits for as well. The packed weight is
 // resident, so its first blocks are requested and converted before the
 // dependency wait. One unit of work per CTA.
-template <typename T, int BN, int STAGES, bool TMAE, bool KS = false, bool QB = false>
+// EX: what is accumulated after the main loop (GemmPlain, GemmAdapted); with
+// split K the last slice takes it.
+template <typename T, int BN, int STAGES, bool TMAE, bool KS = false, bool QB = false, typename EX = GemmPlain>
 __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                                                     const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmR,
-                                                    const __grid_constant__ GemmArgs args) {
+                                                    const __grid_constant__ GemmArgs args, const __grid_constant__ EX ex) {
+  static_assert(!(EX::kOn && QB), "adapters beside a packed weight are added to a separate product");
   static_assert(!KS || TMAE, "split K runs with the TMA-store epilogue");
   extern __shared__ uint8_t smem_raw[];
   constexpr uint32_t A_BYTES = BM * BK * 2;
@@ -999,12 +1032,34 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           } else {
             if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
             mbar_arrive_expect_tx(&full[stage], A_BYTES + B_BYTES);
-            tma_load_2d(sA + stage * A_BYTES, &tmA, &full[stage], kb * BK, m0);
-            tma_load_2d(sB + stage * B_BYTES, &tmB, &full[stage], kb * BK, n0);
+            const int kx = (kb + ex.kb_off) * BK;
+            tma_load_2d(sA + stage * A_BYTES, &tmA, &full[stage], kx, m0);
+            if constexpr (EX::kWT) {
+              for (int h = 0; h < BN / 64; h++) tma_load_2d(sB + stage * B_BYTES + h * 8192, &tmB, &full[stage], n0 + 64 * h, kx);
+            } else {
+              tma_load_2d(sB + stage * B_BYTES, &tmB, &full[stage], kx, n0);
+            }
           }
           issued[stage] = 1;
           iss_phase[stage] = phase;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if constexpr (EX::kOn) {
+          if (kb1 < KB) continue;  // another slice of K takes the adapters
+          for (int s = __ldg(ex.tile_first + m0 / BM); s < ex.nsegs && ok; s++) {
+            const int4 seg = __ldg(ex.segs + s);
+            if (seg.x >= m0 + BM) break;
+            for (int c = 0; c < ex.nchunks; c++) {
+              if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
+              mbar_arrive_expect_tx(&full[stage], A_BYTES + (BN / 64) * ex.prows * 128);
+              tma_load_2d(sA + stage * A_BYTES, &ex.tmU, &full[stage], c * 64, m0);
+              for (int h = 0; h < BN / 64; h++)
+                tma_load_3d(sB + stage * B_BYTES + h * 8192, &ex.tmP, &full[stage], n0 + 64 * h, (c % ex.pgroups) * 64, seg.z);
+              issued[stage] = 1;
+              iss_phase[stage] = phase;
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+          }
         }
       }
       // drain: every copy this thread issued must have landed before the CTA exits
@@ -1023,6 +1078,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
     // ---------------- MMA issuer
     if (lane == 0) {
       const uint32_t idesc = idesc_f16<T, BN>();
+      [[maybe_unused]] const uint32_t idesc_t = idesc_f16<T, BN, 128, true>();
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -1042,13 +1098,36 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           tc_fence_after();
           const uint32_t a0 = smem_u32(sA + stage * A_BYTES), b0 = smem_u32(sB + stage * B_BYTES);
 #pragma unroll
-          for (int k = 0; k < BK / 16; k++)
-            tc_mma(d, sdesc_sw128(a0 + k * 32), sdesc_sw128(b0 + k * 32), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < BK / 16; k++) {
+            if constexpr (EX::kWT) tc_mma(d, sdesc_sw128(a0 + k * 32), sdesc_sw128_mn(b0 + k * 2048, 8192), idesc_t, (kb > kb0 || k > 0) ? 1u : 0u);
+            else tc_mma(d, sdesc_sw128(a0 + k * 32), sdesc_sw128(b0 + k * 32), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          }
           tc_commit(&empty[stage]);
           committed = true;
           last = &empty[stage];
           last_phase = phase;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if constexpr (EX::kOn) {
+          const int m0 = ((w / S) / args.ntile_n) * BM;
+          for (int s = kb1 < KB ? ex.nsegs : __ldg(ex.tile_first + m0 / BM); s < ex.nsegs && ok; s++) {
+            const int4 seg = __ldg(ex.segs + s);
+            if (seg.x >= m0 + BM) break;
+            uint32_t off[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) off[i] = lanes_off(m0 + 32 * i, seg.x, seg.y);
+            for (int c = 0; c < ex.nchunks; c++) {
+              if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
+              tc_fence_after();
+              const uint32_t a0 = smem_u32(sA + stage * A_BYTES), b0 = smem_u32(sB + stage * B_BYTES);
+              for (int k = 0; k < ex.ksteps; k++)
+                tc_mma_lanes(d, sdesc_sw128(a0 + k * 32), sdesc_sw128_mn(b0 + (k >= ex.half ? k - ex.half : k) * 2048, 8192), idesc_t, 1u, off);
+              tc_commit(&empty[stage]);
+              last = &empty[stage];
+              last_phase = phase;
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+          }
         }
         if (!ok) break;
         tc_commit(&tfull[acc]);
@@ -1188,10 +1267,10 @@ constexpr size_t gemm_pair_smem_bytes() {
   return (size_t)STAGES * (BM * BK * 2 + 128 * BK * 2) + PAIR_EPI_WARPS * PAIR_NBUF * 4096 + 1024 + 512;
 }
 
-template <typename T, int STAGES>
+template <typename T, int STAGES, typename EX = GemmPlain>
 __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                                                            const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmR,
-                                                           const __grid_constant__ GemmArgs args) {
+                                                           const __grid_constant__ GemmArgs args, const __grid_constant__ EX ex) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int BN = 256;
   constexpr uint32_t A_BYTES = BM * BK * 2;
@@ -1258,11 +1337,33 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
         for (int kb = 0; kb < KB; kb++) {
           if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (A_BYTES + B_BYTES));
-          tma_load_2d_pair(sA + stage * A_BYTES, &tmA, full0 + 8 * stage, kb * BK, m0);
-          tma_load_2d_pair(sB + stage * B_BYTES, &tmB, full0 + 8 * stage, kb * BK, n0);
+          const int kx = (kb + ex.kb_off) * BK;
+          tma_load_2d_pair(sA + stage * A_BYTES, &tmA, full0 + 8 * stage, kx, m0);
+          if constexpr (EX::kWT) {
+            for (int h = 0; h < 2; h++) tma_load_2d_pair(sB + stage * B_BYTES + h * 8192, &tmB, full0 + 8 * stage, n0 + 64 * h, kx);
+          } else {
+            tma_load_2d_pair(sB + stage * B_BYTES, &tmB, full0 + 8 * stage, kx, n0);
+          }
           issued[stage] = 1;
           iss_phase[stage] = phase;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if constexpr (EX::kOn) {
+          const int t0 = (t / args.ntile_n) * (2 * BM);
+          for (int s = __ldg(ex.tile_first + t0 / BM); s < ex.nsegs && ok; s++) {
+            const int4 seg = __ldg(ex.segs + s);
+            if (seg.x >= t0 + 2 * BM) break;
+            for (int c = 0; c < ex.nchunks; c++) {
+              if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
+              if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (A_BYTES + 2 * ex.prows * 128));
+              tma_load_2d_pair(sA + stage * A_BYTES, &ex.tmU, full0 + 8 * stage, c * 64, m0);
+              for (int h = 0; h < 2; h++)
+                tma_load_3d_pair(sB + stage * B_BYTES + h * 8192, &ex.tmP, full0 + 8 * stage, n0 + 64 * h, (c % ex.pgroups) * 64, seg.z);
+              issued[stage] = 1;
+              iss_phase[stage] = phase;
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+          }
         }
       }
       // drain: each stage's last fill has been consumed by the pair's MMAs (so it landed)
@@ -1279,6 +1380,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = idesc_f16<T, BN, 256>();
       const uint64_t dA0 = sdesc_sw128(smem_u32(sA)), dB0 = sdesc_sw128(smem_u32(sB));
+      [[maybe_unused]] const uint32_t idesc_t = idesc_f16<T, BN, 256, true>();
+      [[maybe_unused]] const uint64_t dBt0 = sdesc_sw128_mn(smem_u32(sB), 8192);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -1295,11 +1398,35 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
           tc_fence_after();
           const uint64_t da = dA0 + ((stage * A_BYTES) >> 4), db = dB0 + ((stage * B_BYTES) >> 4);
 #pragma unroll
-          for (int k = 0; k < BK / 16; k++) tc_mma_pair(d, da + k * 2, db + k * 2, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < BK / 16; k++) {
+            if constexpr (EX::kWT) tc_mma_pair(d, da + k * 2, dBt0 + ((stage * B_BYTES) >> 4) + k * 128, idesc_t, (kb > 0 || k > 0) ? 1u : 0u);
+            else tc_mma_pair(d, da + k * 2, db + k * 2, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          }
           tc_commit_pair(&empty[stage]);
           last = &empty[stage];
           last_phase = phase;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if constexpr (EX::kOn) {
+          const int t0 = (t / args.ntile_n) * (2 * BM);
+          for (int s = __ldg(ex.tile_first + t0 / BM); s < ex.nsegs && ok; s++) {
+            const int4 seg = __ldg(ex.segs + s);
+            if (seg.x >= t0 + 2 * BM) break;
+            uint32_t off[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) off[i] = lanes_off(t0 + 32 * i, seg.x, seg.y);
+            for (int c = 0; c < ex.nchunks; c++) {
+              if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
+              tc_fence_after();
+              const uint64_t da = dA0 + ((stage * A_BYTES) >> 4), db = dBt0 + ((stage * B_BYTES) >> 4);
+              for (int k = 0; k < ex.ksteps; k++)
+                tc_mma_pair_lanes(d, da + k * 2, db + (k >= ex.half ? k - ex.half : k) * 128, idesc_t, 1u, off);
+              tc_commit_pair(&empty[stage]);
+              last = &empty[stage];
+              last_phase = phase;
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+          }
         }
         if (!ok) break;
         tc_commit_pair(&tfull[acc]);
@@ -1389,29 +1516,29 @@ CUtensorMap tensor_map_u8(const void* ptr, int64_t rows, int64_t cols, int box_c
   return c.emplace(key, m).first->second;
 }
 
-template <typename T, int BN, int STAGES, bool TMAE>
+template <typename T, int BN, int STAGES, bool TMAE, typename EX = GemmPlain>
 void launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my, const CUtensorMap& mr, const GemmArgs& a,
-                 cudaStream_t st) {
+                 cudaStream_t st, const EX& ex = EX()) {
   constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(TMAE);
   static_assert(smem <= 232448, "GEMM shared memory above the 227 KB per-CTA limit");
   static bool attr = false;
   if (!attr) {
-    CUDA_OK(cudaFuncSetAttribute(k_gemm_tc<T, BN, STAGES, TMAE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CUDA_OK(cudaFuncSetAttribute(k_gemm_tc<T, BN, STAGES, TMAE, false, false, EX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attr = true;
   }
   int grid = std::min(a.ntiles, lc::num_sms());
-  lc::launch_chain(k_gemm_tc<T, BN, STAGES, TMAE>, dim3(grid), dim3(GEMM_THREADS), smem, st, ma, mb, my, mr, a);
+  lc::launch_chain(k_gemm_tc<T, BN, STAGES, TMAE, false, false, EX>, dim3(grid), dim3(GEMM_THREADS), smem, st, ma, mb, my, mr, a, ex);
 }
 
 // Split K: clusters of a.ksplit CTAs, one cluster per tile while they fit
 // (QB: the packed-weight instance).
-template <typename T, int BN, int STAGES, bool QB = false>
+template <typename T, int BN, int STAGES, bool QB = false, typename EX = GemmPlain>
 cudaLaunchConfig_t split_config(int S, cudaLaunchAttribute* at, cudaStream_t st) {
   constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(true, true, QB);
   static_assert(smem <= 232448, "GEMM shared memory above the 227 KB per-CTA limit");
   static bool attr = false;
   if (!attr) {
-    CUDA_OK(cudaFuncSetAttribute(k_gemm_tc<T, BN, STAGES, true, true, QB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CUDA_OK(cudaFuncSetAttribute(k_gemm_tc<T, BN, STAGES, true, true, QB, EX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attr = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -1426,31 +1553,31 @@ cudaLaunchConfig_t split_config(int S, cudaLaunchAttribute* at, cudaStream_t st)
   return cfg;
 }
 // clusters of S of this instance that can be resident at once
-template <typename T, int BN, int STAGES, bool QB = false>
+template <typename T, int BN, int STAGES, bool QB = false, typename EX = GemmPlain>
 int split_capacity(int S) {
   static int cap[5] = {0, 0, 0, 0, 0};
   if (!cap[S]) {
     cudaLaunchAttribute at[2];
-    cudaLaunchConfig_t cfg = split_config<T, BN, STAGES, QB>(S, at, nullptr);
+    cudaLaunchConfig_t cfg = split_config<T, BN, STAGES, QB, EX>(S, at, nullptr);
     cfg.gridDim = dim3(S * (lc::num_sms() / S));
     int n = 0;
-    CUDA_OK(cudaOccupancyMaxActiveClusters(&n, k_gemm_tc<T, BN, STAGES, true, true, QB>, &cfg));
+    CUDA_OK(cudaOccupancyMaxActiveClusters(&n, k_gemm_tc<T, BN, STAGES, true, true, QB, EX>, &cfg));
     LC_CHECK(n > 0, "tcgen05 GEMM: no split-K cluster fits");
     cap[S] = n;
   }
   return cap[S];
 }
-template <typename T, int BN, int STAGES, bool QB = false>
+template <typename T, int BN, int STAGES, bool QB = false, typename EX = GemmPlain>
 void launch_gemm_split(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my, const CUtensorMap& mr, const GemmArgs& a,
-                       cudaStream_t st) {
+                       cudaStream_t st, const EX& ex = EX()) {
   const int S = a.ksplit;
   LC_CHECK(S == 1 || S == 2 || S == 4, "tcgen05 GEMM: split-K factor must be 1, 2 or 4");
   cudaLaunchAttribute at[2];
-  cudaLaunchConfig_t cfg = split_config<T, BN, STAGES, QB>(S, at, st);
-  const int cap = split_capacity<T, BN, STAGES, QB>(S);
+  cudaLaunchConfig_t cfg = split_config<T, BN, STAGES, QB, EX>(S, at, st);
+  const int cap = split_capacity<T, BN, STAGES, QB, EX>(S);
   LC_CHECK((S == 1 && !QB) || a.ntiles <= cap, "tcgen05 GEMM: split K needs one resident cluster per tile");
   cfg.gridDim = dim3(S * std::min(a.ntiles, cap));
-  CUDA_OK(cudaLaunchKernelEx(&cfg, k_gemm_tc<T, BN, STAGES, true, true, QB>, ma, mb, my, mr, a));
+  CUDA_OK(cudaLaunchKernelEx(&cfg, k_gemm_tc<T, BN, STAGES, true, true, QB, EX>, ma, mb, my, mr, a, ex));
 }
 int split_capacity_for(int dtype, int BN, int S, bool qb = false) {
   if (qb) {
@@ -1461,8 +1588,9 @@ int split_capacity_for(int dtype, int BN, int S, bool qb = false) {
   return BN == 64 ? split_capacity<__nv_bfloat16, 64, 4>(S) : split_capacity<__nv_bfloat16, 128, 3>(S);
 }
 
-template <typename T, int STAGES>
-void launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my, const CUtensorMap& mr, GemmArgs a, cudaStream_t st) {
+template <typename T, int STAGES, typename EX = GemmPlain>
+void launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my, const CUtensorMap& mr, GemmArgs a, cudaStream_t st,
+                      const EX& ex = EX()) {
   constexpr size_t smem = gemm_pair_smem_bytes<STAGES>();
   static_assert(smem <= 232448, "GEMM shared memory above the 227 KB per-CTA limit");
   static int max_pairs = 0;
@@ -1477,16 +1605,16 @@ void launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtens
   cfg.stream = st;
   lc::chain_attrs(cfg, at, 1);
   if (!max_pairs) {
-    CUDA_OK(cudaFuncSetAttribute(k_gemm_pair<T, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CUDA_OK(cudaFuncSetAttribute(k_gemm_pair<T, STAGES, EX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cfg.gridDim = dim3(2 * (lc::num_sms() / 2));
     int n = 0;
-    CUDA_OK(cudaOccupancyMaxActiveClusters(&n, k_gemm_pair<T, STAGES>, &cfg));
+    CUDA_OK(cudaOccupancyMaxActiveClusters(&n, k_gemm_pair<T, STAGES, EX>, &cfg));
     LC_CHECK(n > 0, "tcgen05 GEMM: no CTA pair fits an SM pair");
     max_pairs = n;
   }
   const int pairs = std::min(a.ntiles, max_pairs);
   cfg.gridDim = dim3(2 * pairs);
-  CUDA_OK(cudaLaunchKernelEx(&cfg, k_gemm_pair<T, STAGES>, ma, mb, my, mr, a));
+  CUDA_OK(cudaLaunchKernelEx(&cfg, k_gemm_pair<T, STAGES, EX>, ma, mb, my, mr, a, ex));
 }
 
 }  // namespace
@@ -1614,6 +1742,101 @@ bool gemm_raw(const void* x, int64_t M, int64_t K, const void* w, int64_t N, con
   return true;
 }
 
+namespace {
+// Boxes of 64 columns x box_rows of a stack of row-major [rows, cols] matrices with row stride ld.
+CUtensorMap tensor_map_stack(const void* ptr, int64_t n, int64_t rows, int64_t cols, int64_t ld, int box_rows, int dtype) {
+  CUtensorMap m;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)n};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(rows * ld) * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  CUresult r = encode_fn()(&m, dtype == LC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(ptr),
+                           dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  LC_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return m;
+}
+
+template <typename T, bool WT>
+void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
+  const int dtype = std::is_same<T, __half>::value ? LC_F16 : LC_BF16;
+  GemmArgs a{};
+  a.M = (int)c.M;
+  a.N = (int)c.N;
+  a.K = c.w ? (int)c.K : 1;  // without a projection: one K block of zeros
+  a.y = c.y;
+  a.ldy = c.ldy;
+  a.vec_ok = (c.ldy % 8 == 0 && ((uintptr_t)c.y & 15) == 0) ? 1 : 0;
+  a.bias = c.bias;
+  a.bias_dtype = c.bias_dtype;
+  a.ksplit = 1;
+  GemmAdapted<WT> ex{};
+  const AdapterShare& s = c.share;
+  ex.tmU = tensor_map(s.u, c.M, s.u_cols, s.u_cols, 64, BM, dtype);
+  ex.prows = std::min(64, s.u_cols / 2);  // rows past the rank arrive as zeros
+  ex.tmP = tensor_map_stack(s.bank, std::max(1, s.n), s.rank, c.N, s.ld, ex.prows, dtype);
+  ex.segs = s.segs;
+  ex.tile_first = s.tile_first;
+  ex.nsegs = s.nsegs;
+  ex.nchunks = (s.u_cols + 63) / 64;
+  ex.ksteps = std::min(4, s.u_cols / 16);
+  ex.half = s.u_cols <= 64 ? s.u_cols / 32 : 4;
+  ex.pgroups = std::max(1, s.u_cols / 128);
+  ex.kb_off = c.w ? 0 : 1;  // a block past the end of the stand-in maps below, which TMA fills with zeros
+  const CUtensorMap ma = c.w ? tensor_map(c.x, c.M, c.K, c.ldx, BK, BM, dtype) : tensor_map(s.u, 1, 8, 8, BK, BM, dtype);
+  auto weight_map = [&](int bn) {
+    if (!c.w) return WT ? tensor_map(s.u, 1, 8, 8, 64, 64, dtype) : tensor_map(s.u, 1, 8, 8, BK, bn, dtype);
+    return WT ? tensor_map(c.w, c.K, c.N, c.ldw, 64, 64, dtype) : tensor_map(c.w, c.N, c.K, c.ldw, BK, bn, dtype);
+  };
+  const bool tmae = a.vec_ok && c.N % 8 == 0;
+  const int sms = num_sms();
+  const int64_t mt = (c.M + BM - 1) / BM;
+  auto tiles = [&](int bn) { return mt * ((c.N + bn - 1) / bn); };
+  LC_CHECK(tiles(64) <= INT32_MAX, "adapters: too many output tiles");
+  auto shape = [&](int bn) {
+    a.ntile_n = (int)((c.N + bn - 1) / bn);
+    a.ntiles = (int)tiles(bn);
+  };
+  if (tmae && (c.N <= 64 || tiles(128) * 2 <= sms)) {
+    // few columns or few rows: narrow tiles, K split over clusters (as in gemm_raw)
+    const int KB = (a.K + BK - 1) / BK;
+    int S = 1;
+    for (int f : {4, 2})
+      if (tiles(64) * f <= sms && KB >= f && tiles(64) <= split_capacity<T, 64, 4, false, GemmAdapted<WT>>(f)) {
+        S = f;
+        break;
+      }
+    shape(64);
+    a.ksplit = S;
+    const CUtensorMap my = tensor_map(c.y, c.M, c.N, c.ldy, 64, S > 1 ? 4 : 32, dtype);
+    launch_gemm_split<T, 64, 4, false, GemmAdapted<WT>>(ma, weight_map(64), my, my, a, st, ex);
+  } else if (tmae && c.N > 128 && tiles(256) >= sms) {
+    shape(256);
+    a.ntiles = (int)(((c.M + 2 * BM - 1) / (2 * BM)) * a.ntile_n);
+    const CUtensorMap my = tensor_map(c.y, c.M, c.N, c.ldy, 64, 32, dtype);
+    launch_gemm_pair<T, 5, GemmAdapted<WT>>(ma, weight_map(128), my, my, a, st, ex);
+  } else {
+    shape(128);
+    if (tmae) {
+      const CUtensorMap my = tensor_map(c.y, c.M, c.N, c.ldy, 64, 32, dtype);
+      launch_gemm<T, 128, 6, true, GemmAdapted<WT>>(ma, weight_map(128), my, my, a, st, ex);
+    } else {
+      launch_gemm<T, 128, 6, false, GemmAdapted<WT>>(ma, weight_map(128), ma, ma, a, st, ex);
+    }
+  }
+  LC_LAUNCHED(1);
+}
+}  // namespace
+
+void gemm_adapted(const GemmAdaptedCall& c, int dtype, cudaStream_t st) {
+  if (dtype == LC_F16) c.transposed ? launch_adapted<__half, true>(c, st) : launch_adapted<__half, false>(c, st);
+  else c.transposed ? launch_adapted<__nv_bfloat16, true>(c, st) : launch_adapted<__nv_bfloat16, false>(c, st);
+}
+
+CUtensorMap tensor_map_3d(const void* ptr, int64_t n, int64_t rows, int64_t cols, int64_t ld, int box_rows, int dtype) {
+  return tensor_map_stack(ptr, n, rows, cols, ld, box_rows, dtype);
+}
+
 // In-kernel dequantisation for few rows; LAYA_CUDA_QGEMM_FUSED=0 makes
 // gemm_raw_q decline (the caller then dequantises into a dense scratch).
 bool gemm_use_qfused() {
@@ -1711,7 +1934,7 @@ bool gemm_linear(const LcTensor* x2, const LcTensor* w, const LcTensor* bias, Lc
 std::string take_device_errors() {
   unsigned int e = 0, z = 0;
   CUDA_OK(cudaMemcpyFromSymbol(&e, g_gemm_err, sizeof(e)));
-  std::string msg = take_attention_errors();
+  std::string msg = take_attention_errors() + take_adapter_errors();
   if (!e) return msg;
   CUDA_OK(cudaMemcpyToSymbol(g_gemm_err, &z, sizeof(z)));
   std::string what = (e & 1u) ? "a pipeline wait timed out (kernel aborted its tile loop)" : "a split-K launch had more tiles than clusters";

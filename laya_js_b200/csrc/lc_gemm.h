@@ -51,7 +51,37 @@ struct GemmQuantB {
   const float* gamma = nullptr;  // optional column scale [K] (a folded LayerNorm weight)
 };
 
+// The adapters' share that gemm_adapted adds to a projection.
+struct AdapterShare {
+  const void* u = nullptr;     // [M, u_cols] 16-bit: high parts (u_cols / 2), then the remainders
+  int u_cols = 0;              // 32, 64 or a multiple of 128
+  const void* bank = nullptr;  // [n, rank, ld] 16-bit, ld % 8 == 0
+  int n = 0, rank = 0;
+  int64_t ld = 0;
+  const int4* segs = nullptr;  // row ranges with an adapter, ascending: lo, hi, adapter
+  const int32_t* tile_first = nullptr;
+  int nsegs = 0;
+};
+// y[M, N] = x·wᵀ for w [N, K], or x·w for w [K, N] (transposed), plus bias and
+// the adapters' share; w null: the share alone. Rows of x, w and the bank are
+// 16-byte aligned (ldx, ldw % 8 == 0); any M, N and K.
+struct GemmAdaptedCall {
+  const void* x = nullptr;
+  int64_t M = 0, K = 0, ldx = 0;
+  const void* w = nullptr;
+  int64_t ldw = 0, N = 0;
+  bool transposed = false;
+  const void* bias = nullptr;
+  int bias_dtype = 0;
+  void* y = nullptr;
+  int64_t ldy = 0;
+  AdapterShare share;
+};
+
 namespace lc {
+void gemm_adapted(const GemmAdaptedCall& c, int dtype, cudaStream_t st);
+// Tensor map over n row-major [rows, cols] matrices (row stride ld), boxes of 64 columns x box_rows (128-byte swizzle).
+CUtensorMap tensor_map_3d(const void* ptr, int64_t n, int64_t rows, int64_t cols, int64_t ld, int box_rows, int dtype);
 // y[M, N] = x[M, K] · w[N, K]ᵀ (+ bias) with the tcgen05 kernel. Returns false
 // (and does nothing) when the shapes/dtypes/alignment do not fit the kernel.
 bool gemm_linear(const LcTensor* x2, const LcTensor* w, const LcTensor* bias, LcTensor* y, const GemmEpilogue& ep);
@@ -78,6 +108,7 @@ bool sdpa_flash(const LcTensor* q, const LcTensor* k, const LcTensor* v, const L
 // Reads and clears the device-side error words of the pipelined kernels.
 std::string take_device_errors();
 std::string take_attention_errors();
+std::string take_adapter_errors();
 // Cached 2-D tiled tensor map (128-byte swizzle) over a row-major [rows, cols] matrix with row stride ld.
 CUtensorMap tensor_map_2d(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows, int dtype);
 // The driver's cuTensorMapEncodeTiled (for maps of other ranks than tensor_map_2d's).

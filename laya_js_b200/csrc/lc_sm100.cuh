@@ -180,6 +180,39 @@ static __device__ __forceinline__ uint64_t sdesc_sw128_mn(uint32_t saddr) {
   return d;
 }
 
+// The same with several 64-element atoms along MN, `mn_stride` bytes apart
+// (the leading offset), each atom's 8-row groups 1024 bytes apart along K.
+static __device__ __forceinline__ uint64_t sdesc_sw128_mn(uint32_t saddr, uint32_t mn_stride) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)(mn_stride >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+static __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// Rows base .. base + 31 outside [lo, hi), as a mask of TMEM lanes an MMA leaves alone.
+static __device__ __forceinline__ uint32_t lanes_off(int base, int lo, int hi) {
+  const int a = max(lo - base, 0), b = min(hi - base, 32);
+  if (a >= b) return ~0u;
+  return ~(((b == 32) ? ~0u : ((1u << b) - 1u)) & ~((1u << a) - 1u));
+}
+// tc_mma that leaves the lanes (rows of D) set in off[4] as they are.
+static __device__ __forceinline__ void tc_mma_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, const uint32_t* off) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      : "memory");
+}
+
 // ---- packed f32 pairs (one instruction for two values; each element rounds
 // exactly as fmaf / __fadd_rn / __fmul_rn)
 static __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -254,6 +287,23 @@ static __device__ __forceinline__ void tc_mma_pair(uint32_t d, uint64_t a, uint6
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// tc_mma_pair that leaves the rows of D set in off[8] (four words per CTA) as they are
+static __device__ __forceinline__ void tc_mma_pair_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, const uint32_t* off) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]),
+      "r"(off[7])
+      : "memory");
+}
+static __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"((uint64_t)map), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
 // arrive once on the mbarrier at the same shared offset in both CTAs of the pair
