@@ -61,6 +61,9 @@ int lc_tensor_info(lc_tensor t, int* dtype, int* ndim, int64_t* shape /* [8] */)
 /* Device pointer of a dense tensor (0 when it is a strided view). Read-only:
    the library treats tensors as immutable (only lc_copy_into writes one). */
 int lc_tensor_data(lc_tensor t, uint64_t* dptr);
+/* lc_tensor_data and lc_tensor_free of n handles in one call (free stops at the first dead handle). */
+int lc_tensors_data(const lc_tensor* ts, int n, uint64_t* dptrs);
+int lc_tensors_free(const lc_tensor* ts, int n);
 /* index.ts:163-164 flush: waits for queued work. */
 int lc_flush(void);
 

@@ -19,6 +19,7 @@ import numpy as np
 
 from . import _lib
 from .host import HostTensor, f32_to_bf16_bits
+from .interop import SharedMemory
 
 
 class AdapterPlan:
@@ -53,7 +54,7 @@ def adapter_linear(backend, x, w, bias, a, bt, scales, plan: AdapterPlan):
     adapters' share alone (beside a projection that is computed elsewhere)."""
     b, out = backend, C.c_uint64()
     _lib.call("lc_adapter_linear", C.byref(out), b._h(x, "adapter_linear"), b._h(w), b._h(bias), b._h(a), b._h(bt), b._h(scales), plan.handle)
-    return b._wrap(out.value)
+    return b._wrap(out.value, x.dtype, (*x.shape[:-1], bt.shape[2]))
 
 
 def adapter_linear_grad(backend, dy, x, w, a, bt, scales, plan: AdapterPlan, want: Sequence[str] = ("dx", "da", "db")):
@@ -65,7 +66,7 @@ def adapter_linear_grad(backend, dy, x, w, a, bt, scales, plan: AdapterPlan, wan
     outs = [C.c_uint64() if k in want else None for k in ("dx", "da", "db")]
     _lib.call("lc_adapter_linear_grad", *[None if o is None else C.byref(o) for o in outs], b._h(dy, "adapter_linear_grad"), b._h(x), b._h(w),
               b._h(a), b._h(bt), b._h(scales), plan.handle)
-    return tuple(None if o is None else b._wrap(o.value) for o in outs)
+    return tuple(None if o is None else b._wrap(o.value, x.dtype, like.shape) for o, like in zip(outs, (x, a, bt)))
 
 
 def clip_grad_norm(backend, grads: Sequence, max_norm: float):
@@ -75,7 +76,10 @@ def clip_grad_norm(backend, grads: Sequence, max_norm: float):
     outs = (C.c_uint64 * max(1, n))()
     norm = C.c_uint64()
     _lib.call("lc_clip_grad_norm", outs, C.byref(norm), hs, n, float(max_norm))
-    return [b._wrap(outs[i]) for i in range(n)], b._wrap(norm.value)
+    clipped = [b._wrap(h, g.dtype, g.shape) for h, g in zip(outs, grads)]
+    if n > 1:
+        SharedMemory(b, clipped)
+    return clipped, b._wrap(norm.value, "f32", ())
 
 
 def _host(dtype: str, v) -> HostTensor:

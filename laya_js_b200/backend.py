@@ -30,11 +30,15 @@ _MODE = {"symmetric": 0, "affine": 1}
 class CudaTensor:
     """An opaque device tensor handle (index.ts:75-78 Tensor: shape + dtype)."""
 
-    __slots__ = ("handle", "shape", "dtype", "disposed", "keep", "_backend", "__weakref__")  # keep: owner of borrowed memory
+    __slots__ = ("handle", "shape", "dtype", "disposed", "keep", "_backend", "__weakref__")  # keep: what else the memory hangs on (interop)
 
-    def __init__(self, backend: "CudaBackend", handle: int):
+    def __init__(self, backend: "CudaBackend", handle: int, dtype: Optional[str] = None, shape: Optional[tuple] = None):
         self._backend = backend
         self.handle = handle
+        self.keep = None
+        if dtype is not None:  # the caller knows them: no call into the library
+            self.shape, self.dtype, self.disposed = shape, dtype, False
+            return
         dt = C.c_int()
         nd = C.c_int()
         sh = (C.c_int64 * 8)()
@@ -65,8 +69,8 @@ class CudaBackend:
         self._destroyed = False
 
     # ------------------------------------------------------------ plumbing
-    def _wrap(self, h: int) -> CudaTensor:
-        t = CudaTensor(self, h)
+    def _wrap(self, h: int, dtype: Optional[str] = None, shape: Optional[tuple] = None) -> CudaTensor:
+        t = CudaTensor(self, h, dtype, shape)
         if self._scopes:
             self._scopes[-1].append(t)
         return t

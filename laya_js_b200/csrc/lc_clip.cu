@@ -1,22 +1,28 @@
 // Global-norm gradient clipping over many tensors (lc_clip_grad_norm,
 // include/laya_cuda_adapters.h): norm = sqrt(Σ g²), out = g·min(1, max/(norm + 1e-6)).
 //
-// Every tensor is cut into chunks of kChunk elements; block b takes chunks b,
-// b + grid, ... Pass one leaves one f64 partial sum of squares per block, pass
-// two adds the partials in a fixed order in every block and scales.
+// Bound by memory: every gradient is read once for the norm, once more to be
+// scaled, and written once. Every tensor is cut into chunks of kChunk values
+// (four 16-byte loads in flight per thread); block b takes chunks b,
+// b + grid, ... Pass one leaves one f64 partial sum of squares per block; pass
+// two adds the partials in a fixed order in every block and scales, taking the
+// chunks in the opposite order so that the values read last by pass one come
+// from L2 (126 MB).
 #include "lc_api.h"
 #include "laya_cuda_adapters.h"
 
 #include <algorithm>
 #include <cmath>
+#include <memory>
 #include <vector>
 
 namespace {
 using namespace lc;
 
-constexpr int kChunk = 8192;       // elements per chunk
-constexpr int kMaxTensors = 640;   // per launch: the table travels as a kernel parameter (at most 32 KB)
 constexpr int kThreads = 256;
+constexpr int kUnroll = 4;                            // 16-byte vectors in flight per thread
+constexpr int kChunkBytes = kThreads * kUnroll * 16;  // 16 KB of one tensor
+constexpr int kMaxTensors = 640;                      // per launch: the table travels as a kernel parameter (at most 32 KB)
 constexpr float kEps = 1e-6f;
 
 struct ClipTensor {
@@ -26,17 +32,23 @@ struct ClipTensor {
   int32_t dtype;
   int32_t chunk0;  // chunks of the tensors before it
 };
-struct ClipTable {
+struct ClipHead {
   int ntensors, nchunks;
   int part0, nparts;  // this launch's first partial, and the partials of all launches
   double max_norm;
   double* parts;
   float* norm;
-  ClipTensor t[kMaxTensors];
+};
+// Tables of three sizes: the launch copies the whole parameter.
+template <int N>
+struct ClipTable {
+  ClipHead h;
+  ClipTensor t[N];
 };
 
-__device__ __forceinline__ const ClipTensor& tensor_of(const ClipTable& tab, int chunk) {
-  int lo = 0, hi = tab.ntensors - 1;
+template <int N>
+__device__ __forceinline__ const ClipTensor& tensor_of(const ClipTable<N>& tab, int chunk) {
+  int lo = 0, hi = tab.h.ntensors - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (tab.t[mid].chunk0 <= chunk) lo = mid;
@@ -58,32 +70,155 @@ __device__ __forceinline__ double block_sum(double v) {
   return r;
 }
 
-__global__ void __launch_bounds__(kThreads) k_clip_norm(const __grid_constant__ ClipTable tab) {
-  double sum = 0;
-  for (int c = blockIdx.x; c < tab.nchunks; c += gridDim.x) {
-    const ClipTensor& t = tensor_of(tab, c);
-    const int64_t lo = (int64_t)(c - t.chunk0) * kChunk, hi = min(t.n, lo + kChunk);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
-      const double g = (double)ld_as<float>(t.in, t.dtype, i);
-      sum = fma(g, g, sum);
-    }
+// The values of a 16-byte vector as f32.
+template <typename T>
+struct Vec {
+  static constexpr int n = 16 / sizeof(T);
+  __device__ static void get(const uint4& u, float* f) {
+    const T* v = (const T*)&u;
+#pragma unroll
+    for (int i = 0; i < n; i++) f[i] = to_f<T>(v[i]);
   }
-  sum = block_sum(sum);
-  if (threadIdx.x == 0) tab.parts[tab.part0 + blockIdx.x] = sum;
+  __device__ static uint4 put(const float* f) {
+    uint4 u;
+    T* v = (T*)&u;
+#pragma unroll
+    for (int i = 0; i < n; i++) v[i] = from_f<T>(f[i]);
+    return u;
+  }
+};
+
+// Squares of a vector, summed in f32 where that loses nothing that counts: a
+// sum outside [1e-30, 1e38] (or not a number) is taken again in f64.
+template <typename T>
+__device__ __forceinline__ double squares(const uint4& u) {
+  float f[Vec<T>::n], p = 0.f;
+  Vec<T>::get(u, f);
+#pragma unroll
+  for (int i = 0; i < Vec<T>::n; i++) p = fmaf(f[i], f[i], p);
+  if (p >= 1e-30f && p <= 1e38f) return (double)p;
+  constexpr uint32_t kMagnitude = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+  if (!((u.x | u.y | u.z | u.w) & kMagnitude)) return 0.0;  // zeros of either sign
+  double d = 0;
+#pragma unroll
+  for (int i = 0; i < Vec<T>::n; i++) d = fma((double)f[i], (double)f[i], d);
+  return d;
 }
 
-__global__ void __launch_bounds__(kThreads) k_clip_scale(const __grid_constant__ ClipTable tab) {
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const ClipTensor& t, int64_t lo, int64_t hi) {
+  const T* in = (const T*)t.in;
   double sum = 0;
-  for (int i = threadIdx.x; i < tab.nparts; i += kThreads) sum += tab.parts[i];
-  const double norm = sqrt(block_sum(sum));
-  const double ratio = tab.max_norm / (norm + (double)kEps);
-  const float f = ratio < 1.0 || isnan(ratio) ? (float)ratio : 1.f;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *tab.norm = (float)norm;
-  for (int c = blockIdx.x; c < tab.nchunks; c += gridDim.x) {
-    const ClipTensor& t = tensor_of(tab, c);
-    const int64_t lo = (int64_t)(c - t.chunk0) * kChunk, hi = min(t.n, lo + kChunk);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) st_as<float>(t.out, t.dtype, i, f * ld_as<float>(t.in, t.dtype, i));
+  int64_t i = lo;
+  if (((uintptr_t)t.in & 15) == 0) {
+    constexpr int V = Vec<T>::n;
+    const int nv = (int)((hi - lo) / V);
+    const uint4* v = (const uint4*)(in + lo);
+    uint4 u[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; k++) {
+      const int j = threadIdx.x + k * kThreads;
+      u[k] = j < nv ? __ldg(v + j) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int k = 0; k < kUnroll; k++) sum += squares<T>(u[k]);
+    i = lo + (int64_t)nv * V;
   }
+  for (i += threadIdx.x; i < hi; i += kThreads) {
+    const double g = (double)to_f<T>(in[i]);
+    sum = fma(g, g, sum);
+  }
+  return sum;
+}
+
+template <typename T>
+__device__ __forceinline__ void chunk_scale(const ClipTensor& t, int64_t lo, int64_t hi, float f) {
+  const T* in = (const T*)t.in;
+  T* out = (T*)t.out;
+  int64_t i = lo;
+  if (((uintptr_t)t.in & 15) == 0) {
+    constexpr int V = Vec<T>::n;
+    const int nv = (int)((hi - lo) / V);
+    const uint4* v = (const uint4*)(in + lo);
+    uint4* o = (uint4*)(out + lo);
+    uint4 u[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; k++) {
+      const int j = threadIdx.x + k * kThreads;
+      if (j < nv) u[k] = __ldg(v + j);
+    }
+#pragma unroll
+    for (int k = 0; k < kUnroll; k++) {
+      const int j = threadIdx.x + k * kThreads;
+      if (j < nv) {
+        float w[V];
+        Vec<T>::get(u[k], w);
+#pragma unroll
+        for (int e = 0; e < V; e++) w[e] *= f;
+        __stcs(o + j, Vec<T>::put(w));
+      }
+    }
+    i = lo + (int64_t)nv * V;
+  }
+  for (i += threadIdx.x; i < hi; i += kThreads) out[i] = from_f<T>(f * to_f<T>(in[i]));
+}
+
+__device__ __forceinline__ int chunk_values(int dtype) { return kChunkBytes / (dtype == LC_F32 ? 4 : 2); }
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) k_clip_norm(const __grid_constant__ ClipTable<N> tab) {
+  pdl_trigger();
+  pdl_wait();
+  double sum = 0;
+  for (int c = blockIdx.x; c < tab.h.nchunks; c += gridDim.x) {
+    const ClipTensor& t = tensor_of(tab, c);
+    const int64_t per = chunk_values(t.dtype), lo = (int64_t)(c - t.chunk0) * per, hi = min(t.n, lo + per);
+    if (t.dtype == LC_F32) sum += chunk_squares<float>(t, lo, hi);
+    else if (t.dtype == LC_F16) sum += chunk_squares<__half>(t, lo, hi);
+    else sum += chunk_squares<__nv_bfloat16>(t, lo, hi);
+  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) tab.h.parts[tab.h.part0 + blockIdx.x] = sum;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) k_clip_scale(const __grid_constant__ ClipTable<N> tab) {
+  pdl_trigger();
+  pdl_wait();
+  double sum = 0;
+  for (int i = threadIdx.x; i < tab.h.nparts; i += kThreads) sum += tab.h.parts[i];
+  const double norm = sqrt(block_sum(sum));
+  const double ratio = tab.h.max_norm / (norm + (double)kEps);
+  const float f = ratio < 1.0 || isnan(ratio) ? (float)ratio : 1.f;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *tab.h.norm = (float)norm;
+  for (int c = tab.h.nchunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
+    const ClipTensor& t = tensor_of(tab, c);
+    const int64_t per = chunk_values(t.dtype), lo = (int64_t)(c - t.chunk0) * per, hi = min(t.n, lo + per);
+    if (t.dtype == LC_F32) chunk_scale<float>(t, lo, hi, f);
+    else if (t.dtype == LC_F16) chunk_scale<__half>(t, lo, hi, f);
+    else chunk_scale<__nv_bfloat16>(t, lo, hi, f);
+  }
+}
+
+// Both passes over the tensors of `t` (consecutive launches of at most N).
+template <int N>
+void clip_launch(const std::vector<ClipTensor>& ts, double max_norm, float* norm, double* parts, const std::vector<int>& first, const std::vector<int>& grid,
+                 cudaStream_t st) {
+  auto tab = std::make_unique<ClipTable<N>>();
+  int nparts = 0;
+  for (int g : grid) nparts += g;
+  for (int pass = 0; pass < 2; pass++)
+    for (size_t l = 0, part0 = 0; l < grid.size(); part0 += grid[l], l++) {
+      const int lo = first[l], n = first[l + 1] - lo;
+      tab->h = {n, 0, (int)part0, nparts, max_norm, parts, norm};
+      for (int i = 0; i < n; i++) {
+        tab->t[i] = ts[lo + i];
+        tab->t[i].chunk0 = tab->h.nchunks;
+        tab->h.nchunks += ts[lo + i].chunk0;  // (its chunk count, until it is placed)
+      }
+      launch_chain(pass ? k_clip_scale<N> : k_clip_norm<N>, dim3(grid[l]), dim3(kThreads), 0, st, *tab);
+      LC_LAUNCHED(1);
+    }
 }
 
 }  // namespace
@@ -131,44 +266,35 @@ int lc_clip_grad_norm(lc_tensor* outs, lc_tensor* norm_out, const lc_tensor* gra
     out[i]->dtype = in[i]->dtype;
     held.ts.push_back(out[i]);
   }
-  std::vector<ClipTable> tabs(1);
-  auto fresh = [&]() { tabs.back().ntensors = tabs.back().nchunks = 0; };
-  fresh();
+  std::vector<ClipTensor> ts;       // chunk0: the number of chunks, for now
+  std::vector<int> first{0}, grid;  // launches: their first tensor, their blocks
+  int64_t chunks = 0, nparts = 0;
+  auto close = [&]() {
+    first.push_back((int)ts.size());
+    grid.push_back((int)std::max<int64_t>(1, std::min<int64_t>(chunks, num_sms() * 8)));
+    nparts += grid.back();
+    chunks = 0;
+  };
   for (int i = 0; i < n; i++) {
-    const int64_t chunks = (in[i]->numel() + kChunk - 1) / kChunk;
-    if (!chunks) continue;
-    if (tabs.back().ntensors == kMaxTensors || tabs.back().nchunks + chunks > INT32_MAX) {
-      LC_CHECK(chunks <= INT32_MAX, "clip_grad_norm: a gradient is too large");
-      tabs.emplace_back();
-      fresh();
-    }
-    ClipTable& tab = tabs.back();
-    tab.t[tab.ntensors++] = {in[i]->data(), out[i]->data(), in[i]->numel(), in[i]->dtype, tab.nchunks};
-    tab.nchunks += (int)chunks;
+    const int64_t bytes_i = in[i]->numel() * dtype_size(in[i]->dtype), c = (bytes_i + kChunkBytes - 1) / kChunkBytes;
+    if (!c) continue;
+    LC_CHECK(c <= INT32_MAX / 2, "clip_grad_norm: a gradient is too large");
+    if ((int)ts.size() - first.back() == kMaxTensors || chunks + c > INT32_MAX / 2) close();
+    ts.push_back({in[i]->data(), out[i]->data(), in[i]->numel(), in[i]->dtype, (int32_t)c});
+    chunks += c;
   }
-  int parts = 0;
-  std::vector<int> grid;
-  for (auto& tab : tabs) {
-    tab.part0 = parts;
-    grid.push_back(std::max(1, std::min(tab.nchunks, num_sms() * 8)));
-    parts += grid.back();
-  }
-  double* pd = (double*)dmalloc((size_t)parts * 8);
-  held.mem.push_back(pd);
-  for (auto& tab : tabs) {
-    tab.nparts = parts;
-    tab.max_norm = max_norm;
-    tab.parts = pd;
-    tab.norm = (float*)norm->data();
-  }
-  for (size_t i = 0; i < tabs.size(); i++) k_clip_norm<<<grid[i], kThreads, 0, stream()>>>(tabs[i]);
-  for (size_t i = 0; i < tabs.size(); i++) k_clip_scale<<<grid[i], kThreads, 0, stream()>>>(tabs[i]);
-  LC_LAUNCHED(2 * (int)tabs.size());
+  close();
+  double* parts = (double*)dmalloc((size_t)nparts * 8);
+  held.mem.push_back(parts);
+  float* np = (float*)norm->data();
+  if (ts.size() <= 16) clip_launch<16>(ts, max_norm, np, parts, first, grid, stream());
+  else if (ts.size() <= 128) clip_launch<128>(ts, max_norm, np, parts, first, grid, stream());
+  else clip_launch<kMaxTensors>(ts, max_norm, np, parts, first, grid, stream());
   for (int i = 0; i < n; i++) outs[i] = handle(out[i]);
   *norm_out = handle(norm);
-  held.ts.erase(std::remove_if(held.ts.begin(), held.ts.end(),
-                               [&](LcTensor* t) { return t == norm || std::find(out.begin(), out.end(), t) != out.end(); }),
-                held.ts.end());
+  // handed to the caller: what was made after the dense copies, but for `all`
+  held.ts.erase(std::find(held.ts.begin(), held.ts.end(), norm));
+  held.ts.resize(held.ts.size() - n);
   LC_API_END
 }
 

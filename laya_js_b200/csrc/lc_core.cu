@@ -574,6 +574,21 @@ int lc_tensor_data(lc_tensor h, uint64_t* dptr) {
   LC_API_END
 }
 
+int lc_tensors_data(const lc_tensor* hs, int n, uint64_t* dptrs) {
+  LC_API_BEGIN
+  for (int i = 0; i < n; i++) {
+    LcTensor* t = check(hs[i], "data");
+    dptrs[i] = t->contiguous() ? reinterpret_cast<uint64_t>(t->data()) : 0;
+  }
+  LC_API_END
+}
+
+int lc_tensors_free(const lc_tensor* hs, int n) {
+  LC_API_BEGIN
+  for (int i = 0; i < n; i++) release(check(hs[i], "dispose"));
+  LC_API_END
+}
+
 int lc_flush(void) {
   LC_API_BEGIN
   ensure_init();

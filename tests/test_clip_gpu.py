@@ -145,3 +145,43 @@ def test_refusals_and_no_gradients():
     b.dispose(g)
     with pytest.raises(LayaCudaError, match="dispose"):
         A.clip_grad_norm(b, [g], 1.0)
+
+
+def test_outputs_as_torch_tensors():
+    """The outputs share an allocation: it lives until the last torch tensor
+    and the last handle over it are gone."""
+    import torch
+
+    from laya_js_b200 import _lib, interop
+    b = backend()
+    rng = np.random.default_rng(8)
+    hosts = [mk(k, rng.standard_normal(s)) for k, s in (("bf16", (3, 5)), ("f32", (7,)), ("bf16", (0, 4)), ("bf16", (300, 41)), ("f16", ()), ("f32", (2, 2, 2)))]
+    want, norm = _want(hosts, 0.5)
+    interop.useTorchStream(b)
+    try:
+        before = b.stats()
+        ins = [b.fromHost(h) for h in hosts]
+        outs, n = A.clip_grad_norm(b, ins, 0.5)
+        ts = [interop.toTorch(b, t) for t in outs[1:]]
+        n = interop.toTorch(b, n)
+        first = interop.toTorch(b, outs[0])  # after the others
+        torch.cuda.synchronize()
+        for t, h, w in zip([first, *ts], hosts, want):
+            assert tuple(t.shape) == tuple(h.shape) and str(t.dtype) == {"bf16": "torch.bfloat16", "f16": "torch.float16", "f32": "torch.float32"}[h.dtype]
+            assert np.all(np.abs(t.double().cpu().numpy() - w) <= (2.0 ** -DIGITS[h.dtype] + 2.0 ** -18) * np.abs(w) + TINY[h.dtype])
+        assert abs(float(n) - norm) <= 2.0 ** -19 * norm
+        for t in outs:
+            b.dispose(t)  # given away: nothing happens
+        keep = ts[2]
+        copy = keep.clone()
+        del ts, first, n, t, outs
+        torch.cuda.synchronize()
+        assert torch.equal(keep, copy)
+        del keep
+        for t in ins:
+            b.dispose(t)
+        after = b.stats()
+        assert after["live_tensors"] == before["live_tensors"] and after["live_bytes"] == before["live_bytes"]
+    finally:
+        torch.cuda.synchronize()
+        _lib.call("lc_set_stream", 0)
