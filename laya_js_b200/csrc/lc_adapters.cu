@@ -346,8 +346,19 @@ struct Padder {
   }
 };
 
-void* shrink_tc(const Operands& o, const Rows& X, const Rows& P, int64_t C, Held& held) {
-  void* Q = held.scratch((size_t)o.T * adapter_u_cols(o.r) * 2);
+// The kernels after the shrink start while it runs (programmatic dependent
+// launch). It releases them after its own dependency wait, so what ran before
+// this operator is complete by then, and each waits for its predecessor before
+// it reads what that wrote and before it ends.
+struct Chained {
+  std::unique_ptr<PdlScope> scope;
+  explicit Chained(const Operands& o) {
+    if (o.plan->nsegs) scope = std::make_unique<PdlScope>();
+  }
+};
+
+// Scratch for Q and the product that fills it.
+AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_t C, Held& held) {
   AdapterShrink c;
   c.X = X.p;
   c.P = P.p;
@@ -357,9 +368,8 @@ void* shrink_tc(const Operands& o, const Rows& X, const Rows& P, int64_t C, Held
   c.n = o.n;
   c.rank = o.r;
   c.scales = o.scale_ptr();
-  c.Q = Q;
-  adapter_shrink_tc(c, *o.plan, o.dtype, stream());
-  return Q;
+  c.Q = held.scratch((size_t)o.T * adapter_u_cols(o.r) * 2);
+  return c;
 }
 
 void expand_tc(const Operands& o, const Rows& X, const Rows& W, const Rows& P, const void* Q, bool transposed, LcTensor* Y) {
@@ -387,18 +397,8 @@ void expand_tc(const Operands& o, const Rows& X, const Rows& W, const Rows& P, c
   c.share.segs = o.plan->segs;
   c.share.tile_first = o.plan->tile_first;
   c.share.nsegs = o.plan->nsegs;
+  c.after_share = o.plan->nsegs > 0;
   gemm_adapted(c, o.dtype, stream());
-}
-
-void outer_tc(const Operands& o, const void* Q, const Rows& X, int64_t C, LcTensor* dP) {
-  AdapterOuter c;
-  c.X = X.p;
-  c.Q = Q;
-  c.C = C;
-  c.ld = X.ld;
-  c.rank = o.r;
-  c.dP = dP->data();
-  adapter_outer_tc(c, *o.plan, o.dtype, stream());
 }
 
 void linear(const Operands& o, LcTensor* y, Held& held) {
@@ -413,24 +413,27 @@ void linear(const Operands& o, LcTensor* y, Held& held) {
   const Rows x = pad.of(o.x, o.T, o.K), w = pad.of(o.w, o.N, o.K), a = pad.of(o.a, (int64_t)o.n * o.r, o.K),
              b = pad.of(o.b, (int64_t)o.n * o.r, o.N);
   pad.run();
-  void* u = shrink_tc(o, x, a, o.K, held);
-  expand_tc(o, x, w, b, u, false, y);
+  const AdapterShrink u = shrink_job(o, x, a, o.K, held);
+  adapter_shrink_tc(&u, 1, nullptr, 0, *o.plan, o.dtype, stream());
+  const Chained chained(o);
+  expand_tc(o, x, w, b, u.Q, false, y);
 }
 
 void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held& held) {
-  if (!o.T) {
+  if (!o.plan->nsegs) {  // no row has an adapter
     for (LcTensor* t : {da, db})
       if (t && t->numel()) CUDA_OK(cudaMemsetAsync(t->data(), 0, t->numel() * dtype_size(o.dtype), stream()));
-    return;
+    da = db = nullptr;
+    if (!o.T) return;
   }
   if (o.dtype == LC_F32) {
     float* q = (float*)held.scratch((size_t)o.T * o.r * 4);
     if (dx || da) {
       shrink_f32(o, o.dy, o.b, o.N, q);
       if (dx) expand_f32(o, o.dy, o.a, q, true, dx);
-      if (da && o.n) outer_f32(o, q, o.x, o.K, da);
+      if (da) outer_f32(o, q, o.x, o.K, da);
     }
-    if (db && o.n) {
+    if (db) {
       shrink_f32(o, o.x, o.a, o.K, q);
       outer_f32(o, q, o.dy, o.N, db);
     }
@@ -440,15 +443,40 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
   const Rows dy = pad.of(o.dy, o.T, o.N), x = da || db ? pad.of(o.x, o.T, o.K) : Rows{}, w = dx ? pad.of(o.w, o.N, o.K) : Rows{},
              a = dx || db ? pad.of(o.a, (int64_t)o.n * o.r, o.K) : Rows{}, b = dx || da ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : Rows{};
   pad.run();
+  AdapterShrink q[2];
+  int nq = 0;
+  const void *g = nullptr, *u = nullptr;
   if (dx || da) {
-    void* g = shrink_tc(o, dy, b, o.N, held);
-    if (dx) expand_tc(o, dy, w, a, g, true, dx);
-    if (da) outer_tc(o, g, x, o.K, da);
+    q[nq] = shrink_job(o, dy, b, o.N, held);
+    g = q[nq++].Q;
   }
   if (db) {
-    void* u = shrink_tc(o, x, a, o.K, held);
-    outer_tc(o, u, dy, o.N, db);
+    q[nq] = shrink_job(o, x, a, o.K, held);
+    u = q[nq++].Q;
   }
+  if (!nq) return;
+  AdapterOuter out[2];
+  int no = 0;
+  size_t words[2] = {0, 0};
+  auto job = [&](const void* Q, const Rows& X, int64_t C, LcTensor* dP) {
+    AdapterOuter& c = out[no];
+    c.X = X.p;
+    c.Q = Q;
+    c.C = C;
+    c.ld = X.ld;
+    c.rank = o.r;
+    c.dP = dP->data();
+    words[no++] = adapter_count_words(*o.plan, o.r, C);
+  };
+  if (db) job(u, dy, o.N, db);
+  if (da) job(g, x, o.K, da);
+  uint32_t* count = no ? (uint32_t*)held.scratch((words[0] + words[1]) * 4) : nullptr;
+  out[0].count = count;
+  out[1].count = count + words[0];
+  adapter_shrink_tc(q, nq, count, words[0] + words[1], *o.plan, o.dtype, stream());
+  const Chained chained(o);
+  if (no) adapter_outer_tc(out, no, *o.plan, o.dtype, stream());
+  if (dx) expand_tc(o, dy, w, a, g, true, dx);
 }
 
 }  // namespace

@@ -33,16 +33,21 @@ struct AdapterShrink {
   const float* scales = nullptr;
   void* Q = nullptr;
 };
-// dP[a] = Σ_{t in a} Q[t] ⊗ X[t], [n, rank, C] dense.
+// dP[a] = Σ_{t in a} Q[t] ⊗ X[t], [n, rank, C] dense; count: adapter_count_words zeros.
 struct AdapterOuter {
   const void *X = nullptr, *Q = nullptr;
   int64_t C = 0, ld = 0;
   int rank = 0;
   void* dP = nullptr;
+  uint32_t* count = nullptr;
 };
 namespace lc {
-void adapter_shrink_tc(const AdapterShrink& c, const AdapterPlan& p, int dtype, cudaStream_t st);
-void adapter_outer_tc(const AdapterOuter& c, const AdapterPlan& p, int dtype, cudaStream_t st);
+// One or two products over the same rows, ranks and scales. The shrink also
+// clears `nzero` words for a kernel that follows it.
+void adapter_shrink_tc(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, const AdapterPlan& p, int dtype, cudaStream_t st);
+void adapter_outer_tc(const AdapterOuter* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
+size_t adapter_count_words(const AdapterPlan& p, int rank, int64_t C);
+int adapter_runs(int tiles, int nchunks);
 }  // namespace lc
 
 void lc_adapters_destroy();

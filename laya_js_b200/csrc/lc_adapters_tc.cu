@@ -70,42 +70,56 @@ __device__ __forceinline__ void split2(float v, T& hi, T& lo) {
 
 // ------------------------------------------------------------- shrink
 //
-// One CTA takes tiles of 128 rows. Per 64-column block of X the ring holds the
-// X block (TMA, 16 KB) and, for up to `nb` of the tile's segments, the block of
-// P_a (R rows); one MMA per segment and 16 columns adds to D [128, R] with the
-// lanes outside the segment switched off, so every row meets its own adapter
-// alone. More segments than nb: the tile's columns are streamed again.
-// D is double-buffered in TMEM; the epilogue scales, splits and stores rows.
+// One CTA takes tiles of 128 rows of one or two products (both directions of a
+// gradient share a launch). Per 64-column block of X the ring holds the X block
+// (TMA, 16 KB) and, for up to `nb` of the tile's segments, their blocks of P_a
+// (R rows each), side by side: one MMA per 16 columns gives every row against
+// every one of these adapters, D [128, n·R] (n·R <= 256), and the epilogue
+// takes from each row's n results the one of its own adapter, scales, splits
+// and stores it. The tensor cores have room for the others: an MMA this narrow
+// costs the reading of X, not its width, and one MMA per segment with the other
+// rows switched off took 131 us where this takes the time below. More segments
+// than nb: the tile's columns are streamed again. D is double-buffered in TMEM.
 //
 // Bound by the read of X. With few tiles the columns are split over clusters
 // of S CTAs, whose partial D meet in shared memory and are added in rank order.
+struct ShrinkJob {
+  CUtensorMap tmX, tmP;
+  void* Q;
+  int C;
+};
 struct ShrinkArgs {
-  int T, C, ntiles, nsegs, R, rank, nb, stages, ucols;
+  ShrinkJob job[2];
+  int njobs, T, ntiles, nsegs, R, rank, nb, stages, ucols, S;
   uint32_t bank_bytes, tmem_cols;
   const int4* segs;
   const int32_t* tile_first;
-  const int32_t* row_adapter;
   const float* scales;
-  void* Q;
+  uint32_t* zero;  // words that the next kernel counts in
+  int nzero;
 };
+// The segments of one pass over a tile: s, s + 1, ... that meet rows [m0, m0 + 128); 0 when the tile is done.
+__device__ __forceinline__ int pass_segments(const ShrinkArgs& args, int s, int m0) {
+  int n = 0;
+  while (n < args.nb && s + n < args.nsegs && __ldg(&args.segs[s + n].x) < m0 + BM) n++;
+  return n;
+}
 
 template <typename T>
-__global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmP,
-                                                             const __grid_constant__ ShrinkArgs args, int S) {
+__global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_constant__ ShrinkArgs args) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t stage_bytes = X_BYTES + args.bank_bytes;
-  uint64_t* full = (uint64_t*)(smem + args.stages * stage_bytes);
+  float* sD = (float*)(smem + args.stages * stage_bytes);  // S > 1: this CTA's share of D [128, R]
+  uint64_t* full = (uint64_t*)(sD + (args.S > 1 ? BM * args.R : 0));
   uint64_t* empty = full + args.stages;
   uint64_t* tfull = empty + args.stages;
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = (uint32_t*)(tempty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = S > 1 ? (int)cluster_rank() : 0;
-  const int KB = (args.C + BK - 1) / BK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
-  const int first = blockIdx.x / S, step = gridDim.x / S;
-  pdl_trigger();
+  const int S = args.S, rank = S > 1 ? (int)cluster_rank() : 0;
+  const int first = blockIdx.x / S, step = gridDim.x / S, nitems = args.njobs * args.ntiles;
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
     for (int a = 0; a < 2; a++) mbar_init(&tfull[a], 1), mbar_init(&tempty[a], 4);
@@ -119,6 +133,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
+  pdl_trigger();  // after the wait: what runs before this kernel is done when the next one starts
+  for (int i = blockIdx.x * TC_THREADS + threadIdx.x; i < args.nzero; i += gridDim.x * TC_THREADS) args.zero[i] = 0;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -126,29 +142,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
       uint32_t phase = 0;
       bool ok = true;
       uint32_t used = 0, last_phase = 0;  // stages filled, and the phase bit of each one's last fill
-      for (int t = first; t < args.ntiles && ok; t += step) {
-        const int m0 = t * BM;
-        for (int s = __ldg(args.tile_first + t); s < args.nsegs && ok; s += args.nb) {
-          if (__ldg(&args.segs[s]).x >= m0 + BM) break;
-          int n = 1;  // segments of this pass
-          int ad[4];
-          ad[0] = __ldg(&args.segs[s]).z;
-#pragma unroll
-          for (int i = 1; i < 4; i++) {
-            ad[i] = 0;
-            if (i < args.nb && n == i && s + i < args.nsegs) {
-              const int4 g = __ldg(&args.segs[s + i]);
-              if (g.x < m0 + BM) ad[i] = g.z, n = i + 1;
-            }
-          }
+      for (int it = first; it < nitems && ok; it += step) {
+        const ShrinkJob& job = args.job[it >= args.ntiles];
+        const int t = it >= args.ntiles ? it - args.ntiles : it, m0 = t * BM;
+        const int KB = (job.C + BK - 1) / BK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
+        int n;
+        for (int s = __ldg(args.tile_first + t); ok && (n = pass_segments(args, s, m0)); s += n) {
           for (int kb = kb0; kb < kb1; kb++) {
             if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
             uint8_t* st = smem + stage * stage_bytes;
             mbar_arrive_expect_tx(&full[stage], X_BYTES + (uint32_t)n * args.R * 128);
-            tma_load_2d(st, &tmX, &full[stage], kb * BK, m0);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              if (i < n) tma_load_3d(st + X_BYTES + i * args.R * 128, &tmP, &full[stage], kb * BK, 0, ad[i]);
+            tma_load_2d(st, &job.tmX, &full[stage], kb * BK, m0);
+            for (int i = 0; i < n; i++)
+              tma_load_3d(st + X_BYTES + i * args.R * 128, &job.tmP, &full[stage], kb * BK, 0, __ldg(&args.segs[s + i].z));
             used |= 1u << stage;
             last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
             if (++stage == args.stages) { stage = 0; phase ^= 1; }
@@ -163,55 +169,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = idesc_rt<T>(args.R, false, false);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       uint64_t* last = nullptr;
       uint32_t last_phase = 0;
-      for (int t = first; t < args.ntiles && ok; t += step) {
-        const int m0 = t * BM;
-        int s = __ldg(args.tile_first + t);
-        if (s >= args.nsegs || __ldg(&args.segs[s]).x >= m0 + BM) continue;
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(acc * args.R);
-        for (; s < args.nsegs && ok; s += args.nb) {
-          if (__ldg(&args.segs[s]).x >= m0 + BM) break;
-          uint32_t off[4][4];
-          int n = 0;
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            if (i < args.nb && n == i && s + i < args.nsegs) {
-              const int4 g = __ldg(&args.segs[s + i]);
-              if (g.x < m0 + BM) {
-                n = i + 1;
-#pragma unroll
-                for (int w = 0; w < 4; w++) off[i][w] = lanes_off(m0 + 32 * w, g.x, g.y);
-              }
-            }
-          }
+      for (int it = first; it < nitems && ok; it += step) {
+        const ShrinkJob& job = args.job[it >= args.ntiles];
+        const int t = it >= args.ntiles ? it - args.ntiles : it, m0 = t * BM;
+        const int KB = (job.C + BK - 1) / BK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
+        int n;
+        for (int s = __ldg(args.tile_first + t); ok && (n = pass_segments(args, s, m0)); s += n) {
+          const uint32_t idesc = idesc_rt<T>(n * args.R, false, false);
+          if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(acc * args.nb * args.R);
           for (int kb = kb0; kb < kb1; kb++) {
             if (!mbar_wait(&full[stage], phase, abort, &g_adapter_err)) { ok = false; break; }
             tc_fence_after();
             const uint32_t a0 = smem_u32(smem + stage * stage_bytes), b0 = a0 + X_BYTES;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              if (i < n)
-#pragma unroll
-                for (int k = 0; k < BK / 16; k++)
-                  tc_mma_lanes(d, sdesc_sw128(a0 + k * 32), sdesc_sw128(b0 + i * args.R * 128 + k * 32), idesc, (kb > kb0 || k > 0) ? 1u : 0u, off[i]);
+            for (int k = 0; k < BK / 16; k++) tc_mma(d, sdesc_sw128(a0 + k * 32), sdesc_sw128(b0 + k * 32), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
             tc_commit(&empty[stage]);
             last = &empty[stage];
             last_phase = phase;
             if (++stage == args.stages) { stage = 0; phase ^= 1; }
           }
+          if (!ok) break;
+          tc_commit(&tfull[acc]);
+          last = &tfull[acc];
+          last_phase = acc_phase;
+          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
         }
-        if (!ok) break;
-        tc_commit(&tfull[acc]);
-        last = &tfull[acc];
-        last_phase = acc_phase;
-        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
       if (last) {  // the MMAs issued here finish before TMEM is freed
         const uint64_t t0 = gtimer();
@@ -219,46 +208,50 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
       }
     }
   } else {
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, half = args.ucols / 2;
     int acc = 0;
     uint32_t acc_phase = 0;
-    T* Q = (T*)args.Q;
-    for (int t = first; t < args.ntiles; t += step) {
-      const int m0 = t * BM, s0 = __ldg(args.tile_first + t);
-      if (s0 >= args.nsegs || __ldg(&args.segs[s0]).x >= m0 + BM) continue;
-      const int row = m0 + quarter * 32 + lane;
-      const int a = row < args.T ? __ldg(args.row_adapter + row) : -1;
-      const float sc = a >= 0 && args.scales ? __ldg(args.scales + a) : 1.f;
-      if (!mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err)) break;
-      tc_fence_after();
-      const uint32_t tb = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * args.R);
-      const int half = args.ucols / 2;
-      for (int c = 0; c < args.R; c += 16) {
-        uint32_t v[16];
-        tmem_ld16(tb + c, v);
-        tmem_wait_ld();
-        if (S > 1) {  // this CTA's share of the columns: to shared memory, added below
-          float* p = (float*)smem + (quarter * 32 + lane) * args.R + c;
+    bool ok = true;
+    for (int it = first; it < nitems && ok; it += step) {
+      const int t = it >= args.ntiles ? it - args.ntiles : it, m0 = t * BM, row = m0 + quarter * 32 + lane;
+      T* Q = (T*)args.job[it >= args.ntiles].Q + (int64_t)row * args.ucols;
+      int n;
+      for (int s = __ldg(args.tile_first + t); ok && (n = pass_segments(args, s, m0)); s += n) {
+        if (!mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err)) { ok = false; break; }
+        tc_fence_after();
+        for (int i = 0; i < n; i++) {
+          const int4 g = __ldg(&args.segs[s + i]);
+          const bool mine = row >= g.x && row < g.y;
+          if (!__any_sync(0xffffffffu, mine)) continue;
+          const float sc = args.scales ? __ldg(args.scales + g.z) : 1.f;
+          const uint32_t tb = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((acc * args.nb + i) * args.R);
+          for (int c = 0; c < args.R; c += 16) {
+            uint32_t v[16];
+            tmem_ld16(tb + c, v);
+            tmem_wait_ld();
+            if (!mine) continue;
+            if (S > 1) {  // this CTA's share of the columns, added below
+              float4* p = (float4*)(sD + (quarter * 32 + lane) * args.R + c);
 #pragma unroll
-          for (int j = 0; j < 16; j++) p[j] = __uint_as_float(v[j]);
-          continue;
-        }
-        T hi[16], lo[16];
+              for (int j = 0; j < 4; j++)
+                p[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+              continue;
+            }
+            alignas(16) T hi[16], lo[16];
 #pragma unroll
-        for (int j = 0; j < 16; j++) split2<T>(c + j < args.rank ? sc * __uint_as_float(v[j]) : 0.f, hi[j], lo[j]);
-        if (a >= 0) {
-          uint4* ph = (uint4*)(Q + (int64_t)row * args.ucols + c);
-          uint4* pl = (uint4*)(Q + (int64_t)row * args.ucols + half + c);
-          ph[0] = ((const uint4*)hi)[0];
-          ph[1] = ((const uint4*)hi)[1];
-          pl[0] = ((const uint4*)lo)[0];
-          pl[1] = ((const uint4*)lo)[1];
+            for (int j = 0; j < 16; j++) split2<T>(c + j < args.rank ? sc * __uint_as_float(v[j]) : 0.f, hi[j], lo[j]);
+            uint4 *ph = (uint4*)(Q + c), *pl = (uint4*)(Q + half + c);
+            ph[0] = ((const uint4*)hi)[0];
+            ph[1] = ((const uint4*)hi)[1];
+            pl[0] = ((const uint4*)lo)[0];
+            pl[1] = ((const uint4*)lo)[1];
+          }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[acc]);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[acc]);
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
   }
   if (threadIdx.x == 0 && *abort) {  // after a timeout, let copies still in flight land before the CTA exits
@@ -268,20 +261,31 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
   tc_fence_before();
   if (S > 1) {
     cluster_sync();
-    // rank r adds rows [r·128/S, (r+1)·128/S) of all the CTAs' shares
-    const int m0 = first * BM, rows = BM / S;
-    T* Q = (T*)args.Q;
-    for (int e = threadIdx.x; e < rows * args.R; e += TC_THREADS) {
-      const int lr = rank * rows + e / args.R, c = e % args.R, row = m0 + lr;
-      const int a = row < args.T ? __ldg(args.row_adapter + row) : -1;
+    // one item per cluster: rank r adds rows [r·128/S, (r+1)·128/S) of all the CTAs' shares
+    const int t = first >= args.ntiles ? first - args.ntiles : first, m0 = t * BM, rows = BM / S;
+    T* Q = (T*)args.job[first >= args.ntiles].Q;
+    for (int lr = rank * rows + (int)threadIdx.x / 16; lr < (rank + 1) * rows; lr += TC_THREADS / 16) {
+      const int row = m0 + lr;
+      int a = -1;
+      for (int s = __ldg(args.tile_first + t); s < args.nsegs; s++) {
+        const int4 g = __ldg(&args.segs[s]);
+        if (g.x > row) break;
+        if (row < g.y) {
+          a = g.z;
+          break;
+        }
+      }
       if (a < 0) continue;
-      const uint32_t at = smem_u32(smem) + (uint32_t)(lr * args.R + c) * 4;
-      float v = 0.f;
-      for (int q = 0; q < S; q++) v += ld_cluster_f32(mapa_rank(at, (uint32_t)q));
-      T hi, lo;
-      split2<T>(c < args.rank ? (args.scales ? __ldg(args.scales + a) : 1.f) * v : 0.f, hi, lo);
-      Q[(int64_t)row * args.ucols + c] = hi;
-      Q[(int64_t)row * args.ucols + args.ucols / 2 + c] = lo;
+      const float sc = args.scales ? __ldg(args.scales + a) : 1.f;
+      for (int c = threadIdx.x & 15; c < args.R; c += 16) {
+        const uint32_t at = smem_u32(sD + lr * args.R + c);
+        float v = 0.f;
+        for (int q = 0; q < S; q++) v += ld_cluster_f32(mapa_rank(at, (uint32_t)q));
+        T hi, lo;
+        split2<T>(c < args.rank ? sc * v : 0.f, hi, lo);
+        Q[(int64_t)row * args.ucols + c] = hi;
+        Q[(int64_t)row * args.ucols + args.ucols / 2 + c] = lo;
+      }
     }
     cluster_sync();  // no CTA leaves while another reads its shared memory
   } else {
@@ -299,43 +303,56 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
 // one adapter: both operands are read MN-major from the row-major blocks that
 // TMA brings (their rows are the contraction). N covers the high and the
 // remainder parts of up to 64 rank rows; the epilogue adds the two. A block
-// that ends inside its adapter's rows loads rows of other requests too: the
-// MMA warp writes zeros over them, up to the next multiple of 16, before the
-// MMA reads them, and issues no steps past that.
+// that ends inside its adapter's rows is loaded up to the next multiple of 16
+// rows, which may be another request's: a warp of its own writes zeros over
+// those before the MMA reads them (a product with zero would let an inf or NaN
+// of that request through).
 //
 // The blocks of all adapters, in adapter order, are cut into G equal runs; a
-// CTA takes one run for one 128-column tile (and one group of 64 rank rows).
-// A run that holds all of an adapter's blocks stores dP; otherwise it stores
-// an f32 partial, in slot run + adapter (distinct for every pair that
-// occurs), and k_outer_join adds an adapter's partials in the order of the
-// runs: the same bits every time, without atomics. Bound by the read of X.
-struct OuterArgs {
-  int C, rank, nchunks, n, G, ucols, rgroups, nmma, stages;
-  uint32_t q_bytes, tmem_cols;
-  const int4* chunks;     // row0, rows, adapter
-  const int32_t* chunk_ptr;
-  float* part;
+// CTA takes one run for one 128-column tile (and one group of 64 rank rows) of
+// one or two products. A run that holds all of an adapter's blocks stores dP;
+// otherwise it stores an f32 partial, in slot run + adapter (distinct for every
+// pair that occurs), counts itself in, and the last of the adapter's runs to
+// arrive adds all partials in the order of the runs: the same bits every time.
+// Bound by the read of X.
+constexpr int OUTER_THREADS = TC_THREADS + 32;  // and the warp that clears rows
+struct OuterJob {
+  CUtensorMap tmX, tmQ, tmX16, tmQ16;  // boxes of 64 and of 16 rows
+  float* part;                         // [G + n, rank, C]
+  uint32_t* count;                     // [n, ctiles, rgroups]: runs that have stored their partial
   void* dP;
+  int C, ctiles;
+};
+struct OuterArgs {
+  OuterJob job[2];
+  int rank, nchunks, n, G, ucols, rgroups, nmma, stages;
+  uint32_t q_bytes, tmem_cols;
+  const int4* chunks;  // row0, rows, adapter
+  const int32_t* chunk_ptr;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(TC_THREADS, 1) k_outer_tc(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmQ,
-                                                            const __grid_constant__ OuterArgs args) {
+__global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_constant__ OuterArgs args) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t stage_bytes = X_BYTES + args.q_bytes;
   uint64_t* full = (uint64_t*)(smem + args.stages * stage_bytes);
   uint64_t* empty = full + args.stages;
-  uint64_t* tfull = empty + args.stages;
+  uint64_t* cleared = empty + args.stages;
+  uint64_t* tfull = cleared + args.stages;
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = (uint32_t*)(tempty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
+  volatile int* arrived = abort + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c0 = blockIdx.x * BM, g = blockIdx.y, j0 = blockIdx.z * 64;
+  const bool second = (int)blockIdx.x >= args.job[0].ctiles;
+  const OuterJob& job = args.job[second];
+  const int ct = second ? (int)blockIdx.x - args.job[0].ctiles : (int)blockIdx.x;
+  const int c0 = ct * BM, g = blockIdx.y, j0 = blockIdx.z * 64;
   const int lo = (int)((int64_t)g * args.nchunks / args.G), hi = (int)((int64_t)(g + 1) * args.nchunks / args.G);
-  pdl_trigger();
+  const int blocks = (int)(stage_bytes >> 13);  // 64 x 64 blocks of a stage
   if (threadIdx.x == 0) {
-    for (int s = 0; s < args.stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    for (int s = 0; s < args.stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1), mbar_init(&cleared[s], 1);
     for (int a = 0; a < 2; a++) mbar_init(&tfull[a], 1), mbar_init(&tempty[a], 4);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -347,20 +364,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_outer_tc(const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
+  pdl_trigger();
 
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0, used = 0, last_phase = 0;
       for (int c = lo; c < hi; c++) {
-        const int row0 = __ldg(&args.chunks[c]).x;
+        const int4 ch = __ldg(&args.chunks[c]);
         if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_adapter_err)) break;
         uint8_t* st = smem + stage * stage_bytes;
-        mbar_arrive_expect_tx(&full[stage], stage_bytes);
-        tma_load_2d(st, &tmX, &full[stage], c0, row0);
-        tma_load_2d(st + 8192, &tmX, &full[stage], c0 + 64, row0);
-        tma_load_2d(st + X_BYTES, &tmQ, &full[stage], j0, row0);
-        if (args.q_bytes > 8192) tma_load_2d(st + X_BYTES + 8192, &tmQ, &full[stage], args.ucols / 2 + j0, row0);
+        const int n16 = (ch.y + 15) >> 4;
+        mbar_arrive_expect_tx(&full[stage], (uint32_t)(blocks * n16) * 2048);
+        auto bring = [&](uint8_t* dst, const CUtensorMap* big, const CUtensorMap* small, int x) {
+          if (n16 == 4) tma_load_2d(dst, big, &full[stage], x, ch.x);
+          else
+            for (int i = 0; i < n16; i++) tma_load_2d(dst + i * 2048, small, &full[stage], x, ch.x + 16 * i);
+        };
+        bring(st, &job.tmX, &job.tmX16, c0);
+        bring(st + 8192, &job.tmX, &job.tmX16, c0 + 64);
+        bring(st + X_BYTES, &job.tmQ, &job.tmQ16, j0);
+        if (blocks == 4) bring(st + X_BYTES + 8192, &job.tmQ, &job.tmQ16, args.ucols / 2 + j0);
         used |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
         if (++stage == args.stages) { stage = 0; phase ^= 1; }
@@ -372,61 +396,85 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_outer_tc(const __grid_constan
         }
     }
   } else if (warp == 1) {
-    const uint32_t idesc = idesc_rt<T>(args.nmma, true, true);
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    bool ok = true;
-    uint64_t* last = nullptr;
-    uint32_t last_phase = 0;
-    for (int c = lo; c < hi && ok;) {
-      const int a = __ldg(&args.chunks[c]).z, end = min(hi, __ldg(args.chunk_ptr + a + 1)), begin = c;
-      if (!__all_sync(0xffffffffu, mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_adapter_err))) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t d = tmem + (uint32_t)(acc * args.nmma);
-      for (; c < end; c++) {
-        const int rows = __ldg(&args.chunks[c]).y, steps = (rows + 15) >> 4;
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort, &g_adapter_err))) { ok = false; break; }
-        uint8_t* st = smem + stage * stage_bytes;
-        if (rows & 15) {  // rows of other requests in the last step: zeros in both operands
-          const int z0 = rows * 128, zn = (steps * 16 - rows) * 8;  // 16-byte pieces per 64-column block
-          const int blocks = (int)(stage_bytes >> 13);
-          for (int i = lane; i < zn * blocks; i += 32) *(uint4*)(st + (i / zn) * 8192 + z0 + (i % zn) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
+    if (lane == 0) {
+      const uint32_t idesc = idesc_rt<T>(args.nmma, true, true);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      uint64_t* last = nullptr;
+      uint32_t last_phase = 0;
+      for (int c = lo; c < hi && ok;) {
+        const int a = __ldg(&args.chunks[c].z), end = min(hi, __ldg(args.chunk_ptr + a + 1)), begin = c;
+        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t a0 = smem_u32(st), b0 = a0 + X_BYTES;
+        const uint32_t d = tmem + (uint32_t)(acc * args.nmma);
+        for (; c < end; c++) {
+          const int rows = __ldg(&args.chunks[c].y), steps = (rows + 15) >> 4;
+          if (!mbar_wait(&full[stage], phase, abort, &g_adapter_err)) { ok = false; break; }
+          if (!mbar_wait(&cleared[stage], phase, abort, &g_adapter_err)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(smem + stage * stage_bytes), b0 = a0 + X_BYTES;
           for (int k = 0; k < steps; k++)
             tc_mma(d, sdesc_sw128_mn(a0 + k * 2048, 8192), sdesc_sw128_mn(b0 + k * 2048, 8192), idesc, (c > begin || k > 0) ? 1u : 0u);
           tc_commit(&empty[stage]);
+          last = &empty[stage];
+          last_phase = phase;
+          if (++stage == args.stages) { stage = 0; phase ^= 1; }
         }
-        __syncwarp();
-        last = &empty[stage];
-        last_phase = phase;
-        if (++stage == args.stages) { stage = 0; phase ^= 1; }
+        if (!ok) break;
+        tc_commit(&tfull[acc]);
+        last = &tfull[acc];
+        last_phase = acc_phase;
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
-      if (!ok) break;
-      if (lane == 0) tc_commit(&tfull[acc]);
-      __syncwarp();
-      last = &tfull[acc];
-      last_phase = acc_phase;
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      if (last) {
+        const uint64_t t0 = gtimer();
+        while (!mbar_try_wait(last, last_phase) && gtimer() - t0 < kWaitNs) {}
+      }
     }
-    if (last) {
-      const uint64_t t0 = gtimer();
-      while (!mbar_try_wait(last, last_phase) && gtimer() - t0 < kWaitNs) {}
+  } else if (warp == 6) {
+    // clears the rows of a block that are not its adapter's; passes on every
+    // block, so that it is never a whole turn of the ring ahead or behind
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int c = lo; c < hi; c++) {
+      const int rows = __ldg(&args.chunks[c].y);
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort, &g_adapter_err))) break;
+      if (rows & 15) {
+        uint8_t* st = smem + stage * stage_bytes + rows * 128;
+        const int zn = (16 - (rows & 15)) * 8;  // 16-byte pieces per 64-column block
+        for (int k = 0; k < blocks; k++)
+          for (int i = lane; i < zn; i += 32) *(uint4*)(st + k * 8192 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&cleared[stage]);
+      if (++stage == args.stages) { stage = 0; phase ^= 1; }
     }
     __syncwarp();
   } else {
     const int quarter = warp & 3, col = c0 + quarter * 32 + lane;
     const int nh = args.nmma / 2;  // rank rows of this CTA, rounded up
+    const int64_t size = (int64_t)args.rank * job.C;
+    T* dP = (T*)job.dP;
+    // barriers of the four epilogue warps, which take the same turns; all4 says whether the condition holds for all of them
+    auto sync4 = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    auto all4 = [](bool p) {
+      uint32_t r;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(r)
+          : "r"((uint32_t)p)
+          : "memory");
+      return r != 0;
+    };
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int c = lo; c < hi;) {
-      const int a = __ldg(&args.chunks[c]).z, p0 = __ldg(args.chunk_ptr + a), p1 = __ldg(args.chunk_ptr + a + 1);
+      const int a = __ldg(&args.chunks[c].z), p0 = __ldg(args.chunk_ptr + a), p1 = __ldg(args.chunk_ptr + a + 1);
       const bool whole = p0 >= lo && p1 <= hi;
-      if (!mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err)) break;
+      // a timeout ends the loop of all epilogue warps: none is left at a barrier below
+      if (!all4(mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err))) break;
       tc_fence_after();
       const uint32_t tb = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * args.nmma);
       for (int j = 0; j < nh; j += 16) {
@@ -437,10 +485,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_outer_tc(const __grid_constan
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           const int row = j0 + j + i;
-          if (row < args.rank && col < args.C) {
+          if (row < args.rank && col < job.C) {
             const float v = __uint_as_float(vh[i]) + __uint_as_float(vl[i]);
-            if (whole) ((T*)args.dP)[((int64_t)a * args.rank + row) * args.C + col] = TcFmt<T>::cvt(v);
-            else args.part[((int64_t)(g + a) * args.rank + row) * args.C + col] = v;
+            if (whole) dP[a * size + (int64_t)row * job.C + col] = TcFmt<T>::cvt(v);
+            else job.part[(g + a) * size + (int64_t)row * job.C + col] = v;
           }
         }
       }
@@ -448,8 +496,40 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_outer_tc(const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      if (!whole) {  // the runs of the first and the last block: run g begins at floor(g·nchunks / G)
+        const int g0 = (int)((((int64_t)p0 + 1) * args.G - 1) / args.nchunks), g1 = (int)(((int64_t)p1 * args.G - 1) / args.nchunks);
+        __threadfence();
+        sync4();
+        if (warp == 2 && lane == 0) {
+          const uint32_t was = atomicAdd(job.count + ((int64_t)a * job.ctiles + ct) * args.rgroups + blockIdx.z, 1u);
+          *arrived = was == (uint32_t)(g1 - g0);
+        }
+        sync4();
+        const bool join = *arrived != 0;
+        if (join && col < job.C) {
+          __threadfence();
+          for (int j = 0; j < nh; j += 16) {
+            float v[16] = {};
+#pragma unroll 4
+            for (int q = g0; q <= g1; q++) {
+              const float* p = job.part + (q + a) * size + (int64_t)(j0 + j) * job.C + col;
+#pragma unroll
+              for (int i = 0; i < 16; i++)
+                if (j0 + j + i < args.rank) v[i] += __ldcg(p + (int64_t)i * job.C);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+              if (j0 + j + i < args.rank) dP[a * size + (int64_t)(j0 + j + i) * job.C + col] = TcFmt<T>::cvt(v[i]);
+          }
+        }
+        sync4();  // `arrived` is read before it is written again
+      }
       c = min(hi, p1);
     }
+    if (g == 0 && col < job.C)  // adapters without rows
+      for (int a = 0; a < args.n; a++)
+        if (__ldg(args.chunk_ptr + a) == __ldg(args.chunk_ptr + a + 1))
+          for (int j = j0; j < min(args.rank, j0 + nh); j++) dP[a * size + (int64_t)j * job.C + col] = TcFmt<T>::cvt(0.f);
   }
   if (threadIdx.x == 0 && *abort) {
     const uint64_t t0 = gtimer();
@@ -463,27 +543,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_outer_tc(const __grid_constan
   }
 }
 
-// dP of the adapters whose blocks lie in several runs (the sum of their
-// partials) or that have no blocks (zeros).
-template <typename T>
-__global__ void __launch_bounds__(256) k_outer_join(const float* __restrict__ part, const int32_t* __restrict__ chunk_ptr, T* __restrict__ dP,
-                                                    int nchunks, int G, int64_t size) {
-  pdl_trigger();
-  pdl_wait();
-  const int a = blockIdx.y, p0 = chunk_ptr[a], p1 = chunk_ptr[a + 1];
-  int g0 = 0, g1 = -1;
-  if (p1 > p0) {  // the runs of the first and the last block: run g begins at floor(g·nchunks / G)
-    g0 = (int)((((int64_t)p0 + 1) * G - 1) / nchunks);
-    g1 = (int)(((int64_t)p1 * G - 1) / nchunks);
-    if (g0 == g1) return;
-  }
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-    float v = 0.f;
-    for (int g = g0; g <= g1; g++) v += part[(int64_t)(g + a) * size + i];
-    dP[(int64_t)a * size + i] = from_f<T>(v);
-  }
-}
-
 uint32_t tmem_columns(int want) {
   uint32_t c = 32;
   while ((int)c < want) c *= 2;
@@ -491,35 +550,44 @@ uint32_t tmem_columns(int want) {
 }
 
 template <typename T>
-void shrink_t(const AdapterShrink& c, const AdapterPlan& p, cudaStream_t st) {
+void shrink_t(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, const AdapterPlan& p, cudaStream_t st) {
   const int dtype = std::is_same<T, __half>::value ? LC_F16 : LC_BF16;
   ShrinkArgs a{};
+  a.njobs = njobs;
   a.T = p.rows;
-  a.C = (int)c.C;
   a.ntiles = (p.rows + BM - 1) / BM;
   a.nsegs = p.nsegs;
-  a.rank = c.rank;
-  a.R = adapter_u_cols(c.rank) / 2;
-  a.nb = std::max(1, std::min(4, 64 / a.R));
+  a.rank = c[0].rank;
+  a.ucols = adapter_u_cols(a.rank);
+  a.R = a.ucols / 2;
+  // adapters side by side: 128 columns of D, 192 for rank 64 (a ragged tile of
+  // 128 rows meets two or three requests), which leaves five stages or more
+  a.nb = a.R <= 32 ? 128 / a.R : a.R == 64 ? 3 : 1;
   a.bank_bytes = (uint32_t)(a.nb * a.R * 128);
-  a.stages = std::min(8, (int)((200u << 10) / (X_BYTES + a.bank_bytes)));
-  a.ucols = adapter_u_cols(c.rank);
-  a.tmem_cols = tmem_columns(2 * a.R);
+  a.tmem_cols = tmem_columns(2 * a.nb * a.R);
   a.segs = p.segs;
   a.tile_first = p.tile_first;
-  a.row_adapter = p.row_adapter;
-  a.scales = c.scales;
-  a.Q = c.Q;
-  const CUtensorMap mx = tensor_map_2d(c.X, p.rows, c.C, c.ld, BK, BM, dtype);
-  const CUtensorMap mp = tensor_map_3d(c.P, c.n, c.rank, c.C, c.ldp, a.R, dtype);
-  const int KB = (a.C + BK - 1) / BK;
-  int S = 1;
+  a.scales = c[0].scales;
+  a.zero = zero;
+  a.nzero = (int)nzero;
+  int KB = INT32_MAX;
+  for (int j = 0; j < njobs; j++) {
+    a.job[j].tmX = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, BK, BM, dtype);
+    a.job[j].tmP = tensor_map_3d(c[j].P, c[j].n, c[j].rank, c[j].C, c[j].ldp, a.R, dtype);
+    a.job[j].Q = c[j].Q;
+    a.job[j].C = (int)c[j].C;
+    KB = std::min(KB, (a.job[j].C + BK - 1) / BK);
+  }
+  const int64_t items = (int64_t)njobs * a.ntiles;
+  a.S = 1;
   for (int f : {8, 4, 2})
-    if (a.ntiles * f <= num_sms() && KB >= 2 * f) {
-      S = f;
+    if (a.R <= 64 && items * f <= num_sms() && KB >= 2 * f) {
+      a.S = f;
       break;
     }
-  const size_t smem = (size_t)a.stages * (X_BYTES + a.bank_bytes) + 1024 + 512;
+  const size_t d_bytes = a.S > 1 ? (size_t)BM * a.R * 4 : 0;
+  a.stages = std::min(8, (int)(((224u << 10) - d_bytes) / (X_BYTES + a.bank_bytes)));
+  const size_t smem = (size_t)a.stages * (X_BYTES + a.bank_bytes) + d_bytes + 1024 + 512;
   static bool attr = false;
   if (!attr) {
     CUDA_OK(cudaFuncSetAttribute(k_shrink_tc<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 << 10));
@@ -528,32 +596,30 @@ void shrink_t(const AdapterShrink& c, const AdapterPlan& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   int n = 0;
-  if (S > 1) {
+  if (a.S > 1) {
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = S;
+    at[0].val.clusterDim.x = a.S;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     n = 1;
   }
-  cfg.gridDim = dim3(S > 1 ? S * a.ntiles : std::min(a.ntiles, num_sms()));
+  cfg.gridDim = dim3((unsigned)(a.S > 1 ? a.S * items : std::min<int64_t>(items, num_sms())));
   cfg.blockDim = dim3(TC_THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   chain_attrs(cfg, at, n);
-  CUDA_OK(cudaLaunchKernelEx(&cfg, k_shrink_tc<T>, mx, mp, a, S));
+  CUDA_OK(cudaLaunchKernelEx(&cfg, k_shrink_tc<T>, a));
   LC_LAUNCHED(1);
 }
 
 template <typename T>
-void outer_t(const AdapterOuter& c, const AdapterPlan& p, cudaStream_t st) {
+void outer_t(const AdapterOuter* c, int njobs, const AdapterPlan& p, cudaStream_t st) {
   const int dtype = std::is_same<T, __half>::value ? LC_F16 : LC_BF16;
-  const int64_t size = (int64_t)c.rank * c.C;
   OuterArgs a{};
-  a.C = (int)c.C;
-  a.rank = c.rank;
+  a.rank = c[0].rank;
   a.nchunks = p.nchunks;
   a.n = p.n_adapters;
-  a.ucols = adapter_u_cols(c.rank);
+  a.ucols = adapter_u_cols(a.rank);
   a.rgroups = std::max(1, a.ucols / 128);
   a.nmma = std::min(a.ucols, 128);
   a.q_bytes = a.ucols > 64 ? 16384 : 8192;
@@ -561,39 +627,35 @@ void outer_t(const AdapterOuter& c, const AdapterPlan& p, cudaStream_t st) {
   a.tmem_cols = tmem_columns(2 * a.nmma);
   a.chunks = p.chunks;
   a.chunk_ptr = p.chunk_ptr;
-  a.dP = c.dP;
-  const int ct = (int)((c.C + BM - 1) / BM) * a.rgroups, sms = num_sms();
-  // runs: one wave of CTAs at least, and whole waves as far as 16 runs can make them
-  int G = 1;
-  double best = 0;
-  for (int f = 1; f <= 64 && f <= p.nchunks; f++) {
-    const int64_t ctas = (int64_t)ct * f, waves = (ctas + sms - 1) / sms;
-    const double fill = (double)ctas / (double)(waves * sms);
-    if (fill > best + 0.03) best = fill, G = f;
-    if (waves > 2) break;
-  }
-  a.G = G;
+  int ctiles = 0;
+  for (int j = 0; j < njobs; j++) ctiles += (int)((c[j].C + BM - 1) / BM);
+  a.G = adapter_runs(ctiles * a.rgroups, p.nchunks);
   struct Partials {
-    void* p = nullptr;
-    ~Partials() { if (p) dfree(p); }
+    void* p[2] = {nullptr, nullptr};
+    ~Partials() {
+      for (void* q : p)
+        if (q) dfree(q);
+    }
   } part;
-  if (G > 1) part.p = dmalloc((size_t)(G + p.n_adapters) * size * 4);
-  a.part = (float*)part.p;
-  const CUtensorMap mx = tensor_map_2d(c.X, p.rows, c.C, c.ld, 64, 64, dtype);
-  const CUtensorMap mq = tensor_map_2d(c.Q, p.rows, a.ucols, a.ucols, 64, 64, dtype);
+  for (int j = 0; j < njobs; j++) {
+    OuterJob& o = a.job[j];
+    o.C = (int)c[j].C;
+    o.ctiles = (o.C + BM - 1) / BM;
+    o.tmX = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 64, dtype);
+    o.tmQ = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 64, dtype);
+    o.tmX16 = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 16, dtype);
+    o.tmQ16 = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 16, dtype);
+    o.dP = c[j].dP;
+    o.count = c[j].count;
+    if (a.G > 1) o.part = (float*)(part.p[j] = dmalloc((size_t)(a.G + p.n_adapters) * a.rank * c[j].C * 4));
+  }
   const size_t smem = (size_t)a.stages * (X_BYTES + a.q_bytes) + 1024 + 512;
   static bool attr = false;
   if (!attr) {
     CUDA_OK(cudaFuncSetAttribute(k_outer_tc<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 << 10));
     attr = true;
   }
-  LC_CHECK(p.n_adapters <= 65535, "adapters: more than 65535 adapters");
-  if (p.nchunks) {
-    launch_chain(k_outer_tc<T>, dim3((unsigned)((c.C + BM - 1) / BM), (unsigned)G, (unsigned)a.rgroups), dim3(TC_THREADS), smem, st, mx, mq, a);
-    LC_LAUNCHED(1);
-  }
-  launch_chain(k_outer_join<T>, dim3((unsigned)std::min<int64_t>((size + 1023) / 1024, 256), (unsigned)p.n_adapters), dim3(256), 0, st,
-               (const float*)part.p, (const int32_t*)p.chunk_ptr, (T*)c.dP, p.nchunks, G, size);
+  launch_chain(k_outer_tc<T>, dim3((unsigned)ctiles, (unsigned)a.G, (unsigned)a.rgroups), dim3(OUTER_THREADS), smem, st, a);
   LC_LAUNCHED(1);
 }
 
@@ -601,14 +663,32 @@ void outer_t(const AdapterOuter& c, const AdapterPlan& p, cudaStream_t st) {
 
 namespace lc {
 
-void adapter_shrink_tc(const AdapterShrink& c, const AdapterPlan& p, int dtype, cudaStream_t st) {
+void adapter_shrink_tc(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, const AdapterPlan& p, int dtype, cudaStream_t st) {
   if (!p.nsegs) return;
-  dtype == LC_F16 ? shrink_t<__half>(c, p, st) : shrink_t<__nv_bfloat16>(c, p, st);
+  LC_CHECK(nzero <= INT32_MAX, "adapters: too many adapters");
+  dtype == LC_F16 ? shrink_t<__half>(c, njobs, zero, nzero, p, st) : shrink_t<__nv_bfloat16>(c, njobs, zero, nzero, p, st);
 }
 
-void adapter_outer_tc(const AdapterOuter& c, const AdapterPlan& p, int dtype, cudaStream_t st) {
-  if (!p.n_adapters) return;
-  dtype == LC_F16 ? outer_t<__half>(c, p, st) : outer_t<__nv_bfloat16>(c, p, st);
+int adapter_runs(int tiles, int nchunks) {
+  // one wave of CTAs, or two where one would leave SMs idle
+  const int sms = num_sms();
+  int G = 1;
+  double best = 0;
+  for (int f = 1; f <= 64 && f <= nchunks; f++) {
+    const int64_t ctas = (int64_t)tiles * f, waves = (ctas + sms - 1) / sms;
+    const double fill = (double)ctas / (double)(waves * sms);
+    if (fill > best + 0.03) best = fill, G = f;
+    if (waves > 2) break;
+  }
+  return G;
+}
+
+size_t adapter_count_words(const AdapterPlan& p, int rank, int64_t C) {
+  return (size_t)p.n_adapters * ((C + BM - 1) / BM) * std::max(1, adapter_u_cols(rank) / 128);
+}
+
+void adapter_outer_tc(const AdapterOuter* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st) {
+  dtype == LC_F16 ? outer_t<__half>(c, njobs, p, st) : outer_t<__nv_bfloat16>(c, njobs, p, st);
 }
 
 std::string take_adapter_errors() {

@@ -82,8 +82,18 @@ struct GemmAdapted {
   int half;                   // steps after which P's rows start over (high and low part in one block), else ksteps
   int pgroups;                // 64-row blocks of P_a
   int prows;                  // rows of P_a per block (box height of tmP)
+  int per;                    // segments whose blocks of P share a stage (64 / prows; 1 with several blocks of U)
+  int defer;                  // x, w and bias were complete when the previous kernel let this one start: only U waits for it
   int kb_off;                 // added to the K block of the main loop's loads (past the operands' end: zeros)
 };
+
+// The segments of one stage: s, s + 1, ... that begin before row `end`; 0 when the tile is done.
+template <bool WT>
+__device__ __forceinline__ int stage_segments(const GemmAdapted<WT>& ex, int s, int end) {
+  int n = 0;
+  while (n < ex.per && s + n < ex.nsegs && __ldg(&ex.segs[s + n].x) < end) n++;
+  return n;
+}
 
 __device__ __forceinline__ float gelu_exact(float x) { return 0.5f * x * (1.0f + erff(x * 0.7071067811865476f)); }
 
@@ -1003,7 +1013,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
     const size_t lo = per * blockIdx.x, hi = lo + per < total ? lo + per : total;
     for (size_t o = lo; o < hi; o += 65536) bulk_prefetch_l2((const char*)args.ep.l2_next + o, (uint32_t)(hi - o < 65536 ? hi - o : 65536));
   }
-  if (!QB) pdl_wait();  // the kernel that wrote the activations has completed
+  if constexpr (EX::kOn) {
+    if (!ex.defer) pdl_wait();
+  } else if (!QB) {
+    pdl_wait();  // the kernel that wrote the activations has completed
+  }
 
   if (warp == 0) {
     // ---------------- TMA producer
@@ -1046,20 +1060,22 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
         }
         if constexpr (EX::kOn) {
           if (kb1 < KB) continue;  // another slice of K takes the adapters
-          for (int s = __ldg(ex.tile_first + m0 / BM); s < ex.nsegs && ok; s++) {
-            const int4 seg = __ldg(ex.segs + s);
-            if (seg.x >= m0 + BM) break;
+          if (ex.defer) pdl_wait();  // the kernel that wrote U
+          int n;
+          for (int s = __ldg(ex.tile_first + m0 / BM); ok && (n = stage_segments(ex, s, m0 + BM)); s += n)
             for (int c = 0; c < ex.nchunks; c++) {
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
-              mbar_arrive_expect_tx(&full[stage], A_BYTES + (BN / 64) * ex.prows * 128);
+              mbar_arrive_expect_tx(&full[stage], A_BYTES + n * (BN / 64) * ex.prows * 128);
               tma_load_2d(sA + stage * A_BYTES, &ex.tmU, &full[stage], c * 64, m0);
-              for (int h = 0; h < BN / 64; h++)
-                tma_load_3d(sB + stage * B_BYTES + h * 8192, &ex.tmP, &full[stage], n0 + 64 * h, (c % ex.pgroups) * 64, seg.z);
+              for (int i = 0; i < n; i++) {
+                const int a = __ldg(&ex.segs[s + i].z);
+                for (int h = 0; h < BN / 64; h++)
+                  tma_load_3d(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, (c % ex.pgroups) * 64, a);
+              }
               issued[stage] = 1;
               iss_phase[stage] = phase;
               if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
-          }
         }
       }
       // drain: every copy this thread issued must have landed before the CTA exits
@@ -1110,24 +1126,26 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
         }
         if constexpr (EX::kOn) {
           const int m0 = ((w / S) / args.ntile_n) * BM;
-          for (int s = kb1 < KB ? ex.nsegs : __ldg(ex.tile_first + m0 / BM); s < ex.nsegs && ok; s++) {
-            const int4 seg = __ldg(ex.segs + s);
-            if (seg.x >= m0 + BM) break;
-            uint32_t off[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) off[i] = lanes_off(m0 + 32 * i, seg.x, seg.y);
+          int n;
+          for (int s = kb1 < KB ? ex.nsegs : __ldg(ex.tile_first + m0 / BM); ok && (n = stage_segments(ex, s, m0 + BM)); s += n)
             for (int c = 0; c < ex.nchunks; c++) {
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
               tc_fence_after();
               const uint32_t a0 = smem_u32(sA + stage * A_BYTES), b0 = smem_u32(sB + stage * B_BYTES);
-              for (int k = 0; k < ex.ksteps; k++)
-                tc_mma_lanes(d, sdesc_sw128(a0 + k * 32), sdesc_sw128_mn(b0 + (k >= ex.half ? k - ex.half : k) * 2048, 8192), idesc_t, 1u, off);
+              for (int i = 0; i < n; i++) {
+                const int4 seg = __ldg(ex.segs + s + i);
+                uint32_t off[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
+                for (int k = 0; k < ex.ksteps; k++)
+                  tc_mma_lanes(d, sdesc_sw128(a0 + k * 32), sdesc_sw128_mn(b0 + i * ex.prows * 128 + (k >= ex.half ? k - ex.half : k) * 2048, 8192),
+                               idesc_t, 1u, off);
+              }
               tc_commit(&empty[stage]);
               last = &empty[stage];
               last_phase = phase;
               if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
-          }
         }
         if (!ok) break;
         tc_commit(&tfull[acc]);
@@ -1244,6 +1262,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
     const uint64_t t0 = gtimer();
     while (gtimer() - t0 < 1000000ull) {}
   }
+  if constexpr (EX::kOn) pdl_wait();  // this kernel is not done before the ones it follows
   tc_fence_before();
   if constexpr (KS) cluster_sync();  // no CTA leaves while another may read its partial or arrive on its barriers
   else __syncthreads();
@@ -1320,7 +1339,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
   cluster_sync();  // both CTAs' barriers exist before any remote arrival or copy
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();  // the kernel that wrote the activations has completed
+  if constexpr (EX::kOn) {
+    if (!ex.defer) pdl_wait();
+  } else {
+    pdl_wait();  // the kernel that wrote the activations has completed
+  }
 
   if (warp == 0) {
     // ---------------- TMA producer (both CTAs)
@@ -1350,20 +1373,23 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
         }
         if constexpr (EX::kOn) {
           const int t0 = (t / args.ntile_n) * (2 * BM);
-          for (int s = __ldg(ex.tile_first + t0 / BM); s < ex.nsegs && ok; s++) {
-            const int4 seg = __ldg(ex.segs + s);
-            if (seg.x >= t0 + 2 * BM) break;
+          if (ex.defer) pdl_wait();  // the kernel that wrote U
+          int n;
+          for (int s = __ldg(ex.tile_first + t0 / BM); ok && (n = stage_segments(ex, s, t0 + 2 * BM)); s += n)
             for (int c = 0; c < ex.nchunks; c++) {
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
-              if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (A_BYTES + 2 * ex.prows * 128));
+              if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (A_BYTES + n * 2 * ex.prows * 128));
               tma_load_2d_pair(sA + stage * A_BYTES, &ex.tmU, full0 + 8 * stage, c * 64, m0);
-              for (int h = 0; h < 2; h++)
-                tma_load_3d_pair(sB + stage * B_BYTES + h * 8192, &ex.tmP, full0 + 8 * stage, n0 + 64 * h, (c % ex.pgroups) * 64, seg.z);
+              for (int i = 0; i < n; i++) {
+                const int a = __ldg(&ex.segs[s + i].z);
+                for (int h = 0; h < 2; h++)
+                  tma_load_3d_pair(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, full0 + 8 * stage, n0 + 64 * h,
+                                   (c % ex.pgroups) * 64, a);
+              }
               issued[stage] = 1;
               iss_phase[stage] = phase;
               if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
-          }
         }
       }
       // drain: each stage's last fill has been consumed by the pair's MMAs (so it landed)
@@ -1409,24 +1435,25 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
         }
         if constexpr (EX::kOn) {
           const int t0 = (t / args.ntile_n) * (2 * BM);
-          for (int s = __ldg(ex.tile_first + t0 / BM); s < ex.nsegs && ok; s++) {
-            const int4 seg = __ldg(ex.segs + s);
-            if (seg.x >= t0 + 2 * BM) break;
-            uint32_t off[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) off[i] = lanes_off(t0 + 32 * i, seg.x, seg.y);
+          int n;
+          for (int s = __ldg(ex.tile_first + t0 / BM); ok && (n = stage_segments(ex, s, t0 + 2 * BM)); s += n)
             for (int c = 0; c < ex.nchunks; c++) {
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
               tc_fence_after();
               const uint64_t da = dA0 + ((stage * A_BYTES) >> 4), db = dBt0 + ((stage * B_BYTES) >> 4);
-              for (int k = 0; k < ex.ksteps; k++)
-                tc_mma_pair_lanes(d, da + k * 2, db + (k >= ex.half ? k - ex.half : k) * 128, idesc_t, 1u, off);
+              for (int i = 0; i < n; i++) {
+                const int4 seg = __ldg(ex.segs + s + i);
+                uint32_t off[8];
+#pragma unroll
+                for (int q = 0; q < 8; q++) off[q] = lanes_off(t0 + 32 * q, seg.x, seg.y);
+                for (int k = 0; k < ex.ksteps; k++)
+                  tc_mma_pair_lanes(d, da + k * 2, db + i * ex.prows * 8 + (k >= ex.half ? k - ex.half : k) * 128, idesc_t, 1u, off);
+              }
               tc_commit_pair(&empty[stage]);
               last = &empty[stage];
               last_phase = phase;
               if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
-          }
         }
         if (!ok) break;
         tc_commit_pair(&tfull[acc]);
@@ -1448,6 +1475,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
     const uint64_t t0 = gtimer();
     while (gtimer() - t0 < 1000000ull) {}
   }
+  if constexpr (EX::kOn) pdl_wait();  // this kernel is not done before the ones it follows
   tc_fence_before();
   cluster_sync();  // no CTA leaves while its partner may still read its shared memory or arrive on its barriers
   if (warp == 1) {
@@ -1782,6 +1810,8 @@ void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
   ex.ksteps = std::min(4, s.u_cols / 16);
   ex.half = s.u_cols <= 64 ? s.u_cols / 32 : 4;
   ex.pgroups = std::max(1, s.u_cols / 128);
+  ex.per = 64 / ex.prows;
+  ex.defer = c.after_share ? 1 : 0;
   ex.kb_off = c.w ? 0 : 1;  // a block past the end of the stand-in maps below, which TMA fills with zeros
   const CUtensorMap ma = c.w ? tensor_map(c.x, c.M, c.K, c.ldx, BK, BM, dtype) : tensor_map(s.u, 1, 8, 8, BK, BM, dtype);
   auto weight_map = [&](int bn) {

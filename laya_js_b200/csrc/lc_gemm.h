@@ -76,6 +76,10 @@ struct GemmAdaptedCall {
   void* y = nullptr;
   int64_t ldy = 0;
   AdapterShare share;
+  // The launch follows a kernel of the same operator that lets its successor
+  // start only once everything before it is complete (x, w and bias are then
+  // read at once, share.u after that kernel).
+  bool after_share = false;
 };
 
 namespace lc {
