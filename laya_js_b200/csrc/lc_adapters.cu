@@ -372,6 +372,10 @@ AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_
   return c;
 }
 
+void shrink(const AdapterShrink* c, int njobs, const Operands& o) {
+  if (!adapter_shrink_rows(c, njobs, *o.plan, o.dtype, stream())) adapter_shrink_tc(c, njobs, *o.plan, o.dtype, stream());
+}
+
 void expand_tc(const Operands& o, const Rows& X, const Rows& W, const Rows& P, const void* Q, bool transposed, LcTensor* Y) {
   GemmAdaptedCall c;
   c.x = X.p;
@@ -395,10 +399,9 @@ void expand_tc(const Operands& o, const Rows& X, const Rows& W, const Rows& P, c
   c.share.rank = o.r;
   c.share.ld = P.ld;
   c.share.segs = o.plan->segs;
-  c.share.tile_first = o.plan->tile_first;
-  c.share.nsegs = o.plan->nsegs;
+  c.share.tiles = o.plan->tiles;
   c.after_share = o.plan->nsegs > 0;
-  gemm_adapted(c, o.dtype, stream());
+  if (!adapter_linear_rows(c, *o.plan, o.dtype, stream())) gemm_adapted(c, o.dtype, stream());
 }
 
 void linear(const Operands& o, LcTensor* y, Held& held) {
@@ -414,7 +417,7 @@ void linear(const Operands& o, LcTensor* y, Held& held) {
              b = pad.of(o.b, (int64_t)o.n * o.r, o.N);
   pad.run();
   const AdapterShrink u = shrink_job(o, x, a, o.K, held);
-  adapter_shrink_tc(&u, 1, nullptr, 0, *o.plan, o.dtype, stream());
+  shrink(&u, 1, o);
   const Chained chained(o);
   expand_tc(o, x, w, b, u.Q, false, y);
 }
@@ -457,7 +460,6 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
   if (!nq) return;
   AdapterOuter out[2];
   int no = 0;
-  size_t words[2] = {0, 0};
   auto job = [&](const void* Q, const Rows& X, int64_t C, LcTensor* dP) {
     AdapterOuter& c = out[no];
     c.X = X.p;
@@ -466,14 +468,11 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
     c.ld = X.ld;
     c.rank = o.r;
     c.dP = dP->data();
-    words[no++] = adapter_count_words(*o.plan, o.r, C);
+    no++;
   };
   if (db) job(u, dy, o.N, db);
   if (da) job(g, x, o.K, da);
-  uint32_t* count = no ? (uint32_t*)held.scratch((words[0] + words[1]) * 4) : nullptr;
-  out[0].count = count;
-  out[1].count = count + words[0];
-  adapter_shrink_tc(q, nq, count, words[0] + words[1], *o.plan, o.dtype, stream());
+  shrink(q, nq, o);
   const Chained chained(o);
   if (no) adapter_outer_tc(out, no, *o.plan, o.dtype, stream());
   if (dx) expand_tc(o, dy, w, a, g, true, dx);
@@ -523,11 +522,13 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   }
   std::vector<int32_t> row_adapter(T, -1);
   for (auto& s : segs) std::fill(row_adapter.begin() + s.lo, row_adapter.begin() + s.hi, s.a);
-  std::vector<int32_t> seg4, tile_first((T + 127) / 128);
+  std::vector<int32_t> seg4, tiles;
   for (auto& g : segs) seg4.insert(seg4.end(), {g.lo, g.hi, g.a, 0});
-  for (size_t i = 0, k = 0; i < tile_first.size(); i++) {
-    while (k < S && segs[k].hi <= (int64_t)i * 128) k++;
-    tile_first[i] = (int32_t)k;
+  for (int64_t m0 = 0, k = 0; m0 < T; m0 += 128) {
+    while (k < (int64_t)S && segs[k].hi <= m0) k++;
+    int64_t e = k;
+    while (e < (int64_t)S && segs[e].lo < m0 + 128) e++;
+    tiles.insert(tiles.end(), {(int32_t)k, (int32_t)(e - k)});
   }
   std::vector<int32_t> chunks, chunk_ptr(n_adapters + 1, 0);
   for (int a = 0; a < n_adapters; a++) {
@@ -543,7 +544,7 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
     image.resize((image.size() + 63) / 64 * 64);
     return off;
   };
-  const size_t o_rows = put(row_adapter), o_spans = put(spans), o_ptr = put(span_ptr), o_segs = put(seg4), o_first = put(tile_first),
+  const size_t o_rows = put(row_adapter), o_spans = put(spans), o_ptr = put(span_ptr), o_segs = put(seg4), o_tiles = put(tiles),
                o_chunks = put(chunks), o_chunk_ptr = put(chunk_ptr);
   struct Guard {
     AdapterPlan* p;
@@ -564,9 +565,10 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   p->spans = (int2*)(p->dev + o_spans);
   p->span_ptr = p->dev + o_ptr;
   p->segs = (int4*)(p->dev + o_segs);
-  p->tile_first = p->dev + o_first;
+  p->tiles = (int2*)(p->dev + o_tiles);
   p->chunks = (int4*)(p->dev + o_chunks);
   p->chunk_ptr = p->dev + o_chunk_ptr;
+  p->host_chunk_ptr = std::move(chunk_ptr);
   plans().insert(p);
   g.p = nullptr;
   *out = reinterpret_cast<uint64_t>(p);

@@ -1,6 +1,7 @@
 // Internal definitions of the adapter operators (include/laya_cuda_adapters.h).
 #pragma once
 #include "lc_common.cuh"
+#include "lc_gemm.h"
 
 constexpr int kAdapterMaxRank = 256;
 
@@ -10,11 +11,12 @@ struct AdapterPlan {
   int32_t* dev = nullptr;          // one allocation behind the arrays below
   int32_t* row_adapter = nullptr;  // [rows]: the adapter of each row, -1 = none
   int4* segs = nullptr;            // [nsegs]: row ranges with an adapter, ascending: lo, hi, adapter
-  int32_t* tile_first = nullptr;   // per 128 rows: the first segment that ends after the first of them
+  int2* tiles = nullptr;           // per 128 rows: the first segment that meets them, and how many do
   int2* spans = nullptr;           // [nsegs]: the row ranges adapter by adapter, ascending within one
   int32_t* span_ptr = nullptr;     // [n_adapters + 1]: where each adapter's spans start
   int4* chunks = nullptr;          // [nchunks]: the spans in blocks of at most 64 rows: row, rows, adapter
   int32_t* chunk_ptr = nullptr;    // [n_adapters + 1]: where each adapter's blocks start
+  std::vector<int32_t> host_chunk_ptr;
   cudaStream_t built_on = nullptr;
   cudaEvent_t built = nullptr;     // the arrays are on the device
   bool settled = false;            // `built` has been seen complete
@@ -25,6 +27,25 @@ struct AdapterPlan {
 // rounded up to 16, or to 64 above 32, where a part fills whole 128-byte rows.
 inline int adapter_u_cols(int rank) { return 2 * (rank <= 32 ? (rank + 15) / 16 * 16 : (rank + 63) / 64 * 64); }
 
+// A value as two 16-bit parts, high part and remainder (Q of lc_adapters_tc.cu).
+template <typename T> __device__ __forceinline__ T largest();
+template <> __device__ __forceinline__ __half largest<__half>() { return __ushort_as_half(0x7bff); }
+template <> __device__ __forceinline__ __nv_bfloat16 largest<__nv_bfloat16>() { return __ushort_as_bfloat16(0x7f7f); }
+template <typename T>
+__device__ __forceinline__ void split2(float v, T& hi, T& lo) {
+  hi = from_f<T>(v);
+  float h = to_f<T>(hi);
+  if (!isfinite(h)) {
+    if (!isfinite(v)) {  // the value itself: its remainder would be NaN
+      lo = from_f<T>(0.f);
+      return;
+    }
+    h = copysignf(to_f<T>(largest<T>()), v);
+    hi = from_f<T>(h);
+  }
+  lo = from_f<T>(v - h);
+}
+
 // Q[t] = s_a·P_a·X[t] for X [rows, C] and P [n, rank, C] (row strides ld, ldp: multiples of 8; 16-byte aligned).
 struct AdapterShrink {
   const void *X = nullptr, *P = nullptr;
@@ -33,21 +54,21 @@ struct AdapterShrink {
   const float* scales = nullptr;
   void* Q = nullptr;
 };
-// dP[a] = Σ_{t in a} Q[t] ⊗ X[t], [n, rank, C] dense; count: adapter_count_words zeros.
+// dP[a] = Σ_{t in a} Q[t] ⊗ X[t], [n, rank, C] dense.
 struct AdapterOuter {
   const void *X = nullptr, *Q = nullptr;
   int64_t C = 0, ld = 0;
   int rank = 0;
   void* dP = nullptr;
-  uint32_t* count = nullptr;
 };
 namespace lc {
-// One or two products over the same rows, ranks and scales. The shrink also
-// clears `nzero` words for a kernel that follows it.
-void adapter_shrink_tc(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, const AdapterPlan& p, int dtype, cudaStream_t st);
+// One or two products over the same rows, ranks and scales.
+void adapter_shrink_tc(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
 void adapter_outer_tc(const AdapterOuter* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
-size_t adapter_count_words(const AdapterPlan& p, int rank, int64_t C);
-int adapter_runs(int tiles, int nchunks);
+// The forms for few rows (lc_adapters_rows.cu): false, with nothing launched, for more than these products.
+constexpr int64_t kRowsShrinkMost = 1 << 27, kRowsLinearMost = 1 << 27;
+bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
+bool adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int dtype, cudaStream_t st);
 }  // namespace lc
 
 void lc_adapters_destroy();

@@ -49,25 +49,6 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
-// The two 16-bit parts of a value.
-template <typename T> __device__ __forceinline__ T largest();
-template <> __device__ __forceinline__ __half largest<__half>() { return __ushort_as_half(0x7bff); }
-template <> __device__ __forceinline__ __nv_bfloat16 largest<__nv_bfloat16>() { return __ushort_as_bfloat16(0x7f7f); }
-template <typename T>
-__device__ __forceinline__ void split2(float v, T& hi, T& lo) {
-  hi = TcFmt<T>::cvt(v);
-  float h = TcFmt<T>::back(hi);
-  if (!isfinite(h)) {
-    if (!isfinite(v)) {  // the value itself: its remainder would be NaN
-      lo = TcFmt<T>::cvt(0.f);
-      return;
-    }
-    h = copysignf(TcFmt<T>::back(largest<T>()), v);
-    hi = TcFmt<T>::cvt(h);
-  }
-  lo = TcFmt<T>::cvt(v - h);
-}
-
 // ------------------------------------------------------------- shrink
 //
 // One CTA takes tiles of 128 rows of one or two products (both directions of a
@@ -89,21 +70,53 @@ struct ShrinkJob {
   int C;
 };
 struct ShrinkArgs {
-  ShrinkJob job[2];
-  int njobs, T, ntiles, nsegs, R, rank, nb, stages, ucols, S;
+  ShrinkJob job[2];  // the longer one first
+  int njobs, T, ntiles, R, rank, nb, stages, ucols, S;
+  int extra, filled;  // the second job's tiles that even out the first's last round (ShrinkItems)
   uint32_t bank_bytes, tmem_cols;
   const int4* segs;
-  const int32_t* tile_first;
+  const int2* tiles;
   const float* scales;
-  uint32_t* zero;  // words that the next kernel counts in
-  int nzero;
 };
-// The segments of one pass over a tile: s, s + 1, ... that meet rows [m0, m0 + 128); 0 when the tile is done.
-__device__ __forceinline__ int pass_segments(const ShrinkArgs& args, int s, int m0) {
-  int n = 0;
-  while (n < args.nb && s + n < args.nsegs && __ldg(&args.segs[s + n].x) < m0 + BM) n++;
-  return n;
-}
+// The tiles of one CTA (cluster): the first job's round by round; then, where
+// the last round was not full, `extra` tiles of the second job for each CTA
+// that had none in it; then the rest of the second job, round by round. The
+// next tile's segment range is loaded while the current tile is worked on.
+struct ShrinkItems {
+  const ShrinkArgs& args;
+  int cta, n, rem, t, job, k = 0;
+  int2 segs, ahead;  // first segment and number of segments: of this tile, of the next one
+  int next_t, next_job;
+  __device__ ShrinkItems(const ShrinkArgs& a, int cta_, int n_) : args(a), cta(cta_), n(n_), rem(a.ntiles % n_), next_t(cta_), next_job(0) {
+    settle();
+    load();
+  }
+  // brings (next_job, next_t) to a tile that exists, or next_job to njobs
+  __device__ void settle() {
+    if (next_job == 0 && next_t >= args.ntiles) {
+      next_job = 1;
+      next_t = -1;
+    }
+    if (next_job == 1 && args.njobs == 2 && next_t < 0) {
+      if (cta >= rem && k < args.extra && (cta - rem) * args.extra + k < args.filled) next_t = (cta - rem) * args.extra + k++;
+      else next_t = args.filled + (cta - rem + n) % n, k = args.extra;
+    }
+    if (next_job == 1 && (args.njobs < 2 || next_t >= args.ntiles)) next_job = 2;
+  }
+  __device__ void load() { ahead = next_job < args.njobs ? __ldg(args.tiles + next_t) : make_int2(0, 0); }
+  __device__ bool next() {
+    if (next_job >= args.njobs) return false;
+    t = next_t;
+    job = next_job;
+    segs = ahead;
+    if (next_job == 1 && k < args.extra && next_t < args.filled) next_t = -1;
+    else if (next_job == 1 && next_t < args.filled) next_t = args.filled + (cta - rem + n) % n;
+    else next_t += n;
+    settle();
+    load();
+    return true;
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_constant__ ShrinkArgs args) {
@@ -119,7 +132,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
   volatile int* abort = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = args.S, rank = S > 1 ? (int)cluster_rank() : 0;
-  const int first = blockIdx.x / S, step = gridDim.x / S, nitems = args.njobs * args.ntiles;
+  const int first = blockIdx.x / S, step = gridDim.x / S;
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
     for (int a = 0; a < 2; a++) mbar_init(&tfull[a], 1), mbar_init(&tempty[a], 4);
@@ -134,7 +147,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_trigger();  // after the wait: what runs before this kernel is done when the next one starts
-  for (int i = blockIdx.x * TC_THREADS + threadIdx.x; i < args.nzero; i += gridDim.x * TC_THREADS) args.zero[i] = 0;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -142,19 +154,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
       uint32_t phase = 0;
       bool ok = true;
       uint32_t used = 0, last_phase = 0;  // stages filled, and the phase bit of each one's last fill
-      for (int it = first; it < nitems && ok; it += step) {
-        const ShrinkJob& job = args.job[it >= args.ntiles];
-        const int t = it >= args.ntiles ? it - args.ntiles : it, m0 = t * BM;
+      for (ShrinkItems it(args, first, step); ok && it.next();) {
+        const ShrinkJob& job = args.job[it.job];
         const int KB = (job.C + BK - 1) / BK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
-        int n;
-        for (int s = __ldg(args.tile_first + t); ok && (n = pass_segments(args, s, m0)); s += n) {
+        for (int s = 0; s < it.segs.y && ok; s += args.nb) {
+          const int n = min(args.nb, it.segs.y - s);
+          int ad[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) ad[i] = i < n ? __ldg(&args.segs[it.segs.x + s + i].z) : 0;
           for (int kb = kb0; kb < kb1; kb++) {
             if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
             uint8_t* st = smem + stage * stage_bytes;
             mbar_arrive_expect_tx(&full[stage], X_BYTES + (uint32_t)n * args.R * 128);
-            tma_load_2d(st, &job.tmX, &full[stage], kb * BK, m0);
-            for (int i = 0; i < n; i++)
-              tma_load_3d(st + X_BYTES + i * args.R * 128, &job.tmP, &full[stage], kb * BK, 0, __ldg(&args.segs[s + i].z));
+            tma_load_2d(st, &job.tmX, &full[stage], kb * BK, it.t * BM);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              if (i < n) tma_load_3d(st + X_BYTES + i * args.R * 128, &job.tmP, &full[stage], kb * BK, 0, ad[i]);
             used |= 1u << stage;
             last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
             if (++stage == args.stages) { stage = 0; phase ^= 1; }
@@ -174,12 +189,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
       bool ok = true;
       uint64_t* last = nullptr;
       uint32_t last_phase = 0;
-      for (int it = first; it < nitems && ok; it += step) {
-        const ShrinkJob& job = args.job[it >= args.ntiles];
-        const int t = it >= args.ntiles ? it - args.ntiles : it, m0 = t * BM;
+      for (ShrinkItems it(args, first, step); ok && it.next();) {
+        const ShrinkJob& job = args.job[it.job];
         const int KB = (job.C + BK - 1) / BK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
-        int n;
-        for (int s = __ldg(args.tile_first + t); ok && (n = pass_segments(args, s, m0)); s += n) {
+        for (int s = 0; s < it.segs.y && ok; s += args.nb) {
+          const int n = min(args.nb, it.segs.y - s);
           const uint32_t idesc = idesc_rt<T>(n * args.R, false, false);
           if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
           tc_fence_after();
@@ -212,15 +226,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int it = first; it < nitems && ok; it += step) {
-      const int t = it >= args.ntiles ? it - args.ntiles : it, m0 = t * BM, row = m0 + quarter * 32 + lane;
-      T* Q = (T*)args.job[it >= args.ntiles].Q + (int64_t)row * args.ucols;
-      int n;
-      for (int s = __ldg(args.tile_first + t); ok && (n = pass_segments(args, s, m0)); s += n) {
+    for (ShrinkItems it(args, first, step); ok && it.next();) {
+      const int row = it.t * BM + quarter * 32 + lane;
+      T* Q = (T*)args.job[it.job].Q + (int64_t)row * args.ucols;
+      for (int s = 0; s < it.segs.y && ok; s += args.nb) {
+        const int n = min(args.nb, it.segs.y - s);
         if (!mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err)) { ok = false; break; }
         tc_fence_after();
         for (int i = 0; i < n; i++) {
-          const int4 g = __ldg(&args.segs[s + i]);
+          const int4 g = __ldg(&args.segs[it.segs.x + s + i]);
           const bool mine = row >= g.x && row < g.y;
           if (!__any_sync(0xffffffffu, mine)) continue;
           const float sc = args.scales ? __ldg(args.scales + g.z) : 1.f;
@@ -263,17 +277,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
     cluster_sync();
     // one item per cluster: rank r adds rows [r·128/S, (r+1)·128/S) of all the CTAs' shares
     const int t = first >= args.ntiles ? first - args.ntiles : first, m0 = t * BM, rows = BM / S;
+    const int2 segs = __ldg(args.tiles + t);
     T* Q = (T*)args.job[first >= args.ntiles].Q;
     for (int lr = rank * rows + (int)threadIdx.x / 16; lr < (rank + 1) * rows; lr += TC_THREADS / 16) {
       const int row = m0 + lr;
       int a = -1;
-      for (int s = __ldg(args.tile_first + t); s < args.nsegs; s++) {
-        const int4 g = __ldg(&args.segs[s]);
-        if (g.x > row) break;
-        if (row < g.y) {
-          a = g.z;
-          break;
-        }
+      for (int s = 0; s < segs.y; s++) {
+        const int4 g = __ldg(&args.segs[segs.x + s]);
+        if (row >= g.x && row < g.y) a = g.z;
       }
       if (a < 0) continue;
       const float sc = args.scales ? __ldg(args.scales + a) : 1.f;
@@ -299,8 +310,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
 
 // ------------------------------------------------------------- outer
 //
-// D [128 columns of X, N] += X-blockᵀ · Q-block over blocks of up to 64 rows of
-// one adapter: both operands are read MN-major from the row-major blocks that
+// D [columns of X, N] += X-blockᵀ · Q-block over blocks of up to 64 rows of one
+// adapter and 256 columns (two M = 128 accumulators, so that Q and the steps of
+// a block are shared by twice the columns): both operands are read MN-major from the row-major blocks that
 // TMA brings (their rows are the contraction). N covers the high and the
 // remainder parts of up to 64 rank rows; the epilogue adds the two. A block
 // that ends inside its adapter's rows is loaded up to the next multiple of 16
@@ -309,17 +321,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
 // of that request through).
 //
 // The blocks of all adapters, in adapter order, are cut into G equal runs; a
-// CTA takes one run for one 128-column tile (and one group of 64 rank rows) of
+// CTA takes one run for one 256-column tile (and one group of 64 rank rows) of
 // one or two products. A run that holds all of an adapter's blocks stores dP;
 // otherwise it stores an f32 partial, in slot run + adapter (distinct for every
 // pair that occurs), counts itself in, and the last of the adapter's runs to
 // arrive adds all partials in the order of the runs: the same bits every time.
 // Bound by the read of X.
 constexpr int OUTER_THREADS = TC_THREADS + 32;  // and the warp that clears rows
+constexpr int BC = 256;                         // columns of X per CTA
+constexpr uint32_t XC_BYTES = 64 * BC * 2;
 struct OuterJob {
   CUtensorMap tmX, tmQ, tmX16, tmQ16;  // boxes of 64 and of 16 rows
   float* part;                         // [G + n, rank, C]
-  uint32_t* count;                     // [n, ctiles, rgroups]: runs that have stored their partial
   void* dP;
   int C, ctiles;
 };
@@ -335,7 +348,7 @@ template <typename T>
 __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_constant__ OuterArgs args) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t stage_bytes = X_BYTES + args.q_bytes;
+  const uint32_t stage_bytes = XC_BYTES + args.q_bytes;
   uint64_t* full = (uint64_t*)(smem + args.stages * stage_bytes);
   uint64_t* empty = full + args.stages;
   uint64_t* cleared = empty + args.stages;
@@ -343,14 +356,14 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = (uint32_t*)(tempty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
-  volatile int* arrived = abort + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool second = (int)blockIdx.x >= args.job[0].ctiles;
   const OuterJob& job = args.job[second];
   const int ct = second ? (int)blockIdx.x - args.job[0].ctiles : (int)blockIdx.x;
-  const int c0 = ct * BM, g = blockIdx.y, j0 = blockIdx.z * 64;
+  const int c0 = ct * BC, g = blockIdx.y, j0 = blockIdx.z * 64;
   const int lo = (int)((int64_t)g * args.nchunks / args.G), hi = (int)((int64_t)(g + 1) * args.nchunks / args.G);
-  const int blocks = (int)(stage_bytes >> 13);  // 64 x 64 blocks of a stage
+  const int xblocks = min(BC / 64, (job.C - c0 + 63) / 64), qblocks = (int)(args.q_bytes >> 13);  // 64 x 64 blocks of a stage
+  const int halves = xblocks > 2 ? 2 : 1;                                                         // accumulators of 128 columns
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1), mbar_init(&cleared[s], 1);
     for (int a = 0; a < 2; a++) mbar_init(&tfull[a], 1), mbar_init(&tempty[a], 4);
@@ -370,21 +383,21 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0, used = 0, last_phase = 0;
+      int4 ahead = lo < hi ? __ldg(&args.chunks[lo]) : make_int4(0, 0, 0, 0);
       for (int c = lo; c < hi; c++) {
-        const int4 ch = __ldg(&args.chunks[c]);
+        const int4 ch = ahead;
+        if (c + 1 < hi) ahead = __ldg(&args.chunks[c + 1]);
         if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_adapter_err)) break;
         uint8_t* st = smem + stage * stage_bytes;
         const int n16 = (ch.y + 15) >> 4;
-        mbar_arrive_expect_tx(&full[stage], (uint32_t)(blocks * n16) * 2048);
+        mbar_arrive_expect_tx(&full[stage], (uint32_t)((xblocks + qblocks) * n16) * 2048);
         auto bring = [&](uint8_t* dst, const CUtensorMap* big, const CUtensorMap* small, int x) {
           if (n16 == 4) tma_load_2d(dst, big, &full[stage], x, ch.x);
           else
             for (int i = 0; i < n16; i++) tma_load_2d(dst + i * 2048, small, &full[stage], x, ch.x + 16 * i);
         };
-        bring(st, &job.tmX, &job.tmX16, c0);
-        bring(st + 8192, &job.tmX, &job.tmX16, c0 + 64);
-        bring(st + X_BYTES, &job.tmQ, &job.tmQ16, j0);
-        if (blocks == 4) bring(st + X_BYTES + 8192, &job.tmQ, &job.tmQ16, args.ucols / 2 + j0);
+        for (int b = 0; b < xblocks; b++) bring(st + b * 8192, &job.tmX, &job.tmX16, c0 + 64 * b);
+        for (int b = 0; b < qblocks; b++) bring(st + XC_BYTES + b * 8192, &job.tmQ, &job.tmQ16, b * (args.ucols / 2) + j0);
         used |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
         if (++stage == args.stages) { stage = 0; phase ^= 1; }
@@ -407,15 +420,19 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
         const int a = __ldg(&args.chunks[c].z), end = min(hi, __ldg(args.chunk_ptr + a + 1)), begin = c;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(acc * args.nmma);
+        const uint32_t d = tmem + (uint32_t)(acc * 2 * args.nmma);
         for (; c < end; c++) {
           const int rows = __ldg(&args.chunks[c].y), steps = (rows + 15) >> 4;
           if (!mbar_wait(&full[stage], phase, abort, &g_adapter_err)) { ok = false; break; }
           if (!mbar_wait(&cleared[stage], phase, abort, &g_adapter_err)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + stage * stage_bytes), b0 = a0 + X_BYTES;
-          for (int k = 0; k < steps; k++)
-            tc_mma(d, sdesc_sw128_mn(a0 + k * 2048, 8192), sdesc_sw128_mn(b0 + k * 2048, 8192), idesc, (c > begin || k > 0) ? 1u : 0u);
+          const uint32_t a0 = smem_u32(smem + stage * stage_bytes), b0 = a0 + XC_BYTES;
+          // (a last block of 64 columns or less: the other half of the accumulator's rows reads a stale block and is not stored)
+          for (int k = 0; k < steps; k++) {
+            const uint64_t q = sdesc_sw128_mn(b0 + k * 2048, 8192);
+            tc_mma(d, sdesc_sw128_mn(a0 + k * 2048, 8192), q, idesc, (c > begin || k > 0) ? 1u : 0u);
+            if (halves == 2) tc_mma(d + args.nmma, sdesc_sw128_mn(a0 + 16384 + k * 2048, 8192), q, idesc, (c > begin || k > 0) ? 1u : 0u);
+          }
           tc_commit(&empty[stage]);
           last = &empty[stage];
           last_phase = phase;
@@ -443,8 +460,10 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
       if (rows & 15) {
         uint8_t* st = smem + stage * stage_bytes + rows * 128;
         const int zn = (16 - (rows & 15)) * 8;  // 16-byte pieces per 64-column block
-        for (int k = 0; k < blocks; k++)
-          for (int i = lane; i < zn; i += 32) *(uint4*)(st + k * 8192 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        for (int k = 0; k < xblocks + qblocks; k++) {
+          uint8_t* z = st + (k < xblocks ? k * 8192 : XC_BYTES + (k - xblocks) * 8192);
+          for (int i = lane; i < zn; i += 32) *(uint4*)(z + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -453,42 +472,33 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, col = c0 + quarter * 32 + lane;
+    const int quarter = warp & 3, col0 = c0 + quarter * 32 + lane;  // and col0 + 128
     const int nh = args.nmma / 2;  // rank rows of this CTA, rounded up
     const int64_t size = (int64_t)args.rank * job.C;
     T* dP = (T*)job.dP;
-    // barriers of the four epilogue warps, which take the same turns; all4 says whether the condition holds for all of them
-    auto sync4 = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-    auto all4 = [](bool p) {
-      uint32_t r;
-      asm volatile(
-          "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-          : "=r"(r)
-          : "r"((uint32_t)p)
-          : "memory");
-      return r != 0;
-    };
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int c = lo; c < hi;) {
       const int a = __ldg(&args.chunks[c].z), p0 = __ldg(args.chunk_ptr + a), p1 = __ldg(args.chunk_ptr + a + 1);
       const bool whole = p0 >= lo && p1 <= hi;
-      // a timeout ends the loop of all epilogue warps: none is left at a barrier below
-      if (!all4(mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err))) break;
+      if (!mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err)) break;
       tc_fence_after();
-      const uint32_t tb = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * args.nmma);
-      for (int j = 0; j < nh; j += 16) {
-        uint32_t vh[16], vl[16];
-        tmem_ld16(tb + j, vh);
-        tmem_ld16(tb + nh + j, vl);
-        tmem_wait_ld();
+      for (int h = 0; h < halves; h++) {
+        const int col = col0 + 128 * h;
+        const uint32_t tb = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((acc * 2 + h) * args.nmma);
+        for (int j = 0; j < nh; j += 16) {
+          uint32_t vh[16], vl[16];
+          tmem_ld16(tb + j, vh);
+          tmem_ld16(tb + nh + j, vl);
+          tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int row = j0 + j + i;
-          if (row < args.rank && col < job.C) {
-            const float v = __uint_as_float(vh[i]) + __uint_as_float(vl[i]);
-            if (whole) dP[a * size + (int64_t)row * job.C + col] = TcFmt<T>::cvt(v);
-            else job.part[(g + a) * size + (int64_t)row * job.C + col] = v;
+          for (int i = 0; i < 16; i++) {
+            const int row = j0 + j + i;
+            if (row < args.rank && col < job.C) {
+              const float v = __uint_as_float(vh[i]) + __uint_as_float(vl[i]);
+              if (whole) dP[a * size + (int64_t)row * job.C + col] = TcFmt<T>::cvt(v);
+              else job.part[(g + a) * size + (int64_t)row * job.C + col] = v;
+            }
           }
         }
       }
@@ -496,40 +506,13 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
-      if (!whole) {  // the runs of the first and the last block: run g begins at floor(g·nchunks / G)
-        const int g0 = (int)((((int64_t)p0 + 1) * args.G - 1) / args.nchunks), g1 = (int)(((int64_t)p1 * args.G - 1) / args.nchunks);
-        __threadfence();
-        sync4();
-        if (warp == 2 && lane == 0) {
-          const uint32_t was = atomicAdd(job.count + ((int64_t)a * job.ctiles + ct) * args.rgroups + blockIdx.z, 1u);
-          *arrived = was == (uint32_t)(g1 - g0);
-        }
-        sync4();
-        const bool join = *arrived != 0;
-        if (join && col < job.C) {
-          __threadfence();
-          for (int j = 0; j < nh; j += 16) {
-            float v[16] = {};
-#pragma unroll 4
-            for (int q = g0; q <= g1; q++) {
-              const float* p = job.part + (q + a) * size + (int64_t)(j0 + j) * job.C + col;
-#pragma unroll
-              for (int i = 0; i < 16; i++)
-                if (j0 + j + i < args.rank) v[i] += __ldcg(p + (int64_t)i * job.C);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-              if (j0 + j + i < args.rank) dP[a * size + (int64_t)(j0 + j + i) * job.C + col] = TcFmt<T>::cvt(v[i]);
-          }
-        }
-        sync4();  // `arrived` is read before it is written again
-      }
       c = min(hi, p1);
     }
-    if (g == 0 && col < job.C)  // adapters without rows
+    if (g == 0)  // adapters without rows
       for (int a = 0; a < args.n; a++)
         if (__ldg(args.chunk_ptr + a) == __ldg(args.chunk_ptr + a + 1))
-          for (int j = j0; j < min(args.rank, j0 + nh); j++) dP[a * size + (int64_t)j * job.C + col] = TcFmt<T>::cvt(0.f);
+          for (int j = j0; j < min(args.rank, j0 + nh); j++)
+            for (int col = col0; col < min(job.C, c0 + BC); col += 128) dP[a * size + (int64_t)j * job.C + col] = TcFmt<T>::cvt(0.f);
   }
   if (threadIdx.x == 0 && *abort) {
     const uint64_t t0 = gtimer();
@@ -543,6 +526,28 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
   }
 }
 
+// dP of the adapters that several runs share: the sum of their partials.
+struct JoinArgs {
+  const float* part[2];
+  void* dP[2];
+  int64_t size[2];   // rank · C
+  int3 shared[63];   // adapter, first and last run
+};
+template <typename T>
+__global__ void __launch_bounds__(256) k_outer_join(const __grid_constant__ JoinArgs args) {
+  pdl_wait();
+  pdl_trigger();
+  const int j = blockIdx.z;
+  const int3 s = args.shared[blockIdx.y];
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x), size = args.size[j];
+  if (i >= size) return;
+  const float* p = args.part[j] + (int64_t)(s.y + s.x) * size + i;
+  float v = 0.f;
+#pragma unroll 8
+  for (int g = s.y; g <= s.z; g++, p += size) v += *p;
+  ((T*)args.dP[j])[(int64_t)s.x * size + i] = from_f<T>(v);
+}
+
 uint32_t tmem_columns(int want) {
   uint32_t c = 32;
   while ((int)c < want) c *= 2;
@@ -550,13 +555,12 @@ uint32_t tmem_columns(int want) {
 }
 
 template <typename T>
-void shrink_t(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, const AdapterPlan& p, cudaStream_t st) {
+void shrink_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStream_t st) {
   const int dtype = std::is_same<T, __half>::value ? LC_F16 : LC_BF16;
   ShrinkArgs a{};
   a.njobs = njobs;
   a.T = p.rows;
   a.ntiles = (p.rows + BM - 1) / BM;
-  a.nsegs = p.nsegs;
   a.rank = c[0].rank;
   a.ucols = adapter_u_cols(a.rank);
   a.R = a.ucols / 2;
@@ -566,16 +570,15 @@ void shrink_t(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, c
   a.bank_bytes = (uint32_t)(a.nb * a.R * 128);
   a.tmem_cols = tmem_columns(2 * a.nb * a.R);
   a.segs = p.segs;
-  a.tile_first = p.tile_first;
+  a.tiles = p.tiles;
   a.scales = c[0].scales;
-  a.zero = zero;
-  a.nzero = (int)nzero;
   int KB = INT32_MAX;
   for (int j = 0; j < njobs; j++) {
-    a.job[j].tmX = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, BK, BM, dtype);
-    a.job[j].tmP = tensor_map_3d(c[j].P, c[j].n, c[j].rank, c[j].C, c[j].ldp, a.R, dtype);
-    a.job[j].Q = c[j].Q;
-    a.job[j].C = (int)c[j].C;
+    const AdapterShrink& q = c[njobs == 2 && c[1].C > c[0].C ? 1 - j : j];
+    a.job[j].tmX = tensor_map_2d(q.X, p.rows, q.C, q.ld, BK, BM, dtype);
+    a.job[j].tmP = tensor_map_3d(q.P, q.n, q.rank, q.C, q.ldp, a.R, dtype);
+    a.job[j].Q = q.Q;
+    a.job[j].C = (int)q.C;
     KB = std::min(KB, (a.job[j].C + BK - 1) / BK);
   }
   const int64_t items = (int64_t)njobs * a.ntiles;
@@ -585,6 +588,11 @@ void shrink_t(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, c
       a.S = f;
       break;
     }
+  const int ctas = (int)std::min<int64_t>(items, num_sms());
+  if (njobs == 2 && a.S == 1 && a.ntiles % ctas) {
+    a.extra = ((a.job[0].C + BK - 1) / BK) / ((a.job[1].C + BK - 1) / BK);
+    a.filled = (int)std::min<int64_t>(a.ntiles, (int64_t)a.extra * (ctas - a.ntiles % ctas));
+  }
   const size_t d_bytes = a.S > 1 ? (size_t)BM * a.R * 4 : 0;
   a.stages = std::min(8, (int)(((224u << 10) - d_bytes) / (X_BYTES + a.bank_bytes)));
   const size_t smem = (size_t)a.stages * (X_BYTES + a.bank_bytes) + d_bytes + 1024 + 512;
@@ -603,13 +611,29 @@ void shrink_t(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, c
     at[0].val.clusterDim.z = 1;
     n = 1;
   }
-  cfg.gridDim = dim3((unsigned)(a.S > 1 ? a.S * items : std::min<int64_t>(items, num_sms())));
+  cfg.gridDim = dim3((unsigned)(a.S > 1 ? a.S * items : ctas));
   cfg.blockDim = dim3(TC_THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   chain_attrs(cfg, at, n);
   CUDA_OK(cudaLaunchKernelEx(&cfg, k_shrink_tc<T>, a));
   LC_LAUNCHED(1);
+}
+
+constexpr int kMaxRuns = 64;  // JoinArgs::shared holds a boundary each
+// Runs of blocks per tile of columns.
+int adapter_runs(int tiles, int nchunks) {
+  // one wave of CTAs, or two where one would leave SMs idle
+  const int sms = num_sms();
+  int G = 1;
+  double best = 0;
+  for (int f = 1; f <= kMaxRuns && f <= nchunks; f++) {
+    const int64_t ctas = (int64_t)tiles * f, waves = (ctas + sms - 1) / sms;
+    const double fill = (double)ctas / (double)(waves * sms);
+    if (fill > best + 0.03) best = fill, G = f;
+    if (waves > 2) break;
+  }
+  return G;
 }
 
 template <typename T>
@@ -623,12 +647,12 @@ void outer_t(const AdapterOuter* c, int njobs, const AdapterPlan& p, cudaStream_
   a.rgroups = std::max(1, a.ucols / 128);
   a.nmma = std::min(a.ucols, 128);
   a.q_bytes = a.ucols > 64 ? 16384 : 8192;
-  a.stages = a.q_bytes > 8192 ? 6 : 8;
-  a.tmem_cols = tmem_columns(2 * a.nmma);
+  a.stages = a.q_bytes > 8192 ? 4 : 5;
+  a.tmem_cols = tmem_columns(4 * a.nmma);
   a.chunks = p.chunks;
   a.chunk_ptr = p.chunk_ptr;
   int ctiles = 0;
-  for (int j = 0; j < njobs; j++) ctiles += (int)((c[j].C + BM - 1) / BM);
+  for (int j = 0; j < njobs; j++) ctiles += (int)((c[j].C + BC - 1) / BC);
   a.G = adapter_runs(ctiles * a.rgroups, p.nchunks);
   struct Partials {
     void* p[2] = {nullptr, nullptr};
@@ -640,16 +664,15 @@ void outer_t(const AdapterOuter* c, int njobs, const AdapterPlan& p, cudaStream_
   for (int j = 0; j < njobs; j++) {
     OuterJob& o = a.job[j];
     o.C = (int)c[j].C;
-    o.ctiles = (o.C + BM - 1) / BM;
+    o.ctiles = (o.C + BC - 1) / BC;
     o.tmX = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 64, dtype);
     o.tmQ = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 64, dtype);
     o.tmX16 = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 16, dtype);
     o.tmQ16 = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 16, dtype);
     o.dP = c[j].dP;
-    o.count = c[j].count;
     if (a.G > 1) o.part = (float*)(part.p[j] = dmalloc((size_t)(a.G + p.n_adapters) * a.rank * c[j].C * 4));
   }
-  const size_t smem = (size_t)a.stages * (X_BYTES + a.q_bytes) + 1024 + 512;
+  const size_t smem = (size_t)a.stages * (XC_BYTES + a.q_bytes) + 1024 + 512;
   static bool attr = false;
   if (!attr) {
     CUDA_OK(cudaFuncSetAttribute(k_outer_tc<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 << 10));
@@ -657,34 +680,35 @@ void outer_t(const AdapterOuter* c, int njobs, const AdapterPlan& p, cudaStream_
   }
   launch_chain(k_outer_tc<T>, dim3((unsigned)ctiles, (unsigned)a.G, (unsigned)a.rgroups), dim3(OUTER_THREADS), smem, st, a);
   LC_LAUNCHED(1);
+  // the adapters that several runs share: at most one per boundary between runs
+  JoinArgs join{};
+  int shared = 0;
+  for (int g = 1; g < a.G; g++) {
+    const int at = (int)((int64_t)g * a.nchunks / a.G);  // the first block of run g
+    const int ad = (int)(std::upper_bound(p.host_chunk_ptr.begin(), p.host_chunk_ptr.end(), at) - p.host_chunk_ptr.begin()) - 1;
+    if (p.host_chunk_ptr[ad] == at) continue;  // an adapter begins here
+    if (shared && join.shared[shared - 1].x == ad) join.shared[shared - 1].z = g;
+    else join.shared[shared++] = make_int3(ad, g - 1, g);
+  }
+  if (!shared) return;
+  int64_t most = 0;
+  for (int j = 0; j < njobs; j++) {
+    join.part[j] = a.job[j].part;
+    join.dP[j] = a.job[j].dP;
+    join.size[j] = (int64_t)a.rank * a.job[j].C;
+    most = std::max(most, join.size[j]);
+  }
+  launch_chain(k_outer_join<T>, dim3((unsigned)((most + 255) / 256), (unsigned)shared, (unsigned)njobs), dim3(256), 0, st, join);
+  LC_LAUNCHED(1);
 }
 
 }  // namespace
 
 namespace lc {
 
-void adapter_shrink_tc(const AdapterShrink* c, int njobs, uint32_t* zero, size_t nzero, const AdapterPlan& p, int dtype, cudaStream_t st) {
+void adapter_shrink_tc(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st) {
   if (!p.nsegs) return;
-  LC_CHECK(nzero <= INT32_MAX, "adapters: too many adapters");
-  dtype == LC_F16 ? shrink_t<__half>(c, njobs, zero, nzero, p, st) : shrink_t<__nv_bfloat16>(c, njobs, zero, nzero, p, st);
-}
-
-int adapter_runs(int tiles, int nchunks) {
-  // one wave of CTAs, or two where one would leave SMs idle
-  const int sms = num_sms();
-  int G = 1;
-  double best = 0;
-  for (int f = 1; f <= 64 && f <= nchunks; f++) {
-    const int64_t ctas = (int64_t)tiles * f, waves = (ctas + sms - 1) / sms;
-    const double fill = (double)ctas / (double)(waves * sms);
-    if (fill > best + 0.03) best = fill, G = f;
-    if (waves > 2) break;
-  }
-  return G;
-}
-
-size_t adapter_count_words(const AdapterPlan& p, int rank, int64_t C) {
-  return (size_t)p.n_adapters * ((C + BM - 1) / BM) * std::max(1, adapter_u_cols(rank) / 128);
+  dtype == LC_F16 ? shrink_t<__half>(c, njobs, p, st) : shrink_t<__nv_bfloat16>(c, njobs, p, st);
 }
 
 void adapter_outer_tc(const AdapterOuter* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st) {

@@ -75,8 +75,7 @@ struct GemmAdapted {
   static constexpr bool kOn = true, kWT = WT;
   CUtensorMap tmU, tmP;
   const int4* segs;           // lo, hi, adapter
-  const int32_t* tile_first;  // per 128 rows: the first segment that ends after the first of them
-  int nsegs;
+  const int2* tiles;          // per 128 rows: the first segment that meets them, and how many do
   int nchunks;                // 64-column blocks of U
   int ksteps;                 // 16-column steps used per block
   int half;                   // steps after which P's rows start over (high and low part in one block), else ksteps
@@ -87,12 +86,11 @@ struct GemmAdapted {
   int kb_off;                 // added to the K block of the main loop's loads (past the operands' end: zeros)
 };
 
-// The segments of one stage: s, s + 1, ... that begin before row `end`; 0 when the tile is done.
+// The segments [x, y) that meet the tile of `rows` (128 or 256) rows from m0.
 template <bool WT>
-__device__ __forceinline__ int stage_segments(const GemmAdapted<WT>& ex, int s, int end) {
-  int n = 0;
-  while (n < ex.per && s + n < ex.nsegs && __ldg(&ex.segs[s + n].x) < end) n++;
-  return n;
+__device__ __forceinline__ int2 tile_segments(const GemmAdapted<WT>& ex, int m0, int rows, int M) {
+  const int2 a = __ldg(ex.tiles + m0 / 128), b = rows > 128 && m0 + 128 < M ? __ldg(ex.tiles + m0 / 128 + 1) : a;
+  return make_int2(a.x, b.x + b.y);
 }
 
 __device__ __forceinline__ float gelu_exact(float x) { return 0.5f * x * (1.0f + erff(x * 0.7071067811865476f)); }
@@ -1061,16 +1059,21 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
         if constexpr (EX::kOn) {
           if (kb1 < KB) continue;  // another slice of K takes the adapters
           if (ex.defer) pdl_wait();  // the kernel that wrote U
-          int n;
-          for (int s = __ldg(ex.tile_first + m0 / BM); ok && (n = stage_segments(ex, s, m0 + BM)); s += n)
+          const int2 sg = tile_segments(ex, m0, BM, args.M);
+          for (int s = sg.x; s < sg.y && ok; s += ex.per)
             for (int c = 0; c < ex.nchunks; c++) {
+              const int n = min(ex.per, sg.y - s);
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
               mbar_arrive_expect_tx(&full[stage], A_BYTES + n * (BN / 64) * ex.prows * 128);
               tma_load_2d(sA + stage * A_BYTES, &ex.tmU, &full[stage], c * 64, m0);
-              for (int i = 0; i < n; i++) {
-                const int a = __ldg(&ex.segs[s + i].z);
+              int ad[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) ad[i] = i < n ? __ldg(&ex.segs[s + i].z) : 0;
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                if (i >= n) break;
                 for (int h = 0; h < BN / 64; h++)
-                  tma_load_3d(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, (c % ex.pgroups) * 64, a);
+                  tma_load_3d(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, (c % ex.pgroups) * 64, ad[i]);
               }
               issued[stage] = 1;
               iss_phase[stage] = phase;
@@ -1105,6 +1108,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
       uint32_t last_phase = 0;
       for (int w = blockIdx.x; w < args.ntiles * S && ok; w += gridDim.x) {
         const int kb0 = (w % S) * KB / S, kb1 = (w % S + 1) * KB / S;
+        [[maybe_unused]] int2 sg = make_int2(0, 0);
+        if constexpr (EX::kOn)
+          if (kb1 == KB) sg = tile_segments(ex, ((w / S) / args.ntile_n) * BM, BM, args.M);  // in flight during the main loop
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * BN);
@@ -1126,14 +1132,19 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
         }
         if constexpr (EX::kOn) {
           const int m0 = ((w / S) / args.ntile_n) * BM;
-          int n;
-          for (int s = kb1 < KB ? ex.nsegs : __ldg(ex.tile_first + m0 / BM); ok && (n = stage_segments(ex, s, m0 + BM)); s += n)
+          for (int s = sg.x; s < sg.y && ok; s += ex.per)
             for (int c = 0; c < ex.nchunks; c++) {
+              const int n = min(ex.per, sg.y - s);
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
               tc_fence_after();
               const uint32_t a0 = smem_u32(sA + stage * A_BYTES), b0 = smem_u32(sB + stage * B_BYTES);
-              for (int i = 0; i < n; i++) {
-                const int4 seg = __ldg(ex.segs + s + i);
+              int4 sv[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) sv[i] = __ldg(ex.segs + min(s + i, sg.y - 1));
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                if (i >= n) break;
+                const int4 seg = sv[i];
                 uint32_t off[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
@@ -1374,17 +1385,22 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
         if constexpr (EX::kOn) {
           const int t0 = (t / args.ntile_n) * (2 * BM);
           if (ex.defer) pdl_wait();  // the kernel that wrote U
-          int n;
-          for (int s = __ldg(ex.tile_first + t0 / BM); ok && (n = stage_segments(ex, s, t0 + 2 * BM)); s += n)
+          const int2 sg = tile_segments(ex, t0, 2 * BM, args.M);
+          for (int s = sg.x; s < sg.y && ok; s += ex.per)
             for (int c = 0; c < ex.nchunks; c++) {
+              const int n = min(ex.per, sg.y - s);
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
               if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (A_BYTES + n * 2 * ex.prows * 128));
               tma_load_2d_pair(sA + stage * A_BYTES, &ex.tmU, full0 + 8 * stage, c * 64, m0);
-              for (int i = 0; i < n; i++) {
-                const int a = __ldg(&ex.segs[s + i].z);
+              int ad[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) ad[i] = i < n ? __ldg(&ex.segs[s + i].z) : 0;
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                if (i >= n) break;
                 for (int h = 0; h < 2; h++)
                   tma_load_3d_pair(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, full0 + 8 * stage, n0 + 64 * h,
-                                   (c % ex.pgroups) * 64, a);
+                                   (c % ex.pgroups) * 64, ad[i]);
               }
               issued[stage] = 1;
               iss_phase[stage] = phase;
@@ -1416,6 +1432,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
       uint64_t* last = nullptr;
       uint32_t last_phase = 0;
       for (int t = pair; t < args.ntiles && ok; t += npairs) {
+        [[maybe_unused]] int2 sg = make_int2(0, 0);
+        if constexpr (EX::kOn) sg = tile_segments(ex, (t / args.ntile_n) * (2 * BM), 2 * BM, args.M);  // in flight during the main loop
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * BN);
@@ -1435,14 +1453,19 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
         }
         if constexpr (EX::kOn) {
           const int t0 = (t / args.ntile_n) * (2 * BM);
-          int n;
-          for (int s = __ldg(ex.tile_first + t0 / BM); ok && (n = stage_segments(ex, s, t0 + 2 * BM)); s += n)
+          for (int s = sg.x; s < sg.y && ok; s += ex.per)
             for (int c = 0; c < ex.nchunks; c++) {
+              const int n = min(ex.per, sg.y - s);
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
               tc_fence_after();
               const uint64_t da = dA0 + ((stage * A_BYTES) >> 4), db = dBt0 + ((stage * B_BYTES) >> 4);
-              for (int i = 0; i < n; i++) {
-                const int4 seg = __ldg(ex.segs + s + i);
+              int4 sv[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) sv[i] = __ldg(ex.segs + min(s + i, sg.y - 1));
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                if (i >= n) break;
+                const int4 seg = sv[i];
                 uint32_t off[8];
 #pragma unroll
                 for (int q = 0; q < 8; q++) off[q] = lanes_off(t0 + 32 * q, seg.x, seg.y);
@@ -1804,8 +1827,7 @@ void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
   ex.prows = std::min(64, s.u_cols / 2);  // rows past the rank arrive as zeros
   ex.tmP = tensor_map_stack(s.bank, std::max(1, s.n), s.rank, c.N, s.ld, ex.prows, dtype);
   ex.segs = s.segs;
-  ex.tile_first = s.tile_first;
-  ex.nsegs = s.nsegs;
+  ex.tiles = s.tiles;
   ex.nchunks = (s.u_cols + 63) / 64;
   ex.ksteps = std::min(4, s.u_cols / 16);
   ex.half = s.u_cols <= 64 ? s.u_cols / 32 : 4;

@@ -59,8 +59,7 @@ struct AdapterShare {
   int n = 0, rank = 0;
   int64_t ld = 0;
   const int4* segs = nullptr;  // row ranges with an adapter, ascending: lo, hi, adapter
-  const int32_t* tile_first = nullptr;
-  int nsegs = 0;
+  const int2* tiles = nullptr;  // per 128 rows: the first segment that meets them, and how many do
 };
 // y[M, N] = x·wᵀ for w [N, K], or x·w for w [K, N] (transposed), plus bias and
 // the adapters' share; w null: the share alone. Rows of x, w and the bank are

@@ -23,6 +23,8 @@ SHAPES = [
     (300, 1001, 777, 7, 12, 23), (500, 768, 768, 64, 8, 200), (513, 1024, 1312, 2, 33, 5), (640, 768, 1536, 3, 100, 4),
     (700, 136, 264, 2, 256, 3), (1000, 72, 5, 3, 5, 40), (2049, 768, 2304, 6, 16, 31), (1537, 2624, 1024, 4, 32, 12), (260, 7, 1, 2, 3, 6),
     (4096, 768, 768, 1, 16, 64), (1290, 768, 1025, 5, 24, 100),
+    # long enough that every ring, run and round of tiles goes around more than once
+    (70001, 72, 64, 5, 8, 300), (40000, 64, 392, 3, 40, 900), (33333, 328, 72, 40, 16, 3),
 ]
 
 
@@ -31,6 +33,7 @@ def _up(b, h):
 
 
 def _check(got, want, bound, what):
+    backend().flush()  # a pipeline wait that ran out is reported here
     err = np.abs(got - want)
     bad = ~(err <= bound)
     assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, worst {np.max(err / np.maximum(bound, 1e-300)):.3g} bounds at {np.argwhere(bad)[0]}"
