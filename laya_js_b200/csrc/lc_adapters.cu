@@ -537,6 +537,12 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
         chunks.insert(chunks.end(), {(int32_t)t, (int32_t)std::min<int64_t>(64, spans[2 * k + 1] - t), a, 0});
     chunk_ptr[a + 1] = (int32_t)(chunks.size() / 4);
   }
+  std::vector<int32_t> empty, pieces;
+  for (int a = 0; a < n_adapters; a++)
+    if (span_ptr[a] == span_ptr[a + 1]) empty.push_back(a);
+  if (T <= kRowsMost)
+    for (auto& g : segs)
+      for (int t = g.lo; t < g.hi; t += 8) pieces.insert(pieces.end(), {t, std::min(8, g.hi - t), g.a, 0});
   std::vector<int32_t> image;
   auto put = [&](const std::vector<int32_t>& v) {
     const size_t off = image.size();
@@ -545,7 +551,8 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
     return off;
   };
   const size_t o_rows = put(row_adapter), o_spans = put(spans), o_ptr = put(span_ptr), o_segs = put(seg4), o_tiles = put(tiles),
-               o_chunks = put(chunks), o_chunk_ptr = put(chunk_ptr);
+               o_chunks = put(chunks), o_chunk_ptr = put(chunk_ptr), o_empty = put(empty),
+               o_pieces = put(pieces);
   struct Guard {
     AdapterPlan* p;
     ~Guard() { if (p) plan_release(p); }
@@ -569,6 +576,10 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   p->chunks = (int4*)(p->dev + o_chunks);
   p->chunk_ptr = p->dev + o_chunk_ptr;
   p->host_chunk_ptr = std::move(chunk_ptr);
+  p->empty = p->dev + o_empty;
+  p->nempty = (int)empty.size();
+  p->pieces = (int4*)(p->dev + o_pieces);
+  p->npieces = (int)(pieces.size() / 4);
   plans().insert(p);
   g.p = nullptr;
   *out = reinterpret_cast<uint64_t>(p);

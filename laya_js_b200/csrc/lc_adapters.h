@@ -7,7 +7,7 @@ constexpr int kAdapterMaxRank = 256;
 
 // Rows and adapters of one batch on the device (lc_adapter_plan_create).
 struct AdapterPlan {
-  int rows = 0, n_adapters = 0, nsegs = 0, nchunks = 0;
+  int rows = 0, n_adapters = 0, nsegs = 0, nchunks = 0, nempty = 0, npieces = 0;
   int32_t* dev = nullptr;          // one allocation behind the arrays below
   int32_t* row_adapter = nullptr;  // [rows]: the adapter of each row, -1 = none
   int4* segs = nullptr;            // [nsegs]: row ranges with an adapter, ascending: lo, hi, adapter
@@ -17,6 +17,8 @@ struct AdapterPlan {
   int4* chunks = nullptr;          // [nchunks]: the spans in blocks of at most 64 rows: row, rows, adapter
   int32_t* chunk_ptr = nullptr;    // [n_adapters + 1]: where each adapter's blocks start
   std::vector<int32_t> host_chunk_ptr;
+  int32_t* empty = nullptr;        // [nempty]: the adapters without rows
+  int4* pieces = nullptr;          // [npieces]: the segments in pieces of at most 8 rows (up to kRowsMost rows): row, rows, adapter
   cudaStream_t built_on = nullptr;
   cudaEvent_t built = nullptr;     // the arrays are on the device
   bool settled = false;            // `built` has been seen complete
@@ -66,6 +68,7 @@ namespace lc {
 void adapter_shrink_tc(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
 void adapter_outer_tc(const AdapterOuter* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
 // The forms for few rows (lc_adapters_rows.cu): false, with nothing launched, for more than these products.
+constexpr int kRowsMost = 16384;
 constexpr int64_t kRowsShrinkMost = 1 << 27, kRowsLinearMost = 1 << 27;
 bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
 bool adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int dtype, cudaStream_t st);

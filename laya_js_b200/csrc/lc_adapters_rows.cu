@@ -93,31 +93,29 @@ struct RowsShrinkJob {
 struct RowsShrinkArgs {
   RowsShrinkJob job[2];
   int rank, R, ucols;
-  const int4* chunks;  // blocks of up to 64 rows of one adapter
+  const int4* pieces;  // up to 8 rows of one adapter
   const float* scales;
 };
 
-// grid: (8 pieces of every chunk, groups of 16 rank rows, jobs)
+// grid: (pieces, groups of 16 rank rows, jobs)
 template <typename T>
-__global__ void __launch_bounds__(THREADS) k_shrink_rows(const __grid_constant__ RowsShrinkArgs args) {
+__global__ void __launch_bounds__(THREADS, 1) k_shrink_rows(const __grid_constant__ RowsShrinkArgs args) {
   __shared__ float red[128];
   pdl_wait();
   pdl_trigger();  // after the wait: what runs before this kernel is done when the next one starts
   const RowsShrinkJob& job = args.job[blockIdx.z];
-  const int4 ch = __ldg(&args.chunks[blockIdx.x >> 3]);
-  const int i0 = (blockIdx.x & 7) * ROWS, j0 = blockIdx.y * COLS;
-  if (i0 >= ch.y) return;
-  const int64_t t0 = (int64_t)ch.x + i0;
-  const float v = dot_piece<T>((const T*)job.X + t0 * job.ldx, job.ldx, min(ROWS, ch.y - i0),
-                               (const T*)job.P + ((int64_t)ch.z * args.rank + j0) * job.ldp, job.ldp, args.rank - j0, job.C, red);
+  const int4 pc = __ldg(&args.pieces[blockIdx.x]);
+  const int j0 = blockIdx.y * COLS;
+  const float v = dot_piece<T>((const T*)job.X + pc.x * job.ldx, job.ldx, pc.y, (const T*)job.P + ((int64_t)pc.z * args.rank + j0) * job.ldp,
+                               job.ldp, args.rank - j0, job.C, red);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp >= 4) return;
-  const int i = i0 + (lane & 7), j = j0 + warp * 4 + (lane >> 3);
-  if (i >= ch.y || j >= args.R) return;
-  const float s = args.scales ? __ldg(args.scales + ch.z) : 1.f;
+  const int i = lane & 7, j = j0 + warp * 4 + (lane >> 3);
+  if (i >= pc.y || j >= args.R) return;
+  const float s = args.scales ? __ldg(args.scales + pc.z) : 1.f;
   T hi, lo;
   split2<T>(j < args.rank ? s * v : 0.f, hi, lo);
-  T* q = (T*)job.Q + ((int64_t)ch.x + i) * args.ucols + j;
+  T* q = (T*)job.Q + ((int64_t)pc.x + i) * args.ucols + j;
   q[0] = hi;
   q[args.R] = lo;
 }
@@ -132,7 +130,7 @@ struct RowsLinearArgs {
 
 // grid: (groups of 16 columns, groups of 8 rows)
 template <typename T>
-__global__ void __launch_bounds__(THREADS) k_linear_rows(const __grid_constant__ RowsLinearArgs args) {
+__global__ void __launch_bounds__(THREADS, 1) k_linear_rows(const __grid_constant__ RowsLinearArgs args) {
   __shared__ float red[128];
   if (!args.defer) pdl_wait();
   pdl_trigger();
@@ -166,10 +164,10 @@ void shrink_rows_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cuda
   a.rank = c[0].rank;
   a.ucols = adapter_u_cols(a.rank);
   a.R = a.ucols / 2;
-  a.chunks = p.chunks;
+  a.pieces = p.pieces;
   a.scales = c[0].scales;
   for (int j = 0; j < njobs; j++) a.job[j] = {c[j].X, c[j].P, c[j].Q, c[j].ld, c[j].ldp, (int)c[j].ld};
-  launch_chain(k_shrink_rows<T>, dim3((unsigned)p.nchunks * 8, (unsigned)((a.R + COLS - 1) / COLS), (unsigned)njobs), dim3(THREADS), 0, st, a);
+  launch_chain(k_shrink_rows<T>, dim3((unsigned)p.npieces, (unsigned)((a.R + COLS - 1) / COLS), (unsigned)njobs), dim3(THREADS), 0, st, a);
   LC_LAUNCHED(1);
 }
 
@@ -205,7 +203,7 @@ namespace lc {
 bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st) {
   int64_t C = 0;
   for (int j = 0; j < njobs; j++) C += c[j].ld;
-  if (!p.nsegs || (int64_t)p.rows * (adapter_u_cols(c[0].rank) / 2) * C > kRowsShrinkMost) return false;
+  if (!p.npieces || (int64_t)p.rows * (adapter_u_cols(c[0].rank) / 2) * C > kRowsShrinkMost) return false;
   dtype == LC_F16 ? shrink_rows_t<__half>(c, njobs, p, st) : shrink_rows_t<__nv_bfloat16>(c, njobs, p, st);
   return true;
 }

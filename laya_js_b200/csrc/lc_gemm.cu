@@ -915,8 +915,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
   constexpr uint32_t PK_BYTES = QB ? packed_bytes<BN>() : 0;  // packed stage buffer (QB)
   uint8_t* sB = smem + STAGES * A_BYTES;
   uint8_t* sPk = sB + STAGES * B_BYTES;
-  uint8_t* sE = sPk + STAGES * PK_BYTES;  // epilogue staging (TMAE only), 1024-aligned
-  float* sP = (float*)(sE + (TMAE ? STG_BYTES : 0));  // split-K partial tile (KS only)
+  uint8_t* sE = sPk + STAGES * PK_BYTES;  // epilogue staging (TMAE, or EX with rows TMA cannot store), 1024-aligned
+  float* sP = (float*)(sE + (TMAE || EX::kOn ? STG_BYTES : 0));  // split-K partial tile (KS only)
   uint64_t* full = (uint64_t*)((uint8_t*)sP + (KS ? part_bytes<BN>() : 0));
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
@@ -1066,14 +1066,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
               mbar_arrive_expect_tx(&full[stage], A_BYTES + n * (BN / 64) * ex.prows * 128);
               tma_load_2d(sA + stage * A_BYTES, &ex.tmU, &full[stage], c * 64, m0);
-              int ad[4];
-#pragma unroll
-              for (int i = 0; i < 4; i++) ad[i] = i < n ? __ldg(&ex.segs[s + i].z) : 0;
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                if (i >= n) break;
+#pragma unroll 1
+              for (int i = 0; i < n; i++) {
+                const int a = __ldg(&ex.segs[s + i].z);
                 for (int h = 0; h < BN / 64; h++)
-                  tma_load_3d(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, (c % ex.pgroups) * 64, ad[i]);
+                  tma_load_3d(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, (c % ex.pgroups) * 64, a);
               }
               issued[stage] = 1;
               iss_phase[stage] = phase;
@@ -1138,13 +1135,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
               tc_fence_after();
               const uint32_t a0 = smem_u32(sA + stage * A_BYTES), b0 = smem_u32(sB + stage * B_BYTES);
-              int4 sv[4];
-#pragma unroll
-              for (int i = 0; i < 4; i++) sv[i] = __ldg(ex.segs + min(s + i, sg.y - 1));
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                if (i >= n) break;
-                const int4 seg = sv[i];
+#pragma unroll 1
+              for (int i = 0; i < n; i++) {
+                const int4 seg = __ldg(ex.segs + s + i);
                 uint32_t off[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
@@ -1222,6 +1215,40 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
 #pragma unroll
         for (int j = 0; j < 32; j++) a[j] = __uint_as_float(ra[j]), b[j] = __uint_as_float(rb[j]);
         const int col = n0 + u * 64;
+        if constexpr (EX::kOn) {
+          // Rows off 16 bytes: through shared memory, so that a store covers 32
+          // neighbouring values of one row, not one value of 32 rows.
+          if (col >= args.N) continue;
+          T* st = (T*)(sE + (warp - 2) * 4096);
+          if (args.bias)
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              if (col + j < args.N) a[j] += ld_as<float>((const char*)args.bias, args.bias_dtype, col + j);
+              if (col + 32 + j < args.N) b[j] += ld_as<float>((const char*)args.bias, args.bias_dtype, col + 32 + j);
+            }
+          __syncwarp();  // the previous unit has been read
+#pragma unroll
+          for (int c = 0; c < 8; c++) {
+            const float* src = c < 4 ? a + c * 8 : b + (c - 4) * 8;
+            uint4 v;
+            uint32_t* h = (uint32_t*)&v;
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[j] = pack_pair<T>(make_float2(src[2 * j], src[2 * j + 1]));
+            *(uint4*)((uint8_t*)st + lane * 128 + ((c ^ (lane & 7)) << 4)) = v;
+          }
+          __syncwarp();
+          const int rows = min(32, args.M - (m0 + quarter * 32));
+          T* yp = Y + (int64_t)(m0 + quarter * 32) * args.ldy + col;
+          for (int r = 0; r < rows; r++) {
+            const uint8_t* sr = (const uint8_t*)st + r * 128;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const int cc = lane + 32 * h;
+              if (col + cc < args.N) yp[(int64_t)r * args.ldy + cc] = *(const T*)(sr + (((cc >> 3) ^ (r & 7)) << 4) + (cc & 7) * 2);
+            }
+          }
+          continue;
+        }
         if (!live || col >= (args.ep.kind == EPI_GEGLU ? 2 * args.N : args.N)) continue;
         const GemmEpilogue& ep = args.ep;
         if (ep.ln_stats) ln_apply(ep, col, ln_mu, ln_r, a, b);
@@ -1392,15 +1419,12 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
               if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (A_BYTES + n * 2 * ex.prows * 128));
               tma_load_2d_pair(sA + stage * A_BYTES, &ex.tmU, full0 + 8 * stage, c * 64, m0);
-              int ad[4];
-#pragma unroll
-              for (int i = 0; i < 4; i++) ad[i] = i < n ? __ldg(&ex.segs[s + i].z) : 0;
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                if (i >= n) break;
+#pragma unroll 1
+              for (int i = 0; i < n; i++) {
+                const int a = __ldg(&ex.segs[s + i].z);
                 for (int h = 0; h < 2; h++)
                   tma_load_3d_pair(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, full0 + 8 * stage, n0 + 64 * h,
-                                   (c % ex.pgroups) * 64, ad[i]);
+                                   (c % ex.pgroups) * 64, a);
               }
               issued[stage] = 1;
               iss_phase[stage] = phase;
@@ -1459,13 +1483,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
               tc_fence_after();
               const uint64_t da = dA0 + ((stage * A_BYTES) >> 4), db = dBt0 + ((stage * B_BYTES) >> 4);
-              int4 sv[4];
-#pragma unroll
-              for (int i = 0; i < 4; i++) sv[i] = __ldg(ex.segs + min(s + i, sg.y - 1));
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                if (i >= n) break;
-                const int4 seg = sv[i];
+#pragma unroll 1
+              for (int i = 0; i < n; i++) {
+                const int4 seg = __ldg(ex.segs + s + i);
                 uint32_t off[8];
 #pragma unroll
                 for (int q = 0; q < 8; q++) off[q] = lanes_off(t0 + 32 * q, seg.x, seg.y);
@@ -1570,7 +1590,7 @@ CUtensorMap tensor_map_u8(const void* ptr, int64_t rows, int64_t cols, int box_c
 template <typename T, int BN, int STAGES, bool TMAE, typename EX = GemmPlain>
 void launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my, const CUtensorMap& mr, const GemmArgs& a,
                  cudaStream_t st, const EX& ex = EX()) {
-  constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(TMAE);
+  constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(TMAE || EX::kOn);
   static_assert(smem <= 232448, "GEMM shared memory above the 227 KB per-CTA limit");
   static bool attr = false;
   if (!attr) {
