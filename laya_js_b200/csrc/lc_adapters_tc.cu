@@ -330,6 +330,7 @@ constexpr int BC = 256;                         // columns of X per CTA
 constexpr uint32_t XC_BYTES = 64 * BC * 2;
 struct OuterJob {
   CUtensorMap tmX, tmQ, tmX16, tmQ16;  // boxes of 64 and of 16 rows
+  int whole;                           // tmX brings this many 64-column blocks at once (a 3-D map); 0: one at a time
   float* part;                         // [G + n, rank, C]
   void* dP;
   int C, ctiles;
@@ -388,13 +389,23 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
         if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_adapter_err)) break;
         uint8_t* st = smem + stage * stage_bytes;
         const int n16 = (ch.y + 15) >> 4;
-        mbar_arrive_expect_tx(&full[stage], (uint32_t)((xblocks + qblocks) * n16) * 2048);
+        mbar_arrive_expect_tx(&full[stage], (uint32_t)(((job.whole && n16 == 4 ? job.whole : xblocks) + qblocks) * n16) * 2048);
         auto bring = [&](uint8_t* dst, const CUtensorMap* big, const CUtensorMap* small, int x) {
-          if (n16 == 4) tma_load_2d(dst, big, &full[stage], x, ch.x);
-          else
+          if (n16 == 4) {
+            tma_load_2d(dst, big, &full[stage], x, ch.x);
+          } else {
+#pragma unroll 1
             for (int i = 0; i < n16; i++) tma_load_2d(dst + i * 2048, small, &full[stage], x, ch.x + 16 * i);
+          }
         };
-        for (int b = 0; b < xblocks; b++) bring(st + b * 8192, &job.tmX, &job.tmX16, c0 + 64 * b);
+        if (job.whole && n16 == 4) {
+          tma_load_3d(st, &job.tmX, &full[stage], 0, ch.x, c0 / 64);
+        } else {
+          const CUtensorMap* big = job.whole ? nullptr : &job.tmX;
+#pragma unroll 1
+          for (int b = 0; b < xblocks; b++) bring(st + b * 8192, big, &job.tmX16, c0 + 64 * b);
+        }
+#pragma unroll 1
         for (int b = 0; b < qblocks; b++) bring(st + XC_BYTES + b * 8192, &job.tmQ, &job.tmQ16, b * (args.ucols / 2) + j0);
         used |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
@@ -667,7 +678,10 @@ void outer_t(const AdapterOuter* c, int njobs, const AdapterPlan& p, cudaStream_
     OuterJob& o = a.job[j];
     o.C = (int)c[j].C;
     o.ctiles = (o.C + BC - 1) / BC;
-    o.tmX = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 64, dtype);
+    // columns as blocks of 64, when they are: one load brings the blocks of a CTA, each 64 rows of 128 bytes
+    o.whole = c[j].C % 64 == 0 ? (int)std::min<int64_t>(BC, c[j].C) / 64 : 0;
+    o.tmX = o.whole ? tensor_map_blocks(c[j].X, p.rows, c[j].C, c[j].ld, o.whole, 64, dtype)
+                    : tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 64, dtype);
     o.tmQ = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 64, dtype);
     o.tmX16 = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 16, dtype);
     o.tmQ16 = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 16, dtype);

@@ -1909,6 +1909,20 @@ CUtensorMap tensor_map_3d(const void* ptr, int64_t n, int64_t rows, int64_t cols
   return tensor_map_stack(ptr, n, rows, cols, ld, box_rows, dtype);
 }
 
+CUtensorMap tensor_map_blocks(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_blocks, int box_rows, int dtype) {
+  LC_CHECK(cols % 64 == 0, "tensor map: columns in blocks of 64");
+  CUtensorMap m;
+  cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)(cols / 64)};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * 2, 128};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks};
+  cuuint32_t es[3] = {1, 1, 1};
+  CUresult r = encode_fn()(&m, dtype == LC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(ptr),
+                           dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  LC_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return m;
+}
+
 // In-kernel dequantisation for few rows; LAYA_CUDA_QGEMM_FUSED=0 makes
 // gemm_raw_q decline (the caller then dequantises into a dense scratch).
 bool gemm_use_qfused() {

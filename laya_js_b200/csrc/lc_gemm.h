@@ -85,6 +85,9 @@ namespace lc {
 void gemm_adapted(const GemmAdaptedCall& c, int dtype, cudaStream_t st);
 // Tensor map over n row-major [rows, cols] matrices (row stride ld), boxes of 64 columns x box_rows (128-byte swizzle).
 CUtensorMap tensor_map_3d(const void* ptr, int64_t n, int64_t rows, int64_t cols, int64_t ld, int box_rows, int dtype);
+// Tensor map over a row-major [rows, cols] matrix (cols % 64 == 0) as blocks of 64 columns, coordinates (0, row,
+// block): a box is box_blocks tiles of box_rows x 64, one after the other (128-byte swizzle).
+CUtensorMap tensor_map_blocks(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_blocks, int box_rows, int dtype);
 // y[M, N] = x[M, K] · w[N, K]ᵀ (+ bias) with the tcgen05 kernel. Returns false
 // (and does nothing) when the shapes/dtypes/alignment do not fit the kernel.
 bool gemm_linear(const LcTensor* x2, const LcTensor* w, const LcTensor* bias, LcTensor* y, const GemmEpilogue& ep);
