@@ -9,6 +9,10 @@ gradients, and gradient clipping (include/laya_cuda_adapters.h).
 Tensors are the backend's (``CudaTensor``); ``a`` [n, r, in] and ``bt``
 [n, r, out] hold the adapters of all tenants, ``bt`` the transpose of the
 usual [out, r] matrix (``AdapterBank`` does the layout from host arrays).
+``EncoderAdapters`` puts banks beside the projections of a ``ModernBert``:
+
+    tenants = EncoderAdapters(banks).batch([3, -1, 0], length)   # adapter of each prompt
+    hidden = model.forward(ids, mask, 3, length, tenants=tenants)
 """
 from __future__ import annotations
 
@@ -18,6 +22,7 @@ from typing import Sequence
 import numpy as np
 
 from . import _lib
+from . import compose as Cm
 from .host import HostTensor, f32_to_bf16_bits
 from .interop import SharedMemory
 
@@ -112,3 +117,57 @@ class AdapterBank:
     def dispose(self) -> None:
         for t in (self.a, self.bt, self.scales):
             self.backend.dispose(t)
+
+
+PROJECTIONS = ("Wqkv", "Wo", "Wi", "WoMlp")
+
+
+class EncoderAdapters:
+    """Adapters beside a ModernBert's projections: per layer a dict from
+    projection (``PROJECTIONS``) to its ``AdapterBank``; projections left out
+    have none. Every bank holds the same number of tenants."""
+
+    def __init__(self, banks: Sequence[dict]):
+        sizes = {bank.a.shape[0] for layer in banks for bank in layer.values()}
+        unknown = {name for layer in banks for name in layer} - set(PROJECTIONS)
+        if unknown:
+            raise ValueError(f"EncoderAdapters: unknown projections {sorted(unknown)}, expected {PROJECTIONS}")
+        if len(sizes) != 1:
+            raise ValueError(f"EncoderAdapters: every bank must hold the same number of tenants, got {sorted(sizes)}")
+        self.banks = list(banks)
+        self.n = sizes.pop()
+        self.backend = next(bank for layer in banks for bank in layer.values()).backend
+
+    def batch(self, tenants: Sequence[int], length: int) -> "TenantBatch":
+        """The adapter of each prompt (-1: none) of a padded batch of ``length`` tokens per prompt."""
+        return TenantBatch(self, tenants, length)
+
+    def dispose(self) -> None:
+        for layer in self.banks:
+            for bank in layer.values():
+                bank.dispose()
+
+
+class TenantBatch:
+    """The adapters of one batch of prompts, for ``ModernBert.forward``."""
+
+    def __init__(self, adapters: EncoderAdapters, tenants: Sequence[int], length: int):
+        self.adapters = adapters
+        cu = np.arange(len(tenants) + 1, dtype=np.int64) * int(length)
+        if cu[-1] > np.iinfo(np.int32).max:
+            raise ValueError(f"TenantBatch: {cu[-1]} rows are too many")
+        self.plan = AdapterPlan(adapters.backend, cu, tenants, adapters.n)
+
+    def linear(self, layer: int, name: str, x, w, bias):
+        """The projection ``name`` of a layer with its adapters; a packed weight is multiplied on its own path and the
+        adapters' share added."""
+        b = self.adapters.backend
+        bank = self.adapters.banks[layer].get(name) if layer < len(self.adapters.banks) else None
+        if bank is None:
+            return Cm.linearAny(b, x, w, bias)
+        if Cm.is_quantized(w):
+            return b.add(Cm.linearAny(b, x, w, bias), bank.linear(x, None, None, self.plan))
+        return bank.linear(x, w, bias, self.plan)
+
+    def free(self) -> None:
+        self.plan.free()

@@ -63,11 +63,12 @@ void plan_release(AdapterPlan* p) {
 // Q[t, j] = s_a · Σ_k X[t, k]·P[a, j, k]; rows without an adapter get zeros.
 // A block per row, a warp per rank row j.
 __global__ void __launch_bounds__(128) k_shrink_f32(const float* __restrict__ X, const float* __restrict__ P, const float* __restrict__ scales,
-                                                    const int32_t* __restrict__ row_adapter, float* __restrict__ Q, int C, int r) {
+                                                    const int2* __restrict__ tiles, const int4* __restrict__ segs, float* __restrict__ Q, int C,
+                                                    int r) {
   pdl_trigger();
   pdl_wait();
   const int64_t t = blockIdx.x;
-  const int a = row_adapter[t], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int a = adapter_of_row(tiles, segs, t), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float s = a >= 0 ? (scales ? scales[a] : 1.f) : 0.f;
   const float* x = X + t * C;
   for (int j = warp; j < r; j += 4) {
@@ -86,7 +87,8 @@ __global__ void __launch_bounds__(128) k_shrink_f32(const float* __restrict__ X,
 // W(n, k) = W[n·swn + k·swk]. 64 x 64 tiles, 4 x 4 outputs per thread.
 __global__ void __launch_bounds__(256) k_expand_f32(const float* __restrict__ X, const float* __restrict__ W, int64_t swn, int64_t swk,
                                                     const char* bias, int bias_dtype, const float* __restrict__ Q,
-                                                    const float* __restrict__ P, const int32_t* __restrict__ row_adapter, float* __restrict__ Y,
+                                                    const float* __restrict__ P, const int2* __restrict__ tiles, const int4* __restrict__ segs,
+                                                    float* __restrict__ Y,
                                                     int64_t M, int N, int K, int r) {
   pdl_trigger();
   pdl_wait();
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(256) k_expand_f32(const float* __restrict__ X,
   for (int i = 0; i < 4; i++) {
     const int64_t m = m0 + tm + i;
     if (m >= M) break;
-    const int a = row_adapter[m];
+    const int a = adapter_of_row(tiles, segs, m);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int n = n0 + tn + j;
@@ -266,7 +268,7 @@ Operands operands(const char* op, lc_tensor xh, lc_tensor dyh, lc_tensor wh, lc_
 
 void shrink_f32(const Operands& o, const LcTensor* X, const LcTensor* P, int64_t C, float* Q) {
   launch_chain(k_shrink_f32, dim3((unsigned)o.T), dim3(128), 0, stream(), (const float*)X->data(), (const float*)P->data(), o.scale_ptr(),
-               (const int32_t*)o.plan->row_adapter, Q, (int)C, o.r);
+               (const int2*)o.plan->tiles, (const int4*)o.plan->segs, Q, (int)C, o.r);
   LC_LAUNCHED(1);
 }
 
@@ -278,7 +280,7 @@ void expand_f32(const Operands& o, const LcTensor* X, const LcTensor* P, const f
   LC_CHECK(grid.y <= 65535, "adapters: too many output columns");
   launch_chain(k_expand_f32, grid, dim3(256), 0, stream(), (const float*)X->data(), o.w ? (const float*)o.w->data() : (const float*)nullptr,
                transposed ? (int64_t)1 : o.K, transposed ? o.K : (int64_t)1, bias ? (const char*)bias->data() : (const char*)nullptr,
-               bias ? bias->dtype : 0, Q, (const float*)P->data(), (const int32_t*)o.plan->row_adapter, (float*)Y->data(), o.T, (int)out,
+               bias ? bias->dtype : 0, Q, (const float*)P->data(), (const int2*)o.plan->tiles, (const int4*)o.plan->segs, (float*)Y->data(), o.T, (int)out,
                (int)in, o.r);
   LC_LAUNCHED(1);
 }
@@ -357,8 +359,9 @@ struct Chained {
   }
 };
 
-// Scratch for Q and the product that fills it.
-AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_t C, Held& held) {
+// Bytes of a Q, and the product that fills it.
+size_t q_bytes(const Operands& o) { return ((size_t)o.T * adapter_u_cols(o.r) * 2 + 255) / 256 * 256; }
+AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_t C, void* Q) {
   AdapterShrink c;
   c.X = X.p;
   c.P = P.p;
@@ -368,7 +371,7 @@ AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_
   c.n = o.n;
   c.rank = o.r;
   c.scales = o.scale_ptr();
-  c.Q = held.scratch((size_t)o.T * adapter_u_cols(o.r) * 2);
+  c.Q = Q;
   return c;
 }
 
@@ -416,7 +419,7 @@ void linear(const Operands& o, LcTensor* y, Held& held) {
   const Rows x = pad.of(o.x, o.T, o.K), w = pad.of(o.w, o.N, o.K), a = pad.of(o.a, (int64_t)o.n * o.r, o.K),
              b = pad.of(o.b, (int64_t)o.n * o.r, o.N);
   pad.run();
-  const AdapterShrink u = shrink_job(o, x, a, o.K, held);
+  const AdapterShrink u = shrink_job(o, x, a, o.K, held.scratch(q_bytes(o)));
   shrink(&u, 1, o);
   const Chained chained(o);
   expand_tc(o, x, w, b, u.Q, false, y);
@@ -446,36 +449,35 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
   const Rows dy = pad.of(o.dy, o.T, o.N), x = da || db ? pad.of(o.x, o.T, o.K) : Rows{}, w = dx ? pad.of(o.w, o.N, o.K) : Rows{},
              a = dx || db ? pad.of(o.a, (int64_t)o.n * o.r, o.K) : Rows{}, b = dx || da ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : Rows{};
   pad.run();
-  AdapterShrink q[2];
-  int nq = 0;
-  const void *g = nullptr, *u = nullptr;
-  if (dx || da) {
-    q[nq] = shrink_job(o, dy, b, o.N, held);
-    g = q[nq++].Q;
-  }
-  if (db) {
-    q[nq] = shrink_job(o, x, a, o.K, held);
-    u = q[nq++].Q;
-  }
-  if (!nq) return;
   AdapterOuter out[2];
   int no = 0;
-  auto job = [&](const void* Q, const Rows& X, int64_t C, LcTensor* dP) {
-    AdapterOuter& c = out[no];
+  auto job = [&](const Rows& X, int64_t C, LcTensor* dP) -> AdapterOuter& {
+    AdapterOuter& c = out[no++];
     c.X = X.p;
-    c.Q = Q;
     c.C = C;
     c.ld = X.ld;
     c.rank = o.r;
     c.dP = dP->data();
-    no++;
+    return c;
   };
-  if (db) job(u, dy, o.N, db);
-  if (da) job(g, x, o.K, da);
+  AdapterOuter* of_u = db ? &job(dy, o.N, db) : nullptr;
+  AdapterOuter* of_g = da ? &job(x, o.K, da) : nullptr;
+  const int nq = (dx || da ? 1 : 0) + (db ? 1 : 0);
+  if (!nq) return;
+  char* scratch = (char*)held.scratch(nq * q_bytes(o) + (no ? adapter_part_bytes(out, no, *o.plan) : 0));
+  AdapterShrink q[2];
+  void* Q = scratch;
+  if (db) {
+    q[0] = shrink_job(o, x, a, o.K, Q);
+    of_u->Q = Q;
+    Q = (char*)Q + q_bytes(o);
+  }
+  if (dx || da) q[nq - 1] = shrink_job(o, dy, b, o.N, Q);
+  if (da) of_g->Q = Q;
   shrink(q, nq, o);
   const Chained chained(o);
-  if (no) adapter_outer_tc(out, no, *o.plan, o.dtype, stream());
-  if (dx) expand_tc(o, dy, w, a, g, true, dx);
+  if (no) adapter_outer_tc(out, no, scratch + nq * q_bytes(o), *o.plan, o.dtype, stream());
+  if (dx) expand_tc(o, dy, w, a, Q, true, dx);
 }
 
 }  // namespace
@@ -520,8 +522,6 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
     spans[2 * k] = s.lo;
     spans[2 * k + 1] = s.hi;
   }
-  std::vector<int32_t> row_adapter(T, -1);
-  for (auto& s : segs) std::fill(row_adapter.begin() + s.lo, row_adapter.begin() + s.hi, s.a);
   std::vector<int32_t> seg4, tiles;
   for (auto& g : segs) seg4.insert(seg4.end(), {g.lo, g.hi, g.a, 0});
   for (int64_t m0 = 0, k = 0; m0 < T; m0 += 128) {
@@ -550,7 +550,7 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
     image.resize((image.size() + 63) / 64 * 64);
     return off;
   };
-  const size_t o_rows = put(row_adapter), o_spans = put(spans), o_ptr = put(span_ptr), o_segs = put(seg4), o_tiles = put(tiles),
+  const size_t o_spans = put(spans), o_ptr = put(span_ptr), o_segs = put(seg4), o_tiles = put(tiles),
                o_chunks = put(chunks), o_chunk_ptr = put(chunk_ptr), o_empty = put(empty),
                o_pieces = put(pieces);
   struct Guard {
@@ -568,7 +568,6 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   // pageable source: staged when the call returns
   CUDA_OK(cudaMemcpyAsync(p->dev, image.data(), image.size() * 4, cudaMemcpyHostToDevice, st));
   CUDA_OK(cudaEventRecord(p->built, st));
-  p->row_adapter = p->dev + o_rows;
   p->spans = (int2*)(p->dev + o_spans);
   p->span_ptr = p->dev + o_ptr;
   p->segs = (int4*)(p->dev + o_segs);

@@ -9,7 +9,6 @@ constexpr int kAdapterMaxRank = 256;
 struct AdapterPlan {
   int rows = 0, n_adapters = 0, nsegs = 0, nchunks = 0, nempty = 0, npieces = 0;
   int32_t* dev = nullptr;          // one allocation behind the arrays below
-  int32_t* row_adapter = nullptr;  // [rows]: the adapter of each row, -1 = none
   int4* segs = nullptr;            // [nsegs]: row ranges with an adapter, ascending: lo, hi, adapter
   int2* tiles = nullptr;           // per 128 rows: the first segment that meets them, and how many do
   int2* spans = nullptr;           // [nsegs]: the row ranges adapter by adapter, ascending within one
@@ -24,6 +23,20 @@ struct AdapterPlan {
   bool settled = false;            // `built` has been seen complete
   bool shared = false;             // used on another stream than built_on
 };
+
+// The adapter of row t, or -1: the last of the segments meeting its 128 rows that begins at or before it.
+__device__ __forceinline__ int adapter_of_row(const int2* tiles, const int4* segs, int64_t t) {
+  const int2 tile = __ldg(tiles + t / 128);
+  int lo = tile.x, n = tile.y;
+  if (!n) return -1;
+  while (n > 1) {
+    const int h = n / 2;
+    if (__ldg(&segs[lo + h].x) <= t) lo += h, n -= h;
+    else n = h;
+  }
+  const int4 s = __ldg(segs + lo);
+  return t >= s.x && t < s.y ? s.z : -1;
+}
 
 // 16-bit columns of a row of Q (lc_adapters_tc.cu): two parts of the rank
 // rounded up to 16, or to 64 above 32, where a part fills whole 128-byte rows.
@@ -66,10 +79,15 @@ struct AdapterOuter {
 namespace lc {
 // One or two products over the same rows, ranks and scales.
 void adapter_shrink_tc(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
-void adapter_outer_tc(const AdapterOuter* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
-// The forms for few rows (lc_adapters_rows.cu): false, with nothing launched, for more than these products.
+size_t adapter_part_bytes(const AdapterOuter* c, int njobs, const AdapterPlan& p);  // f32 partial sums of adapter_outer_tc
+void adapter_outer_tc(const AdapterOuter* c, int njobs, void* part, const AdapterPlan& p, int dtype, cudaStream_t st);
+// The forms for few rows (lc_adapters_rows.cu): false, with nothing launched,
+// above so many multiplications. Measured (bf16, rank 16, 768 columns; dot
+// products against tensor cores, one request / requests of 8 rows): shrink
+// 25 M 6.0 / 8.1 us against 8.3 / 16.4, 50 M 10.1 / 13.7 against 8.5 / 16.2;
+// linear 28 M 7.3 us against 9.4 / 9.7, 57 M 13.3 against 9.5 / 10.4.
 constexpr int kRowsMost = 16384;
-constexpr int64_t kRowsShrinkMost = 1 << 27, kRowsLinearMost = 1 << 27;
+constexpr int64_t kRowsShrinkMost = 3 << 24, kRowsLinearMost = 1 << 25;
 bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
 bool adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int dtype, cudaStream_t st);
 }  // namespace lc

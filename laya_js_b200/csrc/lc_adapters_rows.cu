@@ -125,7 +125,8 @@ struct RowsLinearArgs {
   void* y;
   int64_t M, ldx, ldw, ldb, ldy;
   int N, K, rank, ucols, bias_dtype, defer;
-  const int32_t* row_adapter;
+  const int2* tiles;
+  const int4* segs;
 };
 
 // grid: (groups of 16 columns, groups of 8 rows)
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_rows(const __grid_constan
   const int64_t t = t0 + (lane & 7);
   if (warp >= 4 || t >= args.M || n >= args.N) return;
   if (args.bias) v += ld_as<float>((const char*)args.bias, args.bias_dtype, n);
-  const int a = __ldg(args.row_adapter + t);
+  const int a = adapter_of_row(args.tiles, args.segs, t);
   if (a >= 0) {
     const T* q = (const T*)args.Q + t * args.ucols;
     const T* p = (const T*)args.bank + (int64_t)a * args.rank * args.ldb + n;
@@ -191,7 +192,8 @@ void linear_rows_t(const GemmAdaptedCall& c, const AdapterPlan& p, cudaStream_t 
   a.rank = c.share.rank;
   a.ucols = c.share.u_cols;
   a.defer = c.after_share ? 1 : 0;
-  a.row_adapter = p.row_adapter;
+  a.tiles = p.tiles;
+  a.segs = p.segs;
   launch_chain(k_linear_rows<T>, dim3((unsigned)((c.N + COLS - 1) / COLS), (unsigned)((c.M + ROWS - 1) / ROWS)), dim3(THREADS), 0, st, a);
   LC_LAUNCHED(1);
 }

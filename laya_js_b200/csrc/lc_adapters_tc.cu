@@ -634,14 +634,15 @@ void shrink_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStrea
 }
 
 constexpr int kMaxRuns = 64;  // JoinArgs::shared holds a boundary each
-// Runs of blocks per tile of columns.
-int adapter_runs(int tiles, int nchunks) {
-  // one wave of CTAs, or two where one would leave SMs idle
+// Runs of blocks per tile of columns: one wave of CTAs, or two where one would leave SMs idle.
+int adapter_runs(const AdapterOuter* c, int njobs, const AdapterPlan& p) {
+  int64_t tiles = 0;
+  for (int j = 0; j < njobs; j++) tiles += (c[j].C + BC - 1) / BC * std::max(1, adapter_u_cols(c[j].rank) / 128);
   const int sms = num_sms();
   int G = 1;
   double best = 0;
-  for (int f = 1; f <= kMaxRuns && f <= nchunks; f++) {
-    const int64_t ctas = (int64_t)tiles * f, waves = (ctas + sms - 1) / sms;
+  for (int f = 1; f <= kMaxRuns && f <= p.nchunks; f++) {
+    const int64_t ctas = tiles * f, waves = (ctas + sms - 1) / sms;
     const double fill = (double)ctas / (double)(waves * sms);
     if (fill > best + 0.03) best = fill, G = f;
     if (waves > 2) break;
@@ -650,7 +651,7 @@ int adapter_runs(int tiles, int nchunks) {
 }
 
 template <typename T>
-void outer_t(const AdapterOuter* c, int njobs, const AdapterPlan& p, cudaStream_t st) {
+void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p, cudaStream_t st) {
   const int dtype = std::is_same<T, __half>::value ? LC_F16 : LC_BF16;
   OuterArgs a{};
   a.rank = c[0].rank;
@@ -664,20 +665,13 @@ void outer_t(const AdapterOuter* c, int njobs, const AdapterPlan& p, cudaStream_
   a.tmem_cols = tmem_columns(4 * a.nmma);
   a.chunks = p.chunks;
   a.chunk_ptr = p.chunk_ptr;
+  a.G = adapter_runs(c, njobs, p);
   int ctiles = 0;
-  for (int j = 0; j < njobs; j++) ctiles += (int)((c[j].C + BC - 1) / BC);
-  a.G = adapter_runs(ctiles * a.rgroups, p.nchunks);
-  struct Partials {
-    void* p[2] = {nullptr, nullptr};
-    ~Partials() {
-      for (void* q : p)
-        if (q) dfree(q);
-    }
-  } part;
   for (int j = 0; j < njobs; j++) {
     OuterJob& o = a.job[j];
     o.C = (int)c[j].C;
     o.ctiles = (o.C + BC - 1) / BC;
+    ctiles += o.ctiles;
     // columns as blocks of 64, when they are: one load brings the blocks of a CTA, each 64 rows of 128 bytes
     o.whole = c[j].C % 64 == 0 ? (int)std::min<int64_t>(BC, c[j].C) / 64 : 0;
     o.tmX = o.whole ? tensor_map_blocks(c[j].X, p.rows, c[j].C, c[j].ld, o.whole, 64, dtype)
@@ -686,7 +680,8 @@ void outer_t(const AdapterOuter* c, int njobs, const AdapterPlan& p, cudaStream_
     o.tmX16 = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 16, dtype);
     o.tmQ16 = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 16, dtype);
     o.dP = c[j].dP;
-    if (a.G > 1) o.part = (float*)(part.p[j] = dmalloc((size_t)(a.G + p.n_adapters) * a.rank * c[j].C * 4));
+    o.part = part;
+    part += (a.G + p.n_adapters) * (int64_t)a.rank * c[j].C;
   }
   const size_t smem = (size_t)a.stages * (XC_BYTES + a.q_bytes) + 1024 + 512;
   static bool attr = false;
@@ -729,8 +724,15 @@ void adapter_shrink_tc(const AdapterShrink* c, int njobs, const AdapterPlan& p, 
   dtype == LC_F16 ? shrink_t<__half>(c, njobs, p, st) : shrink_t<__nv_bfloat16>(c, njobs, p, st);
 }
 
-void adapter_outer_tc(const AdapterOuter* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st) {
-  dtype == LC_F16 ? outer_t<__half>(c, njobs, p, st) : outer_t<__nv_bfloat16>(c, njobs, p, st);
+size_t adapter_part_bytes(const AdapterOuter* c, int njobs, const AdapterPlan& p) {
+  const int G = adapter_runs(c, njobs, p);
+  size_t n = 0;
+  for (int j = 0; j < njobs; j++) n += G > 1 ? (size_t)(G + p.n_adapters) * c[j].rank * c[j].C * 4 : 0;
+  return n;
+}
+
+void adapter_outer_tc(const AdapterOuter* c, int njobs, void* part, const AdapterPlan& p, int dtype, cudaStream_t st) {
+  dtype == LC_F16 ? outer_t<__half>(c, njobs, (float*)part, p, st) : outer_t<__nv_bfloat16>(c, njobs, (float*)part, p, st);
 }
 
 std::string take_adapter_errors() {

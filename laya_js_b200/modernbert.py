@@ -136,22 +136,25 @@ class ModernBert:
         return b.scope(lambda: b.layerNorm(Cm.embeddingAny(b, w.tokEmbeddings, ids), w.embNorm[0], w.embNorm[1],
                                            self.config["normEps"]))
 
-    def layer(self, i: int, x, mask):
-        """index.ts:342-357."""
+    def layer(self, i: int, x, mask, tenants=None):
+        """index.ts:342-357; ``tenants`` (adapters.TenantBatch) adds each prompt's adapters to the projections."""
         b, c, w = self.backend, self.config, self.weights.layers[i]
+
+        def linear(name, h, weight, bias):
+            return Cm.linearAny(b, h, weight, bias) if tenants is None else tenants.linear(i, name, h, weight, bias)
 
         def f():
             B, L, H = x.shape
             nh, hd = c["numAttentionHeads"], c["headDim"]
             h = b.layerNorm(x, w.attnNorm[0], w.attnNorm[1], c["normEps"]) if w.attnNorm else x
-            qkv = b.transpose(b.reshape(Cm.linearAny(b, h, w.Wqkv, w.WqkvBias), [B, L, 3, nh, hd]), [2, 0, 3, 1, 4])
+            qkv = b.transpose(b.reshape(linear("Wqkv", h, w.Wqkv, w.WqkvBias), [B, L, 3, nh, hd]), [2, 0, 3, 1, 4])
             q, k, v = [b.reshape(t, [B, nh, L, hd]) for t in b.split(qkv, 3, 0)]
             base = c["ropeBase"][w.kind]
             att = b.sdpa(b.rope(q, base), b.rope(k, base), v, mask, hd ** -0.5)
             merged = b.reshape(b.transpose(att, [0, 2, 1, 3]), [B, L, H])
-            x1 = b.add(x, Cm.linearAny(b, merged, w.Wo, w.WoBias))
-            m = Cm.linearAny(b, b.layerNorm(x1, w.mlpNorm[0], w.mlpNorm[1], c["normEps"]), w.Wi, w.WiBias)
-            return b.add(x1, Cm.linearAny(b, Cm.geglu(b, m), w.WoMlp, w.WoMlpBias))
+            x1 = b.add(x, linear("Wo", merged, w.Wo, w.WoBias))
+            m = linear("Wi", b.layerNorm(x1, w.mlpNorm[0], w.mlpNorm[1], c["normEps"]), w.Wi, w.WiBias)
+            return b.add(x1, linear("WoMlp", Cm.geglu(b, m), w.WoMlp, w.WoMlpBias))
         return b.scope(f)
 
     def finalNorm(self, x):
@@ -179,15 +182,15 @@ class ModernBert:
             if t is not None:
                 b.dispose(t)
 
-    def forward(self, input_ids, attention_mask, B: int, L: int, onStage: Optional[Callable] = None):
-        """index.ts:394-401."""
+    def forward(self, input_ids, attention_mask, B: int, L: int, onStage: Optional[Callable] = None, tenants=None):
+        """index.ts:394-401; ``tenants``: the adapters of each of the B prompts (adapters.EncoderAdapters.batch)."""
         inp = self.uploadInputs(input_ids, attention_mask, B, L)
         try:
-            return self.encode(inp, onStage)
+            return self.encode(inp, onStage, tenants)
         finally:
             self.disposeInputs(inp)
 
-    def encode(self, inp: dict, onStage: Optional[Callable] = None):
+    def encode(self, inp: dict, onStage: Optional[Callable] = None, tenants=None):
         """index.ts:407-429."""
         b, c = self.backend, self.config
         kept = []
@@ -201,7 +204,7 @@ class ModernBert:
             x = self.embeddings(inp["ids"])
             emit("embeddings", x, False)
             for i in range(c["numHiddenLayers"]):
-                nxt = self.layer(i, x, masks[c["layerTypes"][i]])
+                nxt = self.layer(i, x, masks[c["layerTypes"][i]], tenants)
                 if not any(k is x for k in kept):
                     b.dispose(x)
                 x = nxt
