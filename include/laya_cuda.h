@@ -61,9 +61,11 @@ int lc_tensor_info(lc_tensor t, int* dtype, int* ndim, int64_t* shape /* [8] */)
 /* Device pointer of a dense tensor (0 when it is a strided view). Read-only:
    the library treats tensors as immutable (only lc_copy_into writes one). */
 int lc_tensor_data(lc_tensor t, uint64_t* dptr);
-/* lc_tensor_data and lc_tensor_free of n handles in one call (free stops at the first dead handle). */
-int lc_tensors_data(const lc_tensor* ts, int n, uint64_t* dptrs);
-int lc_tensors_free(const lc_tensor* ts, int n);
+/* A dense tensor as a DLPack managed tensor (DLManagedTensor*, for a capsule
+   named "dltensor"), which takes the handle over: its deleter frees the tensor
+   in the order of the library's stream at that time. The library treats the
+   memory as immutable; a strided view is an error. u16, u32 and u64 count. */
+int lc_tensor_to_dlpack(lc_tensor t, uint64_t* managed);
 /* index.ts:163-164 flush: waits for queued work. */
 int lc_flush(void);
 

@@ -24,7 +24,6 @@ import numpy as np
 from . import _lib
 from . import compose as Cm
 from .host import HostTensor, f32_to_bf16_bits
-from .interop import SharedMemory
 
 
 class AdapterPlan:
@@ -81,10 +80,7 @@ def clip_grad_norm(backend, grads: Sequence, max_norm: float):
     outs = (C.c_uint64 * max(1, n))()
     norm = C.c_uint64()
     _lib.call("lc_clip_grad_norm", outs, C.byref(norm), hs, n, float(max_norm))
-    clipped = [b._wrap(h, g.dtype, g.shape) for h, g in zip(outs, grads)]
-    if n > 1:
-        SharedMemory(b, clipped)
-    return clipped, b._wrap(norm.value, "f32", ())
+    return [b._wrap(h, g.dtype, g.shape) for h, g in zip(outs, grads)], b._wrap(norm.value, "f32", ())
 
 
 def _host(dtype: str, v) -> HostTensor:

@@ -371,6 +371,31 @@ LcTensor* contiguous(LcTensor* x) {
 
 using namespace lc;
 
+// The structures of the DLPack exchange format (version 0), by which array
+// libraries hand tensors to one another.
+namespace {
+struct DLDevice { int32_t device_type, device_id; };
+struct DLDataType { uint8_t code, bits; uint16_t lanes; };
+struct DLTensor {
+  void* data;
+  DLDevice device;
+  int32_t ndim;
+  DLDataType dtype;
+  int64_t* shape;
+  int64_t* strides;  // null: dense
+  uint64_t byte_offset;
+};
+struct DLManagedTensor {
+  DLTensor dl_tensor;
+  void* manager_ctx;
+  void (*deleter)(DLManagedTensor*);
+};
+struct DlpackTensor {
+  DLManagedTensor managed{};  // first: the deleter gets its address
+  int64_t shape[LC_MAX_DIMS];
+};
+}  // namespace
+
 extern "C" {
 
 const char* lc_last_error(void) { return g_err.c_str(); }
@@ -574,18 +599,25 @@ int lc_tensor_data(lc_tensor h, uint64_t* dptr) {
   LC_API_END
 }
 
-int lc_tensors_data(const lc_tensor* hs, int n, uint64_t* dptrs) {
+int lc_tensor_to_dlpack(lc_tensor h, uint64_t* managed) {
   LC_API_BEGIN
-  for (int i = 0; i < n; i++) {
-    LcTensor* t = check(hs[i], "data");
-    dptrs[i] = t->contiguous() ? reinterpret_cast<uint64_t>(t->data()) : 0;
-  }
-  LC_API_END
-}
-
-int lc_tensors_free(const lc_tensor* hs, int n) {
-  LC_API_BEGIN
-  for (int i = 0; i < n; i++) release(check(hs[i], "dispose"));
+  LcTensor* t = check(h, "toDlpack");
+  LC_CHECK(t->contiguous(), "toDlpack: the tensor must be dense");
+  // DLDataTypeCode: 0 int, 1 uint, 2 float, 4 bfloat, 6 bool
+  static const uint8_t code[LC_NUM_DTYPES] = {2, 2, 4, 0, 6, 1, 0, 1, 0, 1, 1, 0, 2};
+  auto* m = new DlpackTensor();
+  m->managed.dl_tensor.data = t->data();
+  m->managed.dl_tensor.device = {2 /* kDLCUDA */, S().device};
+  m->managed.dl_tensor.ndim = t->ndim;
+  m->managed.dl_tensor.dtype = {code[t->dtype], (uint8_t)(dtype_size(t->dtype) * 8), 1};
+  for (int i = 0; i < t->ndim; i++) m->shape[i] = t->shape[i];
+  m->managed.dl_tensor.shape = m->shape;
+  m->managed.manager_ctx = t;
+  m->managed.deleter = [](DLManagedTensor* d) {
+    release(static_cast<LcTensor*>(d->manager_ctx));  // (a tensor already gone with the library is not freed again)
+    delete reinterpret_cast<DlpackTensor*>(d);
+  };
+  *managed = reinterpret_cast<uint64_t>(&m->managed);
   LC_API_END
 }
 

@@ -11,7 +11,6 @@ tensor handed over is read, not written, while a queued op may still use it.
 from __future__ import annotations
 
 import ctypes as C
-from math import prod
 
 from . import _lib
 from .backend import CudaTensor, _i64
@@ -46,102 +45,23 @@ def fromTorch(b, t) -> CudaTensor:
     return r
 
 
-class _Owner:
-    """Device memory of a tensor as torch reads it; disposes the tensor when torch lets go."""
-
-    __slots__ = ("b", "t", "__cuda_array_interface__")
-
-    def __init__(self, b, t, ptr, typestr):
-        self.b, self.t = b, t
-        self.__cuda_array_interface__ = {"shape": t.shape, "typestr": typestr, "data": (ptr, False), "version": 2, "strides": None}
-
-    def __del__(self):
-        try:
-            self.b.dispose(self.t)
-        except Exception:
-            pass  # the library may be gone at interpreter exit
-
-
-_TYPESTR = {"f32": "<f4", "f16": "<f2", "bf16": "<i2", "i32": "<i4", "bool": "|b1", "u8": "|u1", "i8": "|i1", "i16": "<i2", "i64": "<i8",
-            "f64": "<f8"}
-
-
-class _Owners:
-    """Memory that several handles share, as torch reads it; frees those given to torch when torch lets go."""
-
-    __slots__ = ("b", "taken", "__cuda_array_interface__")
-
-    def __init__(self, b, count, ptr, typestr):
-        self.b, self.taken = b, []
-        self.__cuda_array_interface__ = {"shape": (count,), "typestr": typestr, "data": (ptr, False), "version": 2, "strides": None}
-
-    def __del__(self):
-        try:
-            if self.taken and not self.b._destroyed:
-                _lib.call("lc_tensors_free", (C.c_uint64 * len(self.taken))(*self.taken), len(self.taken))
-        except Exception:
-            pass  # the library may be gone at interpreter exit
-
-
-class SharedMemory:
-    """Dense tensors that an op returned in one allocation (each one's ``keep``
-    is (this, its index)): torch gets views of one storage over it."""
-
-    __slots__ = ("b", "ts", "ptrs", "flat")
-
-    def __init__(self, b, ts):
-        self.b, self.ts, self.ptrs, self.flat = b, [(t.handle, t.dtype, t.shape) for t in ts], None, {}
-        for i, t in enumerate(ts):
-            t.keep = (self, i)
-
-    def _flat(self, dtype: str):
-        """(a flat torch tensor from the first to the last tensor of a dtype, its owner's list, address, value size)."""
-        import torch
-        size = int(_TYPESTR[dtype][-1])
-        mine = [(p, prod(sh) * size) for p, (_, dt, sh) in zip(self.ptrs, self.ts) if dt == dtype and 0 not in sh]
-        lo, hi = min(p for p, _ in mine), max(p + n for p, n in mine)
-        owner = _Owners(self.b, (hi - lo) // size, lo, _TYPESTR[dtype])
-        flat = torch.as_tensor(owner, device=f"cuda:{self.b.device}")
-        return flat.view(torch.bfloat16) if dtype == "bf16" else flat, owner.taken, lo, size
-
-    def torch(self, t: CudaTensor, i: int):
-        if self.ptrs is None:
-            n = len(self.ts)
-            ptrs = (C.c_uint64 * n)()
-            _lib.call("lc_tensors_data", (C.c_uint64 * n)(*[h for h, _, _ in self.ts]), n, ptrs)
-            self.ptrs = list(ptrs)
-        if t.dtype not in self.flat:
-            self.flat[t.dtype] = self._flat(t.dtype)
-        flat, taken, lo, size = self.flat[t.dtype]
-        strides, s = [], 1
-        for d in reversed(t.shape):
-            strides.append(s)
-            s *= d
-        taken.append(t.handle)
-        t.disposed = True  # the handle is torch's now
-        return flat.as_strided(t.shape, strides[::-1], (self.ptrs[i] - lo) // size)
+_capsule = C.pythonapi.PyCapsule_New
+_capsule.restype, _capsule.argtypes = C.py_object, [C.c_void_p, C.c_char_p, C.c_void_p]
 
 
 def toTorch(b, t: CudaTensor):
-    """``t`` as a torch tensor over the same memory. The handle now belongs to
-    the torch tensor (it is disposed with it, in the order of the library's
-    stream) and is not used further."""
+    """``t`` as a torch tensor over the same memory (DLPack). The handle now
+    belongs to the torch tensor, which frees it in the order of the library's
+    stream, and is not used further; a strided view is copied first."""
     import torch
-    if t.dtype not in _TYPESTR:
-        raise TypeError(f"toTorch: no torch dtype for {t.dtype}")
-    if type(t.keep) is tuple and not t.disposed and 0 not in t.shape:
-        return t.keep[0].torch(t, t.keep[1])
-    if 0 in t.shape:
-        out = torch.empty(t.shape, dtype=getattr(torch, _NAMES[t.dtype]), device=f"cuda:{b.device}")
-        b.dispose(t)
-        return out
-    ptr = C.c_uint64()
-    _lib.call("lc_tensor_data", b._h(t, "toTorch"), C.byref(ptr))
-    if not ptr.value:
-        d = b.cast(t, t.dtype)  # a dense copy of the strided view
+    out = C.c_uint64()
+    try:
+        _lib.call("lc_tensor_to_dlpack", b._h(t, "toTorch"), C.byref(out))
+    except _lib.LayaCudaError as e:
+        if "dense" not in str(e):
+            raise
+        d = b.cast(t, t.dtype)
         b.dispose(t)
         return toTorch(b, d)
-    for frame in b._scopes:  # no longer a scope's to dispose
-        frame[:] = [x for x in frame if x is not t]
-    out = torch.as_tensor(_Owner(b, t, ptr.value, _TYPESTR[t.dtype]), device=f"cuda:{b.device}")
-    return out.view(torch.bfloat16) if t.dtype == "bf16" else out
+    t.disposed = True
+    return torch.from_dlpack(_capsule(out.value, b"dltensor", None))

@@ -149,7 +149,7 @@ def test_refusals_and_no_gradients():
 
 def test_outputs_as_torch_tensors():
     """The outputs share an allocation: it lives until the last torch tensor
-    and the last handle over it are gone."""
+    over it is gone."""
     import torch
 
     from laya_js_b200 import _lib, interop
