@@ -30,7 +30,7 @@ extern "C" {
  * -1 = none, else below n_adapters). Both arrays are copied before the call
  * returns. A plan serves every layer's projections of its batch; it is built
  * on the library stream, may be used on another (the use waits for the
- * build), and has to outlive the graphs recorded with it. At most 2^31 - 1
+ * build), and has to outlive the graphs recorded with it. At most 2^31 - 1024
  * rows.
  */
 int lc_adapter_plan_create(uint64_t* plan, const int32_t* cu_rows, const int32_t* adapters, int nseg, int n_adapters);
@@ -42,8 +42,10 @@ int lc_adapter_plan_free(uint64_t plan);
  * that is computed elsewhere, such as a packed one); bias [N] or 0;
  * a [n, r, K], b [n, r, N] and scales f32 [n] (0 = every scale 1) with
  * n = the plan's n_adapters. x, w, a and b share a dtype: f32, f16 or bf16.
- * Sums are held in f32 and rounded once, u included: no row's result depends
- * on another row or on another request's adapter, finite or not.
+ * Sums are held in f32 and rounded once; with f16 and bf16 u is held as two
+ * 16-bit parts, exact to 2^-22 and 2^-16 of each value (f16: to 2^-25, and up
+ * to 131,008). No row's result depends on another row or on another request's
+ * adapter, finite or not.
  */
 int lc_adapter_linear(lc_tensor* out, lc_tensor x, lc_tensor w, lc_tensor bias, lc_tensor a, lc_tensor b, lc_tensor scales, uint64_t plan);
 

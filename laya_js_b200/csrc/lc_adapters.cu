@@ -503,6 +503,7 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
              "adapter plan: request " + std::to_string(i) + " uses adapter " + std::to_string(adapters[i]) + " of " + std::to_string(n_adapters));
   }
   const int T = cu_rows[nseg];
+  LC_CHECK(T <= INT32_MAX - 1023, "adapter plan: too many rows");
   // the requests that have rows and an adapter; neighbours with the same adapter become one
   struct Seg { int lo, hi, a; };
   std::vector<Seg> segs;

@@ -124,19 +124,19 @@ struct RowsLinearArgs {
   const void *x, *w, *bank, *Q, *bias;
   void* y;
   int64_t M, ldx, ldw, ldb, ldy;
-  int N, K, rank, ucols, bias_dtype, defer;
+  int N, K, rank, ucols, bias_dtype, defer, ngroups;  // ngroups: groups of 16 columns
   const int2* tiles;
   const int4* segs;
 };
 
-// grid: (groups of 16 columns, groups of 8 rows)
+// grid: groups of 16 columns, for each group of 8 rows
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1) k_linear_rows(const __grid_constant__ RowsLinearArgs args) {
   __shared__ float red[128];
   if (!args.defer) pdl_wait();
   pdl_trigger();
-  const int n0 = blockIdx.x * COLS;
-  const int64_t t0 = (int64_t)blockIdx.y * ROWS;
+  const int n0 = (int)(blockIdx.x % args.ngroups) * COLS;
+  const int64_t t0 = (int64_t)(blockIdx.x / args.ngroups) * ROWS;
   float v = 0.f;
   if (args.w)
     v = dot_piece<T>((const T*)args.x + t0 * args.ldx, args.ldx, (int)min((int64_t)ROWS, args.M - t0), (const T*)args.w + n0 * args.ldw,
@@ -194,7 +194,8 @@ void linear_rows_t(const GemmAdaptedCall& c, const AdapterPlan& p, cudaStream_t 
   a.defer = c.after_share ? 1 : 0;
   a.tiles = p.tiles;
   a.segs = p.segs;
-  launch_chain(k_linear_rows<T>, dim3((unsigned)((c.N + COLS - 1) / COLS), (unsigned)((c.M + ROWS - 1) / ROWS)), dim3(THREADS), 0, st, a);
+  a.ngroups = (int)((c.N + COLS - 1) / COLS);
+  launch_chain(k_linear_rows<T>, dim3((unsigned)(a.ngroups * ((c.M + ROWS - 1) / ROWS))), dim3(THREADS), 0, st, a);
   LC_LAUNCHED(1);
 }
 

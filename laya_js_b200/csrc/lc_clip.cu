@@ -207,7 +207,9 @@ void clip_launch(const std::vector<ClipTensor>& ts, double max_norm, float* norm
   auto tab = std::make_unique<ClipTable<N>>();
   int nparts = 0;
   for (int g : grid) nparts += g;
-  for (int pass = 0; pass < 2; pass++)
+  std::unique_ptr<PdlScope> chained;  // the second pass starts while the first drains, and waits for it
+  for (int pass = 0; pass < 2; pass++) {
+    if (pass) chained = std::make_unique<PdlScope>();
     for (size_t l = 0, part0 = 0; l < grid.size(); part0 += grid[l], l++) {
       const int lo = first[l], n = first[l + 1] - lo;
       tab->h = {n, 0, (int)part0, nparts, max_norm, parts, norm};
@@ -219,6 +221,7 @@ void clip_launch(const std::vector<ClipTensor>& ts, double max_norm, float* norm
       launch_chain(pass ? k_clip_scale<N> : k_clip_norm<N>, dim3(grid[l]), dim3(kThreads), 0, st, *tab);
       LC_LAUNCHED(1);
     }
+  }
 }
 
 }  // namespace
@@ -231,12 +234,10 @@ int lc_clip_grad_norm(lc_tensor* outs, lc_tensor* norm_out, const lc_tensor* gra
   LC_CHECK(max_norm >= 0, "clip_grad_norm: max_norm must be >= 0");
   struct Held {
     std::vector<LcTensor*> ts;
-    std::vector<void*> mem;
     ~Held() {
       for (auto* t : ts) release(t);
-      for (void* p : mem) dfree(p);
     }
-  } held;
+  } held, results;  // temporaries; what the caller gets, released here if the call fails
   std::vector<LcTensor*> in(n);
   int64_t bytes = 0;
   std::vector<int64_t> offset(n);
@@ -252,8 +253,6 @@ int lc_clip_grad_norm(lc_tensor* outs, lc_tensor* norm_out, const lc_tensor* gra
     if (c != in[i]) held.ts.push_back(c);
     in[i] = c;
   }
-  LcTensor* norm = alloc(LC_F32, {});
-  held.ts.push_back(norm);
   LcTensor* all = alloc(LC_U8, {bytes});
   held.ts.push_back(all);
   std::vector<LcTensor*> out(n);
@@ -264,7 +263,7 @@ int lc_clip_grad_norm(lc_tensor* outs, lc_tensor* norm_out, const lc_tensor* gra
     for (int d = (int)sh.size() - 1; d >= 0; d--) st[d] = s, s *= sh[d];
     out[i] = view_of(all, sh, st, offset[i] / dtype_size(in[i]->dtype));
     out[i]->dtype = in[i]->dtype;
-    held.ts.push_back(out[i]);
+    results.ts.push_back(out[i]);
   }
   std::vector<ClipTensor> ts;       // chunk0: the number of chunks, for now
   std::vector<int> first{0}, grid;  // launches: their first tensor, their blocks
@@ -284,17 +283,19 @@ int lc_clip_grad_norm(lc_tensor* outs, lc_tensor* norm_out, const lc_tensor* gra
     chunks += c;
   }
   close();
-  double* parts = (double*)dmalloc((size_t)nparts * 8);
-  held.mem.push_back(parts);
+  // the norm, and after it the partials
+  LcTensor* room = alloc(LC_F32, {2 + 2 * nparts});
+  held.ts.push_back(room);
+  LcTensor* norm = view_of(room, {}, {}, 0);
+  results.ts.push_back(norm);
   float* np = (float*)norm->data();
+  double* parts = (double*)(np + 2);
   if (ts.size() <= 16) clip_launch<16>(ts, max_norm, np, parts, first, grid, stream());
   else if (ts.size() <= 128) clip_launch<128>(ts, max_norm, np, parts, first, grid, stream());
   else clip_launch<kMaxTensors>(ts, max_norm, np, parts, first, grid, stream());
   for (int i = 0; i < n; i++) outs[i] = handle(out[i]);
   *norm_out = handle(norm);
-  // handed to the caller: what was made after the dense copies, but for `all`
-  held.ts.erase(std::find(held.ts.begin(), held.ts.end(), norm));
-  held.ts.resize(held.ts.size() - n);
+  results.ts.clear();
   LC_API_END
 }
 

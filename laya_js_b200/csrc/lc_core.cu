@@ -393,6 +393,7 @@ struct DLManagedTensor {
 struct DlpackTensor {
   DLManagedTensor managed{};  // first: the deleter gets its address
   int64_t shape[LC_MAX_DIMS];
+  uint64_t storage;
 };
 }  // namespace
 
@@ -613,9 +614,12 @@ int lc_tensor_to_dlpack(lc_tensor h, uint64_t* managed) {
   for (int i = 0; i < t->ndim; i++) m->shape[i] = t->shape[i];
   m->managed.dl_tensor.shape = m->shape;
   m->managed.manager_ctx = t;
+  m->storage = t->st->id;
   m->managed.deleter = [](DLManagedTensor* d) {
-    release(static_cast<LcTensor*>(d->manager_ctx));  // (a tensor already gone with the library is not freed again)
-    delete reinterpret_cast<DlpackTensor*>(d);
+    auto* m = reinterpret_cast<DlpackTensor*>(d);
+    auto* t = static_cast<LcTensor*>(d->manager_ctx);
+    if (S().live.count(t) && t->st->id == m->storage) release(t);  // unless lc_destroy freed it
+    delete m;
   };
   *managed = reinterpret_cast<uint64_t>(&m->managed);
   LC_API_END

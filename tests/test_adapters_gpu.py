@@ -317,3 +317,67 @@ def test_refusals():
             A.adapter_linear(b, t["x"], t["w"], None, t["a"], t["bt"], t["scales"], plan)
         finally:
             _lib.call("lc_debug_set_alloc_cap", 0)
+
+
+def test_inner_values_beyond_f16():
+    """u past the largest f16 value (65504) is held in two parts; y is an
+    ordinary number."""
+    b = backend()
+    rng = np.random.default_rng(16)
+    for T in (4, 300):
+        x = np.abs(rng.standard_normal((T, 64))) + 0.5
+        h = {"x": mk("f16", x), "w": None, "bias": None, "a": mk("f16", np.full((1, 2, 64), 1200.0)), "bt": mk("f16", np.full((1, 2, 72), 2.0 ** -12)),
+             "scales": mk("f32", np.array([1.0])), "dy": mk("f16", rng.standard_normal((T, 72)))}
+        u = vals(h["x"]) @ vals(h["a"])[0].T
+        assert u.min() > 65504 and u.max() < 131008
+        t = _up(b, h)
+        cu, ad = np.array([0, T], np.int32), np.array([0], np.int32)
+        y = vals(b.read(A.adapter_linear(b, t["x"], None, None, t["a"], t["bt"], t["scales"], A.AdapterPlan(b, cu, ad, 1))))
+        want, bound = linear_ref(h, cu, ad, "f16")
+        _check(y, want, bound, "y")
+
+
+@pytest.mark.parametrize("T,K,N", [(600001, 8, 1), (3, 8, 300001)])
+def test_long_and_wide(T, K, N):
+    """More groups of rows or columns than one grid axis of 65,535 holds."""
+    b = backend()
+    h, cu, ad = case("bf16", T, K, N, 2, 2, 3, seed=17)
+    t = _up(b, h)
+    plan = A.AdapterPlan(b, cu, ad, 2)
+    want, bound = linear_ref(h, cu, ad, "bf16")
+    _check(vals(b.read(A.adapter_linear(b, t["x"], t["w"], None, t["a"], t["bt"], t["scales"], plan))), want, bound, "y")
+    want, bound = linear_ref(h, cu, ad, "bf16", grad=True)
+    for name, g, v, m in zip(("dx", "da", "db"), A.adapter_linear_grad(b, t["dy"], t["x"], t["w"], t["a"], t["bt"], t["scales"], plan), want, bound):
+        _check(vals(b.read(g)), v, m, name)
+
+
+def test_with_every_kernel_chained():
+    """LAYA_CUDA_PDL=1 chains the kernels of consecutive ops too: a stack of
+    projections and its gradients keep their bits."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys; sys.path[:0] = ["tests", "."]
+import numpy as np
+from adapters_ref import case
+from laya_js_b200 import createCudaBackend, adapters as A
+b = createCudaBackend(0)
+out = []
+for T, req in ((24, 24), (900, 7)):
+    h, cu, ad = case("bf16", T, 256, 256, 3, 16, req, seed=T)
+    t = {k: None if v is None else b.fromHost(v) for k, v in h.items()}
+    plan = A.AdapterPlan(b, cu, ad, 3)
+    x = t["x"]
+    for _ in range(6):
+        y = A.adapter_linear(b, x, t["w"], None, t["a"], t["bt"], t["scales"], plan)
+        gs = A.adapter_linear_grad(b, y, x, t["w"], t["a"], t["bt"], t["scales"], plan)
+        c, n = A.clip_grad_norm(b, gs[1:], 1.0)
+        x = b.add(b.scale(y, 0.5), gs[0])
+    out += [b.read(v).data.astype(np.float64).ravel() for v in (x, y, *c, n)]
+b.flush()
+sys.stdout.buffer.write(np.concatenate(out).tobytes())
+"""
+    got = [subprocess.run([sys.executable, "-c", code], env={**os.environ, "LAYA_CUDA_PDL": v}, capture_output=True, check=True, timeout=120).stdout
+           for v in ("0", "1")]
+    assert len(got[0]) > 0 and got[0] == got[1]
