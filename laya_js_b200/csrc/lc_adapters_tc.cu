@@ -23,7 +23,8 @@ using namespace lc;
 
 constexpr int TC_THREADS = 192;  // TMA producer, MMA issuer, four epilogue warps
 constexpr int BM = 128, BK = 64;
-constexpr uint32_t X_BYTES = BM * BK * 2;
+constexpr int SK = 128;                       // columns per stage of the shrink
+constexpr uint32_t X_BYTES = BM * SK * 2;
 
 template <typename T>
 __device__ __forceinline__ uint32_t idesc_rt(int n, bool a_mn, bool b_mn) {
@@ -52,22 +53,25 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 // ------------------------------------------------------------- shrink
 //
 // One CTA takes tiles of 128 rows of one or two products (both directions of a
-// gradient share a launch). Per 64-column block of X the ring holds the X block
-// (TMA, 16 KB) and, for up to `nb` of the tile's segments, their blocks of P_a
+// gradient share a launch). Per 128 columns of X the ring holds the X block
+// (TMA, 32 KB) and, for up to `nb` of the tile's segments, their blocks of P_a
 // (R rows each), side by side: one MMA per 16 columns gives every row against
 // every one of these adapters, D [128, n·R] (n·R <= 256), and the epilogue
 // takes from each row's n results the one of its own adapter, scales, splits
 // and stores it. The tensor cores have room for the others: an MMA this narrow
-// costs the reading of X, not its width, and one MMA per segment with the other
-// rows switched off took 131 us where this takes the time below. More segments
-// than nb: the tile's columns are streamed again. D is double-buffered in TMEM.
+// costs the reading of X, not its width; one MMA per segment with the other
+// rows switched off took 131 us for what takes 79. More segments than nb: the
+// tile's columns are streamed again. D is double-buffered in TMEM.
 //
-// Bound by the read of X. With few tiles the columns are split over clusters
-// of S CTAs, whose partial D meet in shared memory and are added in rank order.
+// Bound by the read of X: 69,135 rows of 2304 and of 768 columns in f16 (424 MB),
+// rank 16, take 77 us with one request and 79 with 256 (5.4 TB/s, 0.83 of the
+// measured copy); stages of 64 columns instead of 128 took 79 and 85. With few
+// tiles the columns are split over clusters of S CTAs, whose partial D meet in
+// shared memory and are added in rank order.
 struct ShrinkJob {
   CUtensorMap tmX, tmP;
   void* Q;
-  int C;
+  int C, blocks;  // blocks: tmX brings both 64-column blocks of a stage (a 3-D map)
 };
 struct ShrinkArgs {
   ShrinkJob job[2];  // the longer one first
@@ -156,18 +160,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
       uint32_t used = 0, last_phase = 0;  // stages filled, and the phase bit of each one's last fill
       for (ShrinkItems it(args, first, step); ok && it.next();) {
         const ShrinkJob& job = args.job[it.job];
-        const int KB = (job.C + BK - 1) / BK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
+        const int KB = (job.C + SK - 1) / SK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
         for (int s = 0; s < it.segs.y && ok; s += args.nb) {
           const int n = min(args.nb, it.segs.y - s);
           for (int kb = kb0; kb < kb1; kb++) {
             if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
             uint8_t* st = smem + stage * stage_bytes;
-            mbar_arrive_expect_tx(&full[stage], X_BYTES + (uint32_t)n * args.R * 128);
-            tma_load_2d(st, &job.tmX, &full[stage], kb * BK, it.t * BM);
+            mbar_arrive_expect_tx(&full[stage], X_BYTES + (uint32_t)n * args.R * 256);
+            if (job.blocks) {
+              tma_load_3d(st, &job.tmX, &full[stage], 0, it.t * BM, kb * 2);
+            } else {
+              tma_load_2d(st, &job.tmX, &full[stage], kb * SK, it.t * BM);
+              tma_load_2d(st + X_BYTES / 2, &job.tmX, &full[stage], kb * SK + 64, it.t * BM);
+            }
             // (a rolled loop: unrolled over the possible eight with the loads predicated, the kernel took 103 us instead of 83)
 #pragma unroll 1
-            for (int i = 0; i < n; i++)
-              tma_load_3d(st + X_BYTES + i * args.R * 128, &job.tmP, &full[stage], kb * BK, 0, __ldg(&args.segs[it.segs.x + s + i].z));
+            for (int i = 0; i < n; i++) {
+              const int a = __ldg(&args.segs[it.segs.x + s + i].z);
+              tma_load_3d(st + X_BYTES + i * args.R * 128, &job.tmP, &full[stage], kb * SK, 0, a);
+              tma_load_3d(st + X_BYTES + args.bank_bytes / 2 + i * args.R * 128, &job.tmP, &full[stage], kb * SK + 64, 0, a);
+            }
             used |= 1u << stage;
             last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
             if (++stage == args.stages) { stage = 0; phase ^= 1; }
@@ -189,7 +201,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
       uint32_t last_phase = 0;
       for (ShrinkItems it(args, first, step); ok && it.next();) {
         const ShrinkJob& job = args.job[it.job];
-        const int KB = (job.C + BK - 1) / BK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
+        const int KB = (job.C + SK - 1) / SK, kb0 = (int)((int64_t)rank * KB / S), kb1 = (int)((int64_t)(rank + 1) * KB / S);
         for (int s = 0; s < it.segs.y && ok; s += args.nb) {
           const int n = min(args.nb, it.segs.y - s);
           const uint32_t idesc = idesc_rt<T>(n * args.R, false, false);
@@ -201,7 +213,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
             tc_fence_after();
             const uint32_t a0 = smem_u32(smem + stage * stage_bytes), b0 = a0 + X_BYTES;
 #pragma unroll
-            for (int k = 0; k < BK / 16; k++) tc_mma(d, sdesc_sw128(a0 + k * 32), sdesc_sw128(b0 + k * 32), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < SK / 16; k++)
+              tc_mma(d, sdesc_sw128(a0 + (k / 4) * (X_BYTES / 2) + (k % 4) * 32), sdesc_sw128(b0 + (k / 4) * (args.bank_bytes / 2) + (k % 4) * 32), idesc,
+                     (kb > kb0 || k > 0) ? 1u : 0u);
             tc_commit(&empty[stage]);
             last = &empty[stage];
             last_phase = phase;
@@ -579,8 +593,8 @@ void shrink_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStrea
   a.R = a.ucols / 2;
   // adapters side by side: 128 columns of D, 192 for rank 64 (a ragged tile of
   // 128 rows meets two or three requests), which leaves five stages or more
-  a.nb = a.R <= 32 ? 128 / a.R : a.R == 64 ? 3 : 1;
-  a.bank_bytes = (uint32_t)(a.nb * a.R * 128);
+  a.nb = a.R <= 32 ? 64 / a.R : a.R == 64 ? 2 : 1;
+  a.bank_bytes = (uint32_t)(a.nb * a.R * 256);
   a.tmem_cols = tmem_columns(2 * a.nb * a.R);
   a.segs = p.segs;
   a.tiles = p.tiles;
@@ -588,22 +602,23 @@ void shrink_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStrea
   int KB = INT32_MAX;
   for (int j = 0; j < njobs; j++) {
     const AdapterShrink& q = c[njobs == 2 && c[1].C > c[0].C ? 1 - j : j];
-    a.job[j].tmX = tensor_map_2d(q.X, p.rows, q.C, q.ld, BK, BM, dtype);
+    a.job[j].blocks = q.C % 64 == 0;
+    a.job[j].tmX = a.job[j].blocks ? tensor_map_blocks(q.X, p.rows, q.C, q.ld, 2, BM, dtype) : tensor_map_2d(q.X, p.rows, q.C, q.ld, BK, BM, dtype);
     a.job[j].tmP = tensor_map_3d(q.P, q.n, q.rank, q.C, q.ldp, a.R, dtype);
     a.job[j].Q = q.Q;
     a.job[j].C = (int)q.C;
-    KB = std::min(KB, (a.job[j].C + BK - 1) / BK);
+    KB = std::min(KB, (a.job[j].C + SK - 1) / SK);
   }
   const int64_t items = (int64_t)njobs * a.ntiles;
   a.S = 1;
   for (int f : {8, 4, 2})
-    if (a.R <= 64 && items * f <= num_sms() && KB >= 2 * f) {
+    if (a.R <= 64 && items * f <= num_sms() && KB >= f) {
       a.S = f;
       break;
     }
   const int ctas = (int)std::min<int64_t>(items, num_sms());
   if (njobs == 2 && a.S == 1 && a.ntiles % ctas) {
-    a.extra = ((a.job[0].C + BK - 1) / BK) / ((a.job[1].C + BK - 1) / BK);
+    a.extra = ((a.job[0].C + SK - 1) / SK) / ((a.job[1].C + SK - 1) / SK);
     a.filled = (int)std::min<int64_t>(a.ntiles, (int64_t)a.extra * (ctas - a.ntiles % ctas));
   }
   const size_t d_bytes = a.S > 1 ? (size_t)BM * a.R * 4 : 0;
