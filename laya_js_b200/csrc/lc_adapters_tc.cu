@@ -332,29 +332,49 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
 // those before the MMA reads them (a product with zero would let an inf or NaN
 // of that request through).
 //
-// The blocks of all adapters, in adapter order, are cut into G equal runs; a
-// CTA takes one run for one 256-column tile (and one group of 64 rank rows) of
-// one or two products. A run that holds all of an adapter's blocks stores dP;
-// otherwise it stores an f32 partial, in slot run + adapter (distinct for every
-// pair that occurs), counts itself in, and the last of the adapter's runs to
-// arrive adds all partials in the order of the runs: the same bits every time.
-// Bound by the read of X.
+// The work is the blocks of all adapters, in adapter order, once for every tile
+// (256 columns of one of the products and one group of 64 rank rows), tile
+// after tile; every CTA takes an equal run of it. The blocks of an adapter
+// that lie in one run are summed there and stored; of an adapter that several
+// runs share, each run stores an f32 partial (at most two to a run, one where
+// it begins and one where it ends), and k_outer_join adds them in the order of
+// the runs: the same bits every time. (One CTA adding them, the last to
+// arrive, took longer than the products: 150 us for one adapter of rank 64
+// over 24 runs.)
+//
+// Bound by the read of X: 69,135 rows of 2304 and of 768 columns in f16 (424
+// MB), rank 16, take 79 us with one request and 88 with 256 (5.4 and 4.8 TB/s);
+// 40,000 of 5248 and of 1024 in bf16, rank 32, 115 us. Equal runs: with a whole
+// number of runs per tile (125 of 148 SMs) that was 123.
 constexpr int OUTER_THREADS = TC_THREADS + 32;  // and the warp that clears rows
 constexpr int BC = 256;                         // columns of X per CTA
 constexpr uint32_t XC_BYTES = 64 * BC * 2;
 struct OuterJob {
   CUtensorMap tmX, tmQ, tmX16, tmQ16;  // boxes of 64 and of 16 rows
   int whole;                           // tmX brings this many 64-column blocks at once (a 3-D map); 0: one at a time
-  float* part;                         // [G + n, rank, C]
   void* dP;
   int C, ctiles;
 };
 struct OuterArgs {
   OuterJob job[2];
-  int rank, nchunks, n, G, ucols, rgroups, nmma, stages;
+  int rank, nchunks, ntiles, ucols, rgroups, nmma, stages;
   uint32_t q_bytes, tmem_cols;
   const int4* chunks;  // row0, rows, adapter
   const int32_t* chunk_ptr;
+  float* part;         // [runs, 2, nmma / 2, 256]
+};
+
+struct OuterTile {
+  int job, c0, j0;       // product, first column, first rank row
+  int xblocks, halves;   // 64-column blocks of X, accumulators of 128 columns
+  __device__ OuterTile(const OuterArgs& args, int t) {
+    const int ct = t / args.rgroups;
+    job = ct >= args.job[0].ctiles;
+    c0 = (job ? ct - args.job[0].ctiles : ct) * BC;
+    j0 = (t % args.rgroups) * 64;
+    xblocks = min(BC / 64, (args.job[job].C - c0 + 63) / 64);
+    halves = xblocks > 2 ? 2 : 1;
+  }
 };
 
 template <typename T>
@@ -370,13 +390,8 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
   uint32_t* tmem_slot = (uint32_t*)(tempty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool second = (int)blockIdx.x >= args.job[0].ctiles;
-  const OuterJob& job = args.job[second];
-  const int ct = second ? (int)blockIdx.x - args.job[0].ctiles : (int)blockIdx.x;
-  const int c0 = ct * BC, g = blockIdx.y, j0 = blockIdx.z * 64;
-  const int lo = (int)((int64_t)g * args.nchunks / args.G), hi = (int)((int64_t)(g + 1) * args.nchunks / args.G);
-  const int xblocks = min(BC / 64, (job.C - c0 + 63) / 64), qblocks = (int)(args.q_bytes >> 13);  // 64 x 64 blocks of a stage
-  const int halves = xblocks > 2 ? 2 : 1;                                                         // accumulators of 128 columns
+  const int64_t total = (int64_t)args.ntiles * args.nchunks, lo = blockIdx.x * total / gridDim.x, hi = (blockIdx.x + 1) * total / gridDim.x;
+  const int qblocks = (int)(args.q_bytes >> 13);  // 64-column blocks of Q
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1), mbar_init(&cleared[s], 1);
     for (int a = 0; a < 2; a++) mbar_init(&tfull[a], 1), mbar_init(&tempty[a], 4);
@@ -396,10 +411,15 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0, used = 0, last_phase = 0;
-      int4 ahead = lo < hi ? __ldg(&args.chunks[lo]) : make_int4(0, 0, 0, 0);
-      for (int c = lo; c < hi; c++) {
+      OuterTile t(args, (int)(lo / args.nchunks));
+      int c = (int)(lo % args.nchunks);
+      int4 ahead = __ldg(&args.chunks[c]);
+      for (int64_t f = lo; f < hi; f++) {
         const int4 ch = ahead;
-        if (c + 1 < hi) ahead = __ldg(&args.chunks[c + 1]);
+        if (++c == args.nchunks) c = 0;
+        if (f + 1 < hi) ahead = __ldg(&args.chunks[c]);
+        const OuterJob& job = args.job[t.job];
+        const int c0 = t.c0, j0 = t.j0, xblocks = t.xblocks;
         if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_adapter_err)) break;
         uint8_t* st = smem + stage * stage_bytes;
         const int n16 = (ch.y + 15) >> 4;
@@ -424,6 +444,7 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
         used |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
         if (++stage == args.stages) { stage = 0; phase ^= 1; }
+        if (c == 0 && f + 1 < hi) t = OuterTile(args, (int)((f + 1) / args.nchunks));
       }
       for (int s = 0; s < args.stages; s++)
         if (used >> s & 1) {
@@ -439,8 +460,11 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
       bool ok = true;
       uint64_t* last = nullptr;
       uint32_t last_phase = 0;
-      for (int c = lo; c < hi && ok;) {
-        const int a = __ldg(&args.chunks[c].z), end = min(hi, __ldg(args.chunk_ptr + a + 1)), begin = c;
+      for (int64_t f = lo; f < hi && ok;) {  // the pieces of the run: blocks of one adapter for one tile
+        const int halves = OuterTile(args, (int)(f / args.nchunks)).halves;
+        int c = (int)(f % args.nchunks);
+        const int a = __ldg(&args.chunks[c].z), begin = c, end = (int)min(c + hi - f, (int64_t)__ldg(args.chunk_ptr + a + 1));
+        f += end - begin;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_adapter_err)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * 2 * args.nmma);
@@ -477,8 +501,10 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
     // block, so that it is never a whole turn of the ring ahead or behind
     int stage = 0;
     uint32_t phase = 0;
-    for (int c = lo; c < hi; c++) {
-      const int rows = __ldg(&args.chunks[c].y);
+    OuterTile t(args, (int)(lo / args.nchunks));
+    int c = (int)(lo % args.nchunks);
+    for (int64_t f = lo; f < hi; f++) {
+      const int rows = __ldg(&args.chunks[c].y), xblocks = t.xblocks;
       if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort, &g_adapter_err))) break;
       if (rows & 15) {
         uint8_t* st = smem + stage * stage_bytes + rows * 128;
@@ -492,18 +518,28 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&cleared[stage]);
       if (++stage == args.stages) { stage = 0; phase ^= 1; }
+      if (++c == args.nchunks) {
+        c = 0;
+        if (f + 1 < hi) t = OuterTile(args, (int)((f + 1) / args.nchunks));
+      }
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, col0 = c0 + quarter * 32 + lane;  // and col0 + 128
-    const int nh = args.nmma / 2;  // rank rows of this CTA, rounded up
-    const int64_t size = (int64_t)args.rank * job.C;
-    T* dP = (T*)job.dP;
+    const int quarter = warp & 3;
+    const int nh = args.nmma / 2;  // rank rows of a tile, rounded up
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int c = lo; c < hi;) {
+    for (int64_t f = lo; f < hi;) {
+      const int tt = (int)(f / args.nchunks), c = (int)(f % args.nchunks);
+      const OuterTile t(args, tt);
+      const OuterJob& job = args.job[t.job];
+      const int64_t tile0 = (int64_t)tt * args.nchunks, size = (int64_t)args.rank * job.C;
       const int a = __ldg(&args.chunks[c].z), p0 = __ldg(args.chunk_ptr + a), p1 = __ldg(args.chunk_ptr + a + 1);
-      const bool whole = p0 >= lo && p1 <= hi;
+      const bool whole = tile0 + p0 >= lo && tile0 + p1 <= hi;
+      float* part = args.part + (int64_t)(2 * blockIdx.x + (f == lo ? 0 : 1)) * nh * BC + quarter * 32 + lane;
+      const int col0 = t.c0 + quarter * 32 + lane, j0 = t.j0, halves = t.halves;
+      T* dP = (T*)job.dP;
+      f = min(hi, tile0 + p1);
       if (!mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err)) break;
       tc_fence_after();
       for (int h = 0; h < halves; h++) {
@@ -520,7 +556,7 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
             if (row < args.rank && col < job.C) {
               const float v = __uint_as_float(vh[i]) + __uint_as_float(vl[i]);
               if (whole) dP[a * size + (int64_t)row * job.C + col] = TcFmt<T>::cvt(v);
-              else job.part[(g + a) * size + (int64_t)row * job.C + col] = v;
+              else part[(j + i) * BC + 128 * h] = v;
             }
           }
         }
@@ -529,7 +565,6 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
-      c = min(hi, p1);
     }
   }
   if (threadIdx.x == 0 && *abort) {
@@ -545,33 +580,40 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
 }
 
 // dP of the adapters that several runs share (the sum of their partials) and of those without rows (zeros).
+constexpr int kMaxRuns = 256;
 struct JoinArgs {
-  const float* part[2];
+  const float* part;
   void* dP[2];
-  int64_t size[2];   // rank · C
-  int nshared, nempty;
+  int C[2], ctiles0, njobs;
+  int rank, rgroups, nh, nshared, nempty;
   const int32_t* empty;
-  int3 shared[63];   // adapter, first and last run
+  int4 shared[kMaxRuns - 1];  // tile, adapter, slot of the first partial, number of partials: at most one per boundary
 };
+// grid: (rank rows of a group, shared adapters and then empty ones)
 template <typename T>
-__global__ void __launch_bounds__(256) k_outer_join(const __grid_constant__ JoinArgs args) {
+__global__ void __launch_bounds__(BC) k_outer_join(const __grid_constant__ JoinArgs args) {
   pdl_wait();
   pdl_trigger();
-  const int j = blockIdx.z;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, size = args.size[j];
-  if (i >= size) return;
-  T* dP = (T*)args.dP[j] + i;
   for (int e = blockIdx.y; e < args.nshared + args.nempty; e += gridDim.y) {
     if (e >= args.nshared) {
-      dP[__ldg(args.empty + e - args.nshared) * size] = from_f<T>(0.f);
+      const int64_t a = __ldg(args.empty + e - args.nshared);
+      for (int j = 0; j < args.njobs; j++)
+        for (int row = blockIdx.x; row < args.rank; row += gridDim.x)
+          for (int col = threadIdx.x; col < args.C[j]; col += BC) ((T*)args.dP[j])[(a * args.rank + row) * args.C[j] + col] = from_f<T>(0.f);
       continue;
     }
-    const int3 s = args.shared[e];
-    const float* p = args.part[j] + (int64_t)(s.y + s.x) * size + i;
-    float v = 0.f;
+    const int4 s = args.shared[e];
+    const int ct = s.x / args.rgroups, j = ct >= args.ctiles0;
+    const int col = (j ? ct - args.ctiles0 : ct) * BC + threadIdx.x, row = (s.x % args.rgroups) * 64 + blockIdx.x;
+    const int64_t size = (int64_t)args.rank * args.C[j], at = (int64_t)row * args.C[j] + col;
+    if (row >= args.rank || col >= args.C[j]) continue;
+    // the first partial, and the one each of the next runs begins with
+    const int64_t slot = (int64_t)args.nh * BC;
+    float v = args.part[s.z * slot + blockIdx.x * BC + threadIdx.x];
+    const float* p = args.part + (s.z / 2 + 1) * 2 * slot + blockIdx.x * BC + threadIdx.x;
 #pragma unroll 8
-    for (int g = s.y; g <= s.z; g++, p += size) v += *p;
-    dP[(int64_t)s.x * size] = from_f<T>(v);
+    for (int i = 1; i < s.w; i++, p += 2 * slot) v += *p;
+    ((T*)args.dP[j])[s.y * size + at] = from_f<T>(v);
   }
 }
 
@@ -648,15 +690,16 @@ void shrink_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStrea
   LC_LAUNCHED(1);
 }
 
-constexpr int kMaxRuns = 64;  // JoinArgs::shared holds a boundary each
-// Runs of blocks per tile of columns: as many as one wave of CTAs takes. (Two
-// waves, where one leaves SMs idle, gained nothing: 503 us against 500 for the
-// gradients of 40,000 x 1024 -> 5248 in bf16, 125 CTAs against 275.)
-int adapter_runs(const AdapterOuter* c, int njobs, const AdapterPlan& p) {
-  int64_t tiles = 0;
-  for (int j = 0; j < njobs; j++) tiles += (c[j].C + BC - 1) / BC * std::max(1, adapter_u_cols(c[j].rank) / 128);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxRuns, p.nchunks), num_sms() / tiles));
-}
+// The runs of an outer product's work: one per SM.
+struct OuterRuns {
+  int ntiles = 0, runs = 0;
+  int64_t total = 0;
+  OuterRuns(const AdapterOuter* c, int njobs, const AdapterPlan& p) {
+    for (int j = 0; j < njobs; j++) ntiles += (int)((c[j].C + BC - 1) / BC) * std::max(1, adapter_u_cols(c[j].rank) / 128);
+    total = (int64_t)ntiles * p.nchunks;
+    runs = (int)std::min<int64_t>(std::min(num_sms(), kMaxRuns), total);
+  }
+};
 
 template <typename T>
 void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p, cudaStream_t st) {
@@ -664,7 +707,6 @@ void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p
   OuterArgs a{};
   a.rank = c[0].rank;
   a.nchunks = p.nchunks;
-  a.n = p.n_adapters;
   a.ucols = adapter_u_cols(a.rank);
   a.rgroups = std::max(1, a.ucols / 128);
   a.nmma = std::min(a.ucols, 128);
@@ -673,13 +715,13 @@ void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p
   a.tmem_cols = tmem_columns(4 * a.nmma);
   a.chunks = p.chunks;
   a.chunk_ptr = p.chunk_ptr;
-  a.G = adapter_runs(c, njobs, p);
-  int ctiles = 0;
+  const OuterRuns runs(c, njobs, p);
+  a.ntiles = runs.ntiles;
+  a.part = part;
   for (int j = 0; j < njobs; j++) {
     OuterJob& o = a.job[j];
     o.C = (int)c[j].C;
     o.ctiles = (o.C + BC - 1) / BC;
-    ctiles += o.ctiles;
     // columns as blocks of 64, when they are: one load brings the blocks of a CTA, each 64 rows of 128 bytes
     o.whole = c[j].C % 64 == 0 ? (int)std::min<int64_t>(BC, c[j].C) / 64 : 0;
     o.tmX = o.whole ? tensor_map_blocks(c[j].X, p.rows, c[j].C, c[j].ld, o.whole, 64, dtype)
@@ -688,8 +730,6 @@ void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p
     o.tmX16 = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 16, dtype);
     o.tmQ16 = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 16, dtype);
     o.dP = c[j].dP;
-    o.part = part;
-    part += (a.G + p.n_adapters) * (int64_t)a.rank * c[j].C;
   }
   const size_t smem = (size_t)a.stages * (XC_BYTES + a.q_bytes) + 1024 + 512;
   static bool attr = false;
@@ -697,29 +737,36 @@ void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p
     CUDA_OK(cudaFuncSetAttribute(k_outer_tc<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 << 10));
     attr = true;
   }
-  launch_chain(k_outer_tc<T>, dim3((unsigned)ctiles, (unsigned)a.G, (unsigned)a.rgroups), dim3(OUTER_THREADS), smem, st, a);
+  launch_chain(k_outer_tc<T>, dim3((unsigned)runs.runs), dim3(OUTER_THREADS), smem, st, a);
   LC_LAUNCHED(1);
-  // the adapters that several runs share: at most one per boundary between runs
   JoinArgs join{};
-  int& shared = join.nshared;
-  for (int g = 1; g < a.G; g++) {
-    const int at = (int)((int64_t)g * a.nchunks / a.G);  // the first block of run g
+  for (int i = 1; i < runs.runs; i++) {
+    const int64_t f = i * runs.total / runs.runs;  // where run i begins
+    const int tile = (int)(f / p.nchunks), at = (int)(f % p.nchunks);
     const int ad = (int)(std::upper_bound(p.host_chunk_ptr.begin(), p.host_chunk_ptr.end(), at) - p.host_chunk_ptr.begin()) - 1;
-    if (p.host_chunk_ptr[ad] == at) continue;  // an adapter begins here
-    if (shared && join.shared[shared - 1].x == ad) join.shared[shared - 1].z = g;
-    else join.shared[shared++] = make_int3(ad, g - 1, g);
+    if (p.host_chunk_ptr[ad] == at) continue;  // with an adapter
+    int4* last = join.nshared ? &join.shared[join.nshared - 1] : nullptr;
+    if (last && last->x == tile && last->y == ad) {
+      last->w++;
+    } else {  // run i - 1 ends with it, unless it is all of that run
+      const bool begins = (int64_t)tile * p.nchunks + p.host_chunk_ptr[ad] == (i - 1) * runs.total / runs.runs;
+      join.shared[join.nshared++] = make_int4(tile, ad, 2 * (i - 1) + (begins ? 0 : 1), 2);
+    }
   }
+  if (!join.nshared && !p.nempty) return;
   join.nempty = p.nempty;
   join.empty = p.empty;
-  if (!shared && !p.nempty) return;
-  int64_t most = 0;
+  join.rank = a.rank;
+  join.rgroups = a.rgroups;
+  join.njobs = njobs;
+  join.ctiles0 = a.job[0].ctiles;
+  join.nh = a.nmma / 2;
+  join.part = part;
   for (int j = 0; j < njobs; j++) {
-    join.part[j] = a.job[j].part;
     join.dP[j] = a.job[j].dP;
-    join.size[j] = (int64_t)a.rank * a.job[j].C;
-    most = std::max(most, join.size[j]);
+    join.C[j] = a.job[j].C;
   }
-  launch_chain(k_outer_join<T>, dim3((unsigned)((most + 255) / 256), (unsigned)std::min(shared + p.nempty, 65535), (unsigned)njobs), dim3(256), 0, st, join);
+  launch_chain(k_outer_join<T>, dim3((unsigned)std::min(a.rank, 64), (unsigned)std::min(join.nshared + p.nempty, 65535)), dim3(BC), 0, st, join);
   LC_LAUNCHED(1);
 }
 
@@ -733,10 +780,8 @@ void adapter_shrink_tc(const AdapterShrink* c, int njobs, const AdapterPlan& p, 
 }
 
 size_t adapter_part_bytes(const AdapterOuter* c, int njobs, const AdapterPlan& p) {
-  const int G = adapter_runs(c, njobs, p);
-  size_t n = 0;
-  for (int j = 0; j < njobs; j++) n += G > 1 ? (size_t)(G + p.n_adapters) * c[j].rank * c[j].C * 4 : 0;
-  return n;
+  const OuterRuns runs(c, njobs, p);
+  return (size_t)runs.runs * 2 * (std::min(adapter_u_cols(c[0].rank), 128) / 2) * BC * 4;
 }
 
 void adapter_outer_tc(const AdapterOuter* c, int njobs, void* part, const AdapterPlan& p, int dtype, cudaStream_t st) {
