@@ -351,7 +351,7 @@ constexpr int BC = 256;                         // columns of X per CTA
 constexpr uint32_t XC_BYTES = 64 * BC * 2;
 struct OuterJob {
   CUtensorMap tmX, tmQ, tmX16, tmQ16;  // boxes of 64 and of 16 rows
-  int whole;                           // tmX brings this many 64-column blocks at once (a 3-D map); 0: one at a time
+  int whole;                           // the maps of X bring this many 64-column blocks at once (3-D maps); 0: one at a time
   void* dP;
   int C, ctiles;
 };
@@ -423,24 +423,23 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
         if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_adapter_err)) break;
         uint8_t* st = smem + stage * stage_bytes;
         const int n16 = (ch.y + 15) >> 4;
-        mbar_arrive_expect_tx(&full[stage], (uint32_t)(((job.whole && n16 == 4 ? job.whole : xblocks) + qblocks) * n16) * 2048);
-        auto bring = [&](uint8_t* dst, const CUtensorMap* big, const CUtensorMap* small, int x) {
-          if (n16 == 4) {
-            tma_load_2d(dst, big, &full[stage], x, ch.x);
+        mbar_arrive_expect_tx(&full[stage], (uint32_t)(((job.whole ? job.whole : xblocks) + qblocks) * n16) * 2048);
+        // X: whole blocks of 64 x 64 one after the other; where the rows end
+        // earlier, 16 rows of all columns after 16 rows
+        const int groups = n16 == 4 ? 1 : n16, high = n16 == 4 ? 8192 : 2048;
+        const CUtensorMap *mx = n16 == 4 ? &job.tmX : &job.tmX16, *mq = n16 == 4 ? &job.tmQ : &job.tmQ16;
+#pragma unroll 1
+        for (int i = 0; i < groups; i++) {
+          if (job.whole) {
+            tma_load_3d(st + i * 8192, mx, &full[stage], 0, ch.x + 16 * i, c0 / 64);
           } else {
 #pragma unroll 1
-            for (int i = 0; i < n16; i++) tma_load_2d(dst + i * 2048, small, &full[stage], x, ch.x + 16 * i);
+            for (int b = 0; b < xblocks; b++) tma_load_2d(st + i * 8192 + b * high, mx, &full[stage], c0 + 64 * b, ch.x + 16 * i);
           }
-        };
-        if (job.whole && n16 == 4) {
-          tma_load_3d(st, &job.tmX, &full[stage], 0, ch.x, c0 / 64);
-        } else {
-          const CUtensorMap* big = job.whole ? nullptr : &job.tmX;
 #pragma unroll 1
-          for (int b = 0; b < xblocks; b++) bring(st + b * 8192, big, &job.tmX16, c0 + 64 * b);
+          for (int b = 0; b < qblocks; b++)
+            tma_load_2d(st + XC_BYTES + b * 8192 + i * 2048, mq, &full[stage], b * (args.ucols / 2) + j0, ch.x + 16 * i);
         }
-#pragma unroll 1
-        for (int b = 0; b < qblocks; b++) bring(st + XC_BYTES + b * 8192, &job.tmQ, &job.tmQ16, b * (args.ucols / 2) + j0);
         used |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
         if (++stage == args.stages) { stage = 0; phase ^= 1; }
@@ -475,10 +474,11 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + stage * stage_bytes), b0 = a0 + XC_BYTES;
           // (a last block of 64 columns or less: the other half of the accumulator's rows reads a stale block and is not stored)
+          const uint32_t high = steps == 4 ? 8192 : 2048, step = steps == 4 ? 2048 : 8192;
           for (int k = 0; k < steps; k++) {
             const uint64_t q = sdesc_sw128_mn(b0 + k * 2048, 8192);
-            tc_mma(d, sdesc_sw128_mn(a0 + k * 2048, 8192), q, idesc, (c > begin || k > 0) ? 1u : 0u);
-            if (halves == 2) tc_mma(d + args.nmma, sdesc_sw128_mn(a0 + 16384 + k * 2048, 8192), q, idesc, (c > begin || k > 0) ? 1u : 0u);
+            tc_mma(d, sdesc_sw128_mn(a0 + k * step, high), q, idesc, (c > begin || k > 0) ? 1u : 0u);
+            if (halves == 2) tc_mma(d + args.nmma, sdesc_sw128_mn(a0 + 2 * high + k * step, high), q, idesc, (c > begin || k > 0) ? 1u : 0u);
           }
           tc_commit(&empty[stage]);
           last = &empty[stage];
@@ -507,10 +507,11 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
       const int rows = __ldg(&args.chunks[c].y), xblocks = t.xblocks;
       if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort, &g_adapter_err))) break;
       if (rows & 15) {
-        uint8_t* st = smem + stage * stage_bytes + rows * 128;
+        uint8_t* st = smem + stage * stage_bytes;
         const int zn = (16 - (rows & 15)) * 8;  // 16-byte pieces per 64-column block
+        const int first = rows > 48 ? rows * 128 : (rows >> 4) * 8192 + (rows & 15) * 128, high = rows > 48 ? 8192 : 2048;
         for (int k = 0; k < xblocks + qblocks; k++) {
-          uint8_t* z = st + (k < xblocks ? k * 8192 : XC_BYTES + (k - xblocks) * 8192);
+          uint8_t* z = k < xblocks ? st + first + k * high : st + XC_BYTES + (k - xblocks) * 8192 + rows * 128;
           for (int i = lane; i < zn; i += 32) *(uint4*)(z + i * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -727,7 +728,8 @@ void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p
     o.tmX = o.whole ? tensor_map_blocks(c[j].X, p.rows, c[j].C, c[j].ld, o.whole, 64, dtype)
                     : tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 64, dtype);
     o.tmQ = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 64, dtype);
-    o.tmX16 = tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 16, dtype);
+    o.tmX16 = o.whole ? tensor_map_blocks(c[j].X, p.rows, c[j].C, c[j].ld, o.whole, 16, dtype)
+                      : tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 16, dtype);
     o.tmQ16 = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 16, dtype);
     o.dP = c[j].dP;
   }
