@@ -67,7 +67,11 @@ struct GemmPlain {
 // leaves the rows outside the segment alone (TMEM lanes switched off), so a
 // row never meets another request's adapter, not even multiplied by zero.
 // U holds each value as a 16-bit high part and the 16-bit remainder, which
-// meet the same rows of P_a: the sum is as exact as an f32 u.
+// meet the same rows of P_a: the sum is as exact as an f32 u, for another two
+// MMA steps per request (rank 16) where one tile of 768 columns in takes 48.
+// Bound by the projection: 69,135 rows, 768 -> 2304 in f16 take 197 us without
+// adapters, 207 with those of 256 requests (U given); adding the share in a
+// kernel of its own would read and write y (318 MB) once more, ~95 us.
 // WT: the shared projection is read transposed, D = X·W for W [K, N] (the
 // gradient with respect to the input): an MN-major B operand as well.
 template <bool WT>
@@ -898,13 +902,12 @@ __device__ __forceinline__ void epilogue_split(const GemmArgs& args, const CUten
 // conv[stage], which the MMA issuer waits for as well. The packed weight is
 // resident, so its first blocks are requested and converted before the
 // dependency wait. One unit of work per CTA.
-// EX: what is accumulated after the main loop (GemmPlain, GemmAdapted); with
-// split K the last slice takes it.
+// EX: what is accumulated after the main loop (GemmPlain, GemmAdapted).
 template <typename T, int BN, int STAGES, bool TMAE, bool KS = false, bool QB = false, typename EX = GemmPlain>
 __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                                                     const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmR,
                                                     const __grid_constant__ GemmArgs args, const __grid_constant__ EX ex) {
-  static_assert(!(EX::kOn && QB), "adapters beside a packed weight are added to a separate product");
+  static_assert(!(EX::kOn && (KS || QB)), "adapters run beside whole products of dense weights");
   static_assert(!KS || TMAE, "split K runs with the TMA-store epilogue");
   extern __shared__ uint8_t smem_raw[];
   constexpr uint32_t A_BYTES = BM * BK * 2;
@@ -1057,7 +1060,6 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
         if constexpr (EX::kOn) {
-          if (kb1 < KB) continue;  // another slice of K takes the adapters
           if (ex.defer) pdl_wait();  // the kernel that wrote U
           const int2 sg = tile_segments(ex, m0, BM, args.M);
           for (int s = sg.x; s < sg.y && ok; s += ex.per)
@@ -1106,8 +1108,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
       for (int w = blockIdx.x; w < args.ntiles * S && ok; w += gridDim.x) {
         const int kb0 = (w % S) * KB / S, kb1 = (w % S + 1) * KB / S;
         [[maybe_unused]] int2 sg = make_int2(0, 0);
-        if constexpr (EX::kOn)
-          if (kb1 == KB) sg = tile_segments(ex, ((w / S) / args.ntile_n) * BM, BM, args.M);  // in flight during the main loop
+        if constexpr (EX::kOn) sg = tile_segments(ex, (w / args.ntile_n) * BM, BM, args.M);  // in flight during the main loop
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * BN);
@@ -1128,7 +1129,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
         if constexpr (EX::kOn) {
-          const int m0 = ((w / S) / args.ntile_n) * BM;
+          const int m0 = (w / args.ntile_n) * BM;
           for (int s = sg.x; s < sg.y && ok; s += ex.per)
             for (int c = 0; c < ex.nchunks; c++) {
               const int n = min(ex.per, sg.y - s);
@@ -1603,13 +1604,13 @@ void launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap
 
 // Split K: clusters of a.ksplit CTAs, one cluster per tile while they fit
 // (QB: the packed-weight instance).
-template <typename T, int BN, int STAGES, bool QB = false, typename EX = GemmPlain>
+template <typename T, int BN, int STAGES, bool QB = false>
 cudaLaunchConfig_t split_config(int S, cudaLaunchAttribute* at, cudaStream_t st) {
   constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(true, true, QB);
   static_assert(smem <= 232448, "GEMM shared memory above the 227 KB per-CTA limit");
   static bool attr = false;
   if (!attr) {
-    CUDA_OK(cudaFuncSetAttribute(k_gemm_tc<T, BN, STAGES, true, true, QB, EX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CUDA_OK(cudaFuncSetAttribute(k_gemm_tc<T, BN, STAGES, true, true, QB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attr = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -1624,31 +1625,31 @@ cudaLaunchConfig_t split_config(int S, cudaLaunchAttribute* at, cudaStream_t st)
   return cfg;
 }
 // clusters of S of this instance that can be resident at once
-template <typename T, int BN, int STAGES, bool QB = false, typename EX = GemmPlain>
+template <typename T, int BN, int STAGES, bool QB = false>
 int split_capacity(int S) {
   static int cap[5] = {0, 0, 0, 0, 0};
   if (!cap[S]) {
     cudaLaunchAttribute at[2];
-    cudaLaunchConfig_t cfg = split_config<T, BN, STAGES, QB, EX>(S, at, nullptr);
+    cudaLaunchConfig_t cfg = split_config<T, BN, STAGES, QB>(S, at, nullptr);
     cfg.gridDim = dim3(S * (lc::num_sms() / S));
     int n = 0;
-    CUDA_OK(cudaOccupancyMaxActiveClusters(&n, k_gemm_tc<T, BN, STAGES, true, true, QB, EX>, &cfg));
+    CUDA_OK(cudaOccupancyMaxActiveClusters(&n, k_gemm_tc<T, BN, STAGES, true, true, QB>, &cfg));
     LC_CHECK(n > 0, "tcgen05 GEMM: no split-K cluster fits");
     cap[S] = n;
   }
   return cap[S];
 }
-template <typename T, int BN, int STAGES, bool QB = false, typename EX = GemmPlain>
+template <typename T, int BN, int STAGES, bool QB = false>
 void launch_gemm_split(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my, const CUtensorMap& mr, const GemmArgs& a,
-                       cudaStream_t st, const EX& ex = EX()) {
+                       cudaStream_t st) {
   const int S = a.ksplit;
   LC_CHECK(S == 1 || S == 2 || S == 4, "tcgen05 GEMM: split-K factor must be 1, 2 or 4");
   cudaLaunchAttribute at[2];
-  cudaLaunchConfig_t cfg = split_config<T, BN, STAGES, QB, EX>(S, at, st);
-  const int cap = split_capacity<T, BN, STAGES, QB, EX>(S);
+  cudaLaunchConfig_t cfg = split_config<T, BN, STAGES, QB>(S, at, st);
+  const int cap = split_capacity<T, BN, STAGES, QB>(S);
   LC_CHECK((S == 1 && !QB) || a.ntiles <= cap, "tcgen05 GEMM: split K needs one resident cluster per tile");
   cfg.gridDim = dim3(S * std::min(a.ntiles, cap));
-  CUDA_OK(cudaLaunchKernelEx(&cfg, k_gemm_tc<T, BN, STAGES, true, true, QB, EX>, ma, mb, my, mr, a, ex));
+  CUDA_OK(cudaLaunchKernelEx(&cfg, k_gemm_tc<T, BN, STAGES, true, true, QB>, ma, mb, my, mr, a, GemmPlain{}));
 }
 int split_capacity_for(int dtype, int BN, int S, bool qb = false) {
   if (qb) {
@@ -1864,25 +1865,19 @@ void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
   const int sms = num_sms();
   const int64_t mt = (c.M + BM - 1) / BM;
   auto tiles = [&](int bn) { return mt * ((c.N + bn - 1) / bn); };
-  LC_CHECK(tiles(64) <= INT32_MAX, "adapters: too many output tiles");
+  LC_CHECK(tiles(128) <= INT32_MAX, "adapters: too many output tiles");
   auto shape = [&](int bn) {
     a.ntile_n = (int)((c.N + bn - 1) / bn);
     a.ntiles = (int)tiles(bn);
   };
-  if (tmae && (c.N <= 64 || tiles(128) * 2 <= sms)) {
-    // few columns or few rows: narrow tiles, K split over clusters (as in gemm_raw)
-    const int KB = (a.K + BK - 1) / BK;
-    int S = 1;
-    for (int f : {4, 2})
-      if (tiles(64) * f <= sms && KB >= f && tiles(64) <= split_capacity<T, 64, 4, false, GemmAdapted<WT>>(f)) {
-        S = f;
-        break;
-      }
-    shape(64);
-    a.ksplit = S;
-    const CUtensorMap my = tensor_map(c.y, c.M, c.N, c.ldy, 64, S > 1 ? 4 : 32, dtype);
-    launch_gemm_split<T, 64, 4, false, GemmAdapted<WT>>(ma, weight_map(64), my, my, a, st, ex);
-  } else if (tmae && c.N > 128 && tiles(256) >= sms) {
+  // CTA pairs on 256 x 256 tiles once 128 x 128 tiles would not fit one wave,
+  // and the columns fill more than a 128-wide tile. Measured (f16, 768 columns
+  // in, rank 16; single / pair, us): 2048 rows to 768 columns (96 tiles of 128)
+  // 9.3 / 11.6, 4096 rows (192) 14.6 / 13.0; 1024 rows to 2304 (144) 9.5 / 12.1,
+  // 2048 rows (288) 15.3 / 13.3, 16,384 rows 92 / 62. Narrower tiles with K
+  // split over a cluster, which gemm_raw takes for few rows, gained nothing at
+  // 128 rows and cost 5-9 us at 2048.
+  if (tmae && c.N > 128 && tiles(128) > sms) {
     shape(256);
     a.ntiles = (int)(((c.M + 2 * BM - 1) / (2 * BM)) * a.ntile_n);
     const CUtensorMap my = tensor_map(c.y, c.M, c.N, c.ldy, 64, 32, dtype);
