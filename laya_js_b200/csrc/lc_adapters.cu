@@ -341,10 +341,12 @@ struct Padder {
     work = std::max(work, rows * ld / 8);
     return {d, ld};
   }
-  void run() {
-    if (!jobs.n || !work) return;
+  // true when a kernel was launched: the next one may start while it runs, and waits for it
+  bool run() {
+    if (!jobs.n || !work) return false;
     launch_chain(k_pad_rows, dim3(blocks_for(work, 256)), dim3(256), 0, stream(), jobs);
     LC_LAUNCHED(1);
+    return true;
   }
 };
 
@@ -375,7 +377,8 @@ AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_
   return c;
 }
 
-void shrink(const AdapterShrink* c, int njobs, const Operands& o) {
+void shrink(const AdapterShrink* c, int njobs, const Operands& o, bool padded) {
+  std::unique_ptr<PdlScope> chained = padded ? std::make_unique<PdlScope>() : nullptr;
   if (!adapter_shrink_rows(c, njobs, *o.plan, o.dtype, stream())) adapter_shrink_tc(c, njobs, *o.plan, o.dtype, stream());
 }
 
@@ -418,9 +421,9 @@ void linear(const Operands& o, LcTensor* y, Held& held) {
   Padder pad{held};
   const Rows x = pad.of(o.x, o.T, o.K), w = pad.of(o.w, o.N, o.K), a = pad.of(o.a, (int64_t)o.n * o.r, o.K),
              b = pad.of(o.b, (int64_t)o.n * o.r, o.N);
-  pad.run();
+  const bool padded = pad.run();
   const AdapterShrink u = shrink_job(o, x, a, o.K, held.scratch(q_bytes(o)));
-  shrink(&u, 1, o);
+  shrink(&u, 1, o, padded);
   const Chained chained(o);
   expand_tc(o, x, w, b, u.Q, false, y);
 }
@@ -448,7 +451,7 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
   Padder pad{held};
   const Rows dy = pad.of(o.dy, o.T, o.N), x = da || db ? pad.of(o.x, o.T, o.K) : Rows{}, w = dx ? pad.of(o.w, o.N, o.K) : Rows{},
              a = dx || db ? pad.of(o.a, (int64_t)o.n * o.r, o.K) : Rows{}, b = dx || da ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : Rows{};
-  pad.run();
+  const bool padded = pad.run();
   AdapterOuter out[2];
   int no = 0;
   auto job = [&](const Rows& X, int64_t C, LcTensor* dP) -> AdapterOuter& {
@@ -474,7 +477,7 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
   }
   if (dx || da) q[nq - 1] = shrink_job(o, dy, b, o.N, Q);
   if (da) of_g->Q = Q;
-  shrink(q, nq, o);
+  shrink(q, nq, o, padded);
   const Chained chained(o);
   if (no) adapter_outer_tc(out, no, scratch + nq * q_bytes(o), *o.plan, o.dtype, stream());
   if (dx) expand_tc(o, dy, w, a, Q, true, dx);

@@ -18,6 +18,7 @@ from .host import CODE
 
 _NAMES = {"f32": "float32", "f16": "float16", "bf16": "bfloat16", "i32": "int32", "bool": "bool", "u8": "uint8", "i8": "int8",
           "i16": "int16", "i64": "int64", "f64": "float64"}
+_DTYPES: dict = {}  # torch dtype -> backend dtype, filled on first use
 _LEGACY_STREAM = 1  # cudaStreamLegacy: torch's default stream has handle 0, which lc_set_stream takes for the library's own
 
 
@@ -31,7 +32,10 @@ def useTorchStream(b) -> None:
 def fromTorch(b, t) -> CudaTensor:
     """A tensor over the memory of ``t`` (contiguous, on the backend's
     device), which stays alive as long as the result does."""
-    dtype = {v: k for k, v in _NAMES.items()}.get(str(t.dtype).replace("torch.", ""))
+    import torch
+    if not _DTYPES:
+        _DTYPES.update({getattr(torch, v): k for k, v in _NAMES.items()})
+    dtype = _DTYPES.get(t.dtype)
     if dtype is None:
         raise TypeError(f"fromTorch: no backend dtype for {t.dtype}")
     if t.device.type != "cuda" or (t.device.index or 0) != b.device:
@@ -40,7 +44,7 @@ def fromTorch(b, t) -> CudaTensor:
         raise ValueError("fromTorch: the tensor must be contiguous")
     out = C.c_uint64()
     _lib.call("lc_from_device", C.byref(out), CODE[dtype], _i64(t.shape), t.dim(), t.data_ptr())
-    r = b._wrap(out.value)
+    r = b._wrap(out.value, dtype, tuple(t.shape))
     r.keep = t
     return r
 
