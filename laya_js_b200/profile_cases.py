@@ -9,6 +9,7 @@ quick timing. Each case fits in a few GB and ends in seconds.
     python -m laya_js_b200.profile_cases prompt_q4 # the same with 4-bit affine g64 weights (fused-dequant GEMMs)
     python -m laya_js_b200.profile_cases sdpa      # the contract's sdpa on the padded configs[2] batch (full / sliding masks)
     python -m laya_js_b200.profile_cases predict   # DecisionModel forward, one 128-token prompt, eager and compiled
+    python -m laya_js_b200.profile_cases adapters  # adapters of 32 tenants beside Wqkv, 256 prompts: forward, gradients, clipping
 
 Every case prints one line with its shape and the device time per launch
 (CUDA events on the library stream, after warm-up).
@@ -198,6 +199,39 @@ def case_predict(b) -> str:
     return f"predict (DecisionModel, 1 x 128 tokens): eager {eager:.3f} ms, compiled {graph:.3f} ms"
 
 
+def case_adapters(b) -> str:
+    """Adapters (rank 16, 32 tenants) beside the Wqkv projection of 256 prompts, f16: forward, gradients and the
+    clipping of 44 bf16 gradient tensors of 32 tenants (69 MB)."""
+    from . import adapters as ad
+    rng = np.random.default_rng(0)
+    lens = WL.lengths(256, 32, 512, seed=2)
+    T, K, N, n, r = int(lens.sum()), 768, 2304, 32, 16
+    half = lambda std, *shape: b.fromHost(HostTensor("f16", shape, (rng.standard_normal(shape, dtype=np.float32) * std).astype(np.float16)))
+    x, w, dy, a, bt = half(1, T, K), half(0.02, N, K), half(0.05, T, N), half(K ** -0.5, n, r, K), half(0.02, n, r, N)
+    scales = b.fromHost(HostTensor("f32", (n,), np.ones(n, np.float32)))
+    plan = ad.AdapterPlan(b, np.concatenate([[0], np.cumsum(lens)]), rng.integers(-1, n, size=256), n)
+    grads = [b.fromHost(HostTensor("bf16", (n, r, K if i % 2 else N), rng.integers(0, 1 << 14, size=(n, r, K if i % 2 else N)).astype(np.uint16)))
+             for i in range(44)]
+
+    def forward():
+        b.dispose(ad.adapter_linear(b, x, w, None, a, bt, scales, plan))
+
+    def gradients():
+        for t in ad.adapter_linear_grad(b, dy, x, w, a, bt, scales, plan):
+            b.dispose(t)
+
+    def clip():
+        clipped, norm = ad.clip_grad_norm(b, grads, 1.0)
+        for t in (*clipped, norm):
+            b.dispose(t)
+    out = []
+    for name, run in (("forward", forward), ("gradients", gradients), ("clipping", clip)):
+        run()
+        out.append(f"{name} {_event_time(b, run, 20) * 1e3:.0f} us")
+    plan.free()
+    return f"adapters of {n} tenants, rank {r}, [{T},{K}] -> {N}: " + ", ".join(out)
+
+
 def _event_time(b, fn, reps: int) -> float:
     """Device ms per call: CUDA events on the library stream around `reps` calls."""
     import torch
@@ -219,7 +253,7 @@ def _event_time(b, fn, reps: int) -> float:
 def main(argv) -> None:
     b = createCudaBackend(0)
     cases = {"encoder": case_encoder, "gemm": case_gemm, "attention": case_attention, "hbm": case_hbm, "prompt": case_prompt,
-             "prompt_q4": case_prompt_q4, "sdpa": case_sdpa, "predict": case_predict}
+             "prompt_q4": case_prompt_q4, "sdpa": case_sdpa, "predict": case_predict, "adapters": case_adapters}
     for name in argv[1:] or list(cases):
         print(cases[name](b), flush=True)
 
