@@ -8,9 +8,10 @@
 //   outer   dP_a    = Σ_{t in a} Q[t] ⊗ X[t]       dA (Q = g, X = x), dB (Q = u, X = dy)
 //
 // f16 and bf16 run on the tensor cores (lc_adapters_tc.cu, gemm_adapted in
-// lc_gemm.cu), which read 16-byte aligned rows: operands with other widths or
-// addresses are copied into padded rows first. The kernels of this file serve
-// f32: one thread block per tile, f32 sums in registers, Q in f32.
+// lc_gemm.cu) or, with few rows, as dot products (lc_adapters_rows.cu). Both
+// read 16-byte aligned rows: operands with other widths or addresses are
+// copied into padded rows first. The kernels of this file serve f32: one
+// thread block per tile, f32 sums in registers, Q in f32.
 #include "lc_adapters.h"
 #include "lc_api.h"
 #include "lc_gemm.h"
@@ -61,7 +62,8 @@ void plan_release(AdapterPlan* p) {
 // ------------------------------------------------------------- f32
 
 // Q[t, j] = s_a · Σ_k X[t, k]·P[a, j, k]; rows without an adapter get zeros.
-// A block per row, a warp per rank row j.
+// A block per row, a warp per rank row j; bound by the reads of P from L2
+// (4096 rows of 768, rank 16: 21 us).
 __global__ void __launch_bounds__(128) k_shrink_f32(const float* __restrict__ X, const float* __restrict__ P, const float* __restrict__ scales,
                                                     const int2* __restrict__ tiles, const int4* __restrict__ segs, float* __restrict__ Q, int C,
                                                     int r) {
@@ -84,7 +86,9 @@ __global__ void __launch_bounds__(128) k_shrink_f32(const float* __restrict__ X,
 }
 
 // Y[m, n] = Σ_k X[m, k]·W(n, k) (+ bias[n]) + Σ_j Q[m, j]·P[a(m), j, n], with
-// W(n, k) = W[n·swn + k·swk]. 64 x 64 tiles, 4 x 4 outputs per thread.
+// W(n, k) = W[n·swn + k·swk]. 64 x 64 tiles, 4 x 4 outputs per thread; bound by
+// the FMA pipe and the shared-memory loads that feed it (4096 rows, 768 -> 768:
+// 217 us, 22 TFLOP/s; the contract's f32 linear takes 389).
 __global__ void __launch_bounds__(256) k_expand_f32(const float* __restrict__ X, const float* __restrict__ W, int64_t swn, int64_t swk,
                                                     const char* bias, int bias_dtype, const float* __restrict__ Q,
                                                     const float* __restrict__ P, const int2* __restrict__ tiles, const int4* __restrict__ segs,
@@ -146,34 +150,37 @@ __global__ void __launch_bounds__(256) k_expand_f32(const float* __restrict__ X,
 
 // dP[a, j, c] = Σ_{t in a} Q[t, j]·X[t, c]: a block per adapter, 8 rank rows
 // and 128 columns; rows in order, in groups of 64 so that a long sum loses no
-// more than a short one.
+// more than a short one. Bound by the latency of a block's rows, which follow
+// one another (4096 rows of 768, 8 adapters of rank 16: 66 us, eight rows'
+// loads at a time; one at a time 124).
 __global__ void __launch_bounds__(128) k_outer_f32(const float* __restrict__ Q, const float* __restrict__ X, const int2* __restrict__ spans,
                                                    const int32_t* __restrict__ span_ptr, float* __restrict__ dP, int C, int r) {
   pdl_trigger();
   pdl_wait();
-  const int a = blockIdx.z, j0 = blockIdx.y * 8, c = blockIdx.x * 128 + threadIdx.x;
+  const int a = blockIdx.z, j0 = blockIdx.y * 8, c = blockIdx.x * 128 + threadIdx.x, cc = min(c, C - 1);
   const int nj = min(8, r - j0);
-  float acc[8] = {}, part[8] = {};
-  int n = 0;
+  float acc[8] = {};
   for (int s = span_ptr[a]; s < span_ptr[a + 1]; s++) {
     const int2 rows = spans[s];
-    for (int t = rows.x; t < rows.y; t++) {
-      const float x = c < C ? X[(int64_t)t * C + c] : 0.f;
-      const float* q = Q + (int64_t)t * r + j0;
+    for (int64_t t0 = rows.x; t0 < rows.y; t0 += 64) {
+      const int64_t t1 = min(t0 + 64, (int64_t)rows.y);
+      float part[8] = {};
+#pragma unroll 8
+      for (int64_t t = t0; t < t1; t++) {
+        const float x = X[t * C + cc];
+        const float* q = Q + t * r + j0;
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (j < nj) part[j] = fmaf(q[j], x, part[j]);
-      if (++n == 64) {
-        n = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) acc[j] += part[j], part[j] = 0.f;
+        for (int j = 0; j < 8; j++)
+          if (j < nj) part[j] = fmaf(q[j], x, part[j]);
       }
+#pragma unroll
+      for (int j = 0; j < 8; j++) acc[j] += part[j];
     }
   }
   if (c < C)
 #pragma unroll
     for (int j = 0; j < 8; j++)
-      if (j < nj) dP[((int64_t)a * r + j0 + j) * C + c] = acc[j] + part[j];
+      if (j < nj) dP[((int64_t)a * r + j0 + j) * C + c] = acc[j];
 }
 
 // ------------------------------------------------------------- operands
@@ -301,7 +308,9 @@ struct Rows {
   int64_t ld = 0;
 };
 
-// Copies rows of `cols` values into rows of `ld` (a multiple of 8), zeros after them.
+// Copies rows of `cols` values into rows of `ld` (a multiple of 8), zeros after
+// them: up to five matrices a launch, eight values per thread step. Bound by
+// the 2-byte loads (1537 x 1001, 777 x 1001 and two banks: 4.4 us).
 struct PadJob {
   const uint16_t* src;
   uint16_t* dst;

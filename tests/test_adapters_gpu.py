@@ -381,3 +381,23 @@ sys.stdout.buffer.write(np.concatenate(out).tobytes())
     got = [subprocess.run([sys.executable, "-c", code], env={**os.environ, "LAYA_CUDA_PDL": v}, capture_output=True, check=True, timeout=120).stdout
            for v in ("0", "1")]
     assert len(got[0]) > 0 and got[0] == got[1]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("T", [20, 900])
+def test_rows_without_an_adapter_over_used_memory(dtype, T):
+    """The scratch of rows without an adapter is never written: with NaN left
+    in freed memory, nothing of it reaches a result."""
+    b = backend()
+    h, cu, ad = case(dtype, T, 256, 264, 3, 12, 11, seed=18, bare=0.6)
+    t = _up(b, h)
+    plan = A.AdapterPlan(b, cu, ad, 3)
+    want, bound = linear_ref(h, cu, ad, dtype)
+    wg, bg = linear_ref(h, cu, ad, dtype, grad=True)
+    for size in (256, 4096, 70000, 1 << 20, 5 << 20):  # what the ops are about to allocate comes from these
+        nan = np.full(size // 2, 0x7fff, np.uint16)
+        for junk in [b.fromHost(HostTensor("bf16", nan.shape, nan)) for _ in range(3)]:
+            b.dispose(junk)
+    _check(vals(b.read(A.adapter_linear(b, t["x"], t["w"], None, t["a"], t["bt"], t["scales"], plan))), want, bound, "y")
+    for name, g, v, m in zip(("dx", "da", "db"), A.adapter_linear_grad(b, t["dy"], t["x"], t["w"], t["a"], t["bt"], t["scales"], plan), wg, bg):
+        _check(vals(b.read(g)), v, m, name)
