@@ -207,16 +207,19 @@ void linear_rows_t(const GemmAdaptedCall& c, const AdapterPlan& p, cudaStream_t 
 
 namespace lc {
 
+// Requests of 16 rows or less on average cost the tensor-core forms a pass each.
+static int short_requests(const AdapterPlan& p) { return (int64_t)p.nsegs * 16 >= p.rows ? 2 : 1; }
+
 bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st) {
   int64_t C = 0;
   for (int j = 0; j < njobs; j++) C += c[j].ld;
-  if (!p.npieces || (int64_t)p.rows * (adapter_u_cols(c[0].rank) / 2) * C > kRowsShrinkMost) return false;
+  if (!p.npieces || (int64_t)p.rows * (adapter_u_cols(c[0].rank) / 2) * C > kRowsShrinkMost * short_requests(p)) return false;
   dtype == LC_F16 ? shrink_rows_t<__half>(c, njobs, p, st) : shrink_rows_t<__nv_bfloat16>(c, njobs, p, st);
   return true;
 }
 
 bool adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int dtype, cudaStream_t st) {
-  if (c.transposed || c.M * c.N * c.K > kRowsLinearMost) return false;
+  if (c.transposed || c.M * c.N * c.K > kRowsLinearMost * short_requests(p)) return false;
   dtype == LC_F16 ? linear_rows_t<__half>(c, p, st) : linear_rows_t<__nv_bfloat16>(c, p, st);
   return true;
 }

@@ -87,6 +87,10 @@ struct GemmAdapted {
   int prows;                  // rows of P_a per block (box height of tmP)
   int per;                    // segments whose blocks of P share a stage (64 / prows; 1 with several blocks of U)
   int defer;                  // x, w and bias were complete when the previous kernel let this one start: only U waits for it
+  // Single-CTA kernel: a tile's U (two blocks at most) stays in shared memory
+  // and stages hold blocks of P alone, 2·per requests to a stage: 500 rows in
+  // 250 requests, 768 -> 2304 in bf16, 77 -> 44 us at rank 40, 28 -> 25 at 16.
+  int resident;
   int kb_off;                 // added to the K block of the main loop's loads (past the operands' end: zeros)
 };
 
@@ -932,7 +936,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
   uint8_t* sPk = sB + STAGES * B_BYTES;
   uint8_t* sE = sPk + STAGES * PK_BYTES;  // epilogue staging (TMAE, or EX with rows TMA cannot store), 1024-aligned
   float* sP = (float*)(sE + (TMAE || EX::kOn ? STG_BYTES : 0));  // split-K partial tile (KS only)
-  uint64_t* full = (uint64_t*)((uint8_t*)sP + (KS ? part_bytes<BN>() : 0));
+  uint64_t* full = (uint64_t*)((uint8_t*)sP + (KS ? part_bytes<BN>() : 0) + (EX::kOn ? 2 * A_BYTES : 0));
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;
@@ -940,8 +944,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
   uint64_t* pbar = rbar + EPI_WARPS;  // KS: the partial slots of this CTA's rows have landed
   uint64_t* pfull = pbar + 1;                  // QB: packed block landed
   uint64_t* conv = pfull + (QB ? STAGES : 0);  // QB: 16-bit operand written
-  uint32_t* tmem_slot = (uint32_t*)(conv + (QB ? STAGES : 0));
+  uint64_t* ufull = conv + (QB ? STAGES : 0);  // EX: U of the tile's rows has landed
+  uint64_t* ufree = ufull + 1;                 // EX: it has been multiplied
+  uint32_t* tmem_slot = (uint32_t*)(ufree + 1);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
+  uint8_t* sU = sE + STG_BYTES;  // EX: two blocks of U
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int KB = (args.K + BK - 1) / BK;
@@ -967,6 +974,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
       mbar_init(&tempty[a], EPI_WARPS);
     }
     mbar_init(&pbar[0], 1);
+    if (EX::kOn) {
+      mbar_init(ufull, 1);
+      mbar_init(ufree, 1);
+    }
     if (KS && S > 1) mbar_arrive_expect_tx(&pbar[0], part_bytes<BN>());  // S slots of 128/S rows
     if (QB)
       for (int s = 0; s < STAGES; s++) {
@@ -1040,6 +1051,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
       uint32_t phase = 0;
       bool ok = true;
       int it = 0;  // k blocks issued so far (the first `pre` have their weight block in flight)
+      [[maybe_unused]] uint32_t u_phase = 0;
+      [[maybe_unused]] bool u_issued = false;
       for (int w = blockIdx.x; w < args.ntiles * S && ok; w += gridDim.x) {
         const int t = w / S, kb0 = (w % S) * KB / S, kb1 = (w % S + 1) * KB / S;
         int m0 = (t / args.ntile_n) * BM, n0 = (t % args.ntile_n) * BN;
@@ -1074,6 +1087,28 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
         if constexpr (EX::kOn) {
           if (ex.defer) pdl_wait();  // the kernel that wrote U
           const int2 sg = tile_segments(ex, m0, BM, args.M);
+          if (ex.resident && sg.x < sg.y) {
+            if (!mbar_wait(ufree, u_phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
+            mbar_arrive_expect_tx(ufull, ex.nchunks * A_BYTES);
+            for (int c = 0; c < ex.nchunks; c++) tma_load_2d(sU + c * A_BYTES, &ex.tmU, ufull, c * 64, m0);
+            u_issued = true;
+            u_phase ^= 1;
+            for (int s = sg.x; s < sg.y; s += 2 * ex.per) {
+              const int n = min(2 * ex.per, sg.y - s);
+              if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
+              mbar_arrive_expect_tx(&full[stage], n * (BN / 64) * ex.prows * 128);
+#pragma unroll 1
+              for (int i = 0; i < n; i++) {
+                const int a = __ldg(&ex.segs[s + i].z);
+                uint8_t* dst = i < ex.per ? sA + stage * A_BYTES : sB + stage * B_BYTES - ex.per * (BN / 64) * ex.prows * 128;
+                for (int h = 0; h < BN / 64; h++) tma_load_3d(dst + (i * (BN / 64) + h) * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, 0, a);
+              }
+              issued[stage] = 1;
+              iss_phase[stage] = phase;
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+            continue;
+          }
           for (int s = sg.x; s < sg.y && ok; s += ex.per)
             for (int c = 0; c < ex.nchunks; c++) {
               const int n = min(ex.per, sg.y - s);
@@ -1103,6 +1138,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           while (!mbar_try_wait(&pfull[s], pk_phase[s]) && gtimer() - t0 < kWaitNs) {}
         }
       }
+      if (EX::kOn && u_issued) {
+        uint64_t t0 = gtimer();
+        while (!mbar_try_wait(ufull, u_phase ^ 1) && gtimer() - t0 < kWaitNs) {}
+      }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer
@@ -1117,6 +1156,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
       bool committed = false;
       uint64_t* last = nullptr;
       uint32_t last_phase = 0;
+      [[maybe_unused]] uint32_t u_phase = 0;
       for (int w = blockIdx.x; w < args.ntiles * S && ok; w += gridDim.x) {
         const int kb0 = (w % S) * KB / S, kb1 = (w % S + 1) * KB / S;
         [[maybe_unused]] int2 sg = make_int2(0, 0);
@@ -1142,6 +1182,36 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
         }
         if constexpr (EX::kOn) {
           const int m0 = (w / args.ntile_n) * BM;
+          if (ex.resident && sg.x < sg.y) {
+            if (!mbar_wait(ufull, u_phase, abort, &g_gemm_err)) { ok = false; break; }
+            u_phase ^= 1;
+            const uint32_t high = smem_u32(sU), low = ex.nchunks == 1 ? high + ex.prows * 2 : high + A_BYTES;
+            for (int s = sg.x; s < sg.y; s += 2 * ex.per) {
+              const int n = min(2 * ex.per, sg.y - s);
+              if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
+              tc_fence_after();
+#pragma unroll 1
+              for (int i = 0; i < n; i++) {
+                const int4 seg = __ldg(ex.segs + s + i);
+                uint32_t off[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
+                const uint32_t p = (i < ex.per ? smem_u32(sA + stage * A_BYTES) : smem_u32(sB + stage * B_BYTES) - ex.per * (BN / 64) * ex.prows * 128) +
+                                   i * (BN / 64) * ex.prows * 128;
+                for (int k = 0; k < ex.prows / 16; k++) {
+                  const uint64_t pd = sdesc_sw128_mn(p + k * 2048, ex.prows * 128);
+                  tc_mma_lanes(d, sdesc_sw128(high + k * 32), pd, idesc_t, 1u, off);
+                  tc_mma_lanes(d, sdesc_sw128(low + k * 32), pd, idesc_t, 1u, off);
+                }
+              }
+              tc_commit(&empty[stage]);
+              last = &empty[stage];
+              last_phase = phase;
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            tc_commit(ufree);
+          } else
           for (int s = sg.x; s < sg.y && ok; s += ex.per)
             for (int c = 0; c < ex.nchunks; c++) {
               const int n = min(ex.per, sg.y - s);
@@ -1604,7 +1674,7 @@ CUtensorMap tensor_map_u8(const void* ptr, int64_t rows, int64_t cols, int box_c
 template <typename T, int BN, int STAGES, bool TMAE, typename EX = GemmPlain>
 void launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my, const CUtensorMap& mr, const GemmArgs& a,
                  cudaStream_t st, const EX& ex = EX()) {
-  constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(TMAE || EX::kOn);
+  constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(TMAE || EX::kOn) + (EX::kOn ? 2 * BM * BK * 2 : 0);
   static_assert(smem <= 232448, "GEMM shared memory above the 227 KB per-CTA limit");
   static bool attr = false;
   if (!attr) {
@@ -1867,6 +1937,7 @@ void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
   ex.half = s.u_cols <= 64 ? s.u_cols / 32 : 4;
   ex.pgroups = std::max(1, s.u_cols / 128);
   ex.per = 64 / ex.prows;
+  ex.resident = s.u_cols <= 128;
   ex.defer = c.after_share ? 1 : 0;
   ex.kb_off = c.w ? 0 : 1;  // a block past the end of the stand-in maps below, which TMA fills with zeros
   const CUtensorMap ma = c.w ? tensor_map(c.x, c.M, c.K, c.ldx, BK, BM, dtype) : tensor_map(s.u, 1, 8, 8, BK, BM, dtype);
@@ -1899,9 +1970,9 @@ void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
     shape(128);
     if (tmae) {
       const CUtensorMap my = tensor_map(c.y, c.M, c.N, c.ldy, 64, 32, dtype);
-      launch_gemm<T, 128, 6, true, GemmAdapted<WT>>(ma, weight_map(128), my, my, a, st, ex);
+      launch_gemm<T, 128, 5, true, GemmAdapted<WT>>(ma, weight_map(128), my, my, a, st, ex);
     } else {
-      launch_gemm<T, 128, 6, false, GemmAdapted<WT>>(ma, weight_map(128), ma, ma, a, st, ex);
+      launch_gemm<T, 128, 5, false, GemmAdapted<WT>>(ma, weight_map(128), ma, ma, a, st, ex);
     }
   }
   LC_LAUNCHED(1);
