@@ -185,12 +185,47 @@ __global__ void __launch_bounds__(128) k_outer_f32(const float* __restrict__ Q, 
 
 // ------------------------------------------------------------- operands
 
-struct Held {  // tensors made inside an op, released when it returns or throws
+// Scratch kept from call to call (padded operands, Q, partial sums): an
+// allocation and its release cost 1.2 us each call, a tenth of a small one.
+// It belongs to the stream of its first use (one that nobody can destroy: the
+// library's own or CUDA's default ones), whose order separates one call's
+// contents from the next; calls on other streams, in captures and beyond
+// kMost allocate theirs. It grows to what the calls before have asked for.
+struct Workspace {
+  static constexpr size_t kMost = (size_t)32 << 20;
+  char* p = nullptr;
+  size_t bytes = 0, want = 0;
+  cudaStream_t st = nullptr;
+  bool usable() {
+    if (capturing() || !want || !permanent_stream() || (p && st != stream())) return false;
+    if (want > bytes) {
+      if (p) dfree(p);
+      p = nullptr;
+      bytes = 0;
+      const size_t n = want;
+      want = 0;  // (set again below: a failed allocation is not tried at every call)
+      p = (char*)dmalloc(n);
+      st = stream();
+      want = bytes = n;
+    }
+    return p != nullptr;
+  }
+};
+Workspace& workspace() {
+  static Workspace w;
+  return w;
+}
+
+struct Held {  // tensors and scratch of one call, released when it returns or throws
   std::vector<LcTensor*> ts;
   std::vector<void*> mem;
+  const bool kept = workspace().usable();
+  size_t used = 0, asked = 0;  // of the workspace; in all
   ~Held() {
     for (auto* t : ts) release(t);
     for (void* p : mem) dfree(p);
+    Workspace& w = workspace();
+    if (asked <= Workspace::kMost && asked > w.want && !capturing()) w.want = (asked + 65535) / 65536 * 65536;
   }
   LcTensor* dense(LcTensor* t) {
     LcTensor* c = contiguous(t);
@@ -202,6 +237,12 @@ struct Held {  // tensors made inside an op, released when it returns or throws
     return t;
   }
   void* scratch(size_t bytes) {
+    bytes = (bytes + 255) / 256 * 256;
+    asked += bytes;
+    if (kept && used + bytes <= workspace().bytes) {
+      used += bytes;
+      return workspace().p + used - bytes;
+    }
     mem.push_back(nullptr);
     return mem.back() = dmalloc(bytes);
   }
@@ -497,6 +538,8 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
 void lc_adapters_destroy() {
   for (auto* p : plans()) plan_release(p);
   plans().clear();
+  if (workspace().p) cudaFree(workspace().p);  // waits for its uses, on whichever stream
+  workspace() = Workspace();
 }
 
 extern "C" {

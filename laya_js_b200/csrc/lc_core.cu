@@ -67,6 +67,10 @@ static void ensure_init() {
 }
 
 cudaStream_t stream() { return S().cur; }
+bool permanent_stream() {
+  const State& s = S();
+  return s.cur == s.own || s.cur == cudaStreamLegacy || s.cur == cudaStreamPerThread;
+}
 int device() { return S().device; }
 int num_sms() { return S().sms; }
 void count_launch(int n) { S().launches += n; }

@@ -401,3 +401,41 @@ def test_rows_without_an_adapter_over_used_memory(dtype, T):
     _check(vals(b.read(A.adapter_linear(b, t["x"], t["w"], None, t["a"], t["bt"], t["scales"], plan))), want, bound, "y")
     for name, g, v, m in zip(("dx", "da", "db"), A.adapter_linear_grad(b, t["dy"], t["x"], t["w"], t["a"], t["bt"], t["scales"], plan), wg, bg):
         _check(vals(b.read(g)), v, m, name)
+
+
+def test_calls_of_every_size_in_turn_and_on_two_streams():
+    """Scratch is kept between calls: small and large calls, padded and not,
+    alternating on the library's stream and on others, keep their bits."""
+    import torch
+
+    from laya_js_b200 import _lib, interop
+    b = backend()
+    jobs = []
+    for T, K, N, r, req in ((4, 64, 72, 8, 4), (900, 201, 129, 12, 7), (3000, 256, 264, 40, 9), (60, 33, 5, 3, 20)):
+        h, cu, ad = case("bf16", T, K, N, 3, r, req, seed=T)
+        t = _up(b, h)
+        jobs.append((t, A.AdapterPlan(b, cu, ad, 3)))
+
+    def run(job):
+        t, plan = job
+        y = A.adapter_linear(b, t["x"], t["w"], None, t["a"], t["bt"], t["scales"], plan)
+        return [y, *A.adapter_linear_grad(b, t["dy"], t["x"], t["w"], t["a"], t["bt"], t["scales"], plan)]
+
+    want = [[b.read(v).data for v in run(j)] for j in jobs]
+    others = [torch.cuda.Stream(), torch.cuda.default_stream()]
+    try:
+        for turn in range(6):
+            for s in (None, *others):
+                torch.cuda.synchronize()
+                if s is None:
+                    _lib.call("lc_set_stream", 0)
+                else:
+                    with torch.cuda.stream(s):
+                        interop.useTorchStream(b)
+                b.flush()
+                got = [run(jobs[(i + turn) % len(jobs)]) for i in range(len(jobs))]  # queued one after the other
+                for i, vs in enumerate(got):
+                    assert all(np.array_equal(b.read(v).data, w) for v, w in zip(vs, want[(i + turn) % len(jobs)]))
+    finally:
+        torch.cuda.synchronize()
+        _lib.call("lc_set_stream", 0)
