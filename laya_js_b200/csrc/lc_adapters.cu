@@ -350,51 +350,51 @@ struct Rows {
 };
 
 // Copies rows of `cols` values into rows of `ld` (a multiple of 8), zeros after
-// them: up to five matrices a launch, eight values per thread step. Bound by
-// the 2-byte loads (1537 x 1001, 777 x 1001 and two banks: 4.4 us).
+// them: up to five matrices a launch, eight values per thread step, the steps
+// of all matrices in one range. Bound by the latency of the 2-byte loads (1537
+// x 1001, 777 x 1001 and two banks: 3.9 us; matrix after matrix 4.4).
 struct PadJob {
   const uint16_t* src;
   uint16_t* dst;
-  int64_t rows, cols, ld;
+  int64_t first, cols, ld;  // first: steps of the matrices before it
 };
 struct PadJobs {
   int n;
+  int64_t total;
   PadJob j[5];
 };
 __global__ void __launch_bounds__(256) k_pad_rows(const __grid_constant__ PadJobs jobs) {
   pdl_trigger();
   pdl_wait();
-  for (int k = 0; k < jobs.n; k++) {
+  LC_GRID_STRIDE(g, jobs.total) {
+    int k = jobs.n - 1;
+    while (g < jobs.j[k].first) k--;
     const PadJob& j = jobs.j[k];
-    const int64_t vecs = j.ld / 8, total = j.rows * vecs;
-    LC_GRID_STRIDE(i, total) {
-      const int64_t row = i / vecs, c = (i % vecs) * 8;
-      const uint16_t* s = j.src + row * j.cols + c;
-      uint16_t v[8];
+    const int64_t i = g - j.first, vecs = j.ld / 8, row = i / vecs, c = (i % vecs) * 8;
+    const uint16_t* s = j.src + row * j.cols + c;
+    uint16_t v[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = c + e < j.cols ? s[e] : (uint16_t)0;
-      *(uint4*)(j.dst + row * j.ld + c) = *(const uint4*)v;
-    }
+    for (int e = 0; e < 8; e++) v[e] = c + e < j.cols ? s[e] : (uint16_t)0;
+    *(uint4*)(j.dst + row * j.ld + c) = *(const uint4*)v;
   }
 }
 
 struct Padder {
   Held& held;
   PadJobs jobs{};
-  int64_t work = 0;
   Rows of(const LcTensor* t, int64_t rows, int64_t cols) {
     if (!t) return {};
     if (cols % 8 == 0 && ((uintptr_t)t->data() & 15) == 0) return {t->data(), cols};
     const int64_t ld = (cols + 7) / 8 * 8;
     void* d = held.scratch((size_t)(rows * ld) * 2);
-    jobs.j[jobs.n++] = {(const uint16_t*)t->data(), (uint16_t*)d, rows, cols, ld};
-    work = std::max(work, rows * ld / 8);
+    jobs.j[jobs.n++] = {(const uint16_t*)t->data(), (uint16_t*)d, jobs.total, cols, ld};
+    jobs.total += rows * ld / 8;
     return {d, ld};
   }
   // true when a kernel was launched: the next one may start while it runs, and waits for it
   bool run() {
-    if (!jobs.n || !work) return false;
-    launch_chain(k_pad_rows, dim3(blocks_for(work, 256)), dim3(256), 0, stream(), jobs);
+    if (!jobs.total) return false;
+    launch_chain(k_pad_rows, dim3(blocks_for(jobs.total, 256)), dim3(256), 0, stream(), jobs);
     LC_LAUNCHED(1);
     return true;
   }
