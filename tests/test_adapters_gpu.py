@@ -439,3 +439,40 @@ def test_calls_of_every_size_in_turn_and_on_two_streams():
     finally:
         torch.cuda.synchronize()
         _lib.call("lc_set_stream", 0)
+
+
+@pytest.mark.parametrize("T,K,N", [(3000001, 768, 8), (300001, 64, 8192), (3000001, 765, 8)])
+def test_more_than_2_31_elements(T, K, N):
+    """Operands of 2.3 to 2.5 thousand million values (made and checked on the
+    device): the last rows, and an adapter that only they use."""
+    import torch
+
+    from laya_js_b200 import _lib, interop
+    b = backend()
+    r, tail = 4, 700
+    g = torch.Generator(device="cuda").manual_seed(T)
+    make = lambda *s, std=1.0: (torch.randn(s, generator=g, device="cuda", dtype=torch.bfloat16) * std).to(torch.bfloat16)
+    x, dy, w, a, bt = make(T, K), make(T, N), make(N, K, std=0.05), make(2, r, K, std=K ** -0.5), make(2, r, N, std=0.1)
+    interop.useTorchStream(b)
+    try:
+        tx, tdy, tw, ta, tb = (interop.fromTorch(b, v) for v in (x, dy, w, a, bt))
+        plan = A.AdapterPlan(b, [0, 1000, T - tail, T], [0, -1, 1], 2)
+        y = interop.toTorch(b, A.adapter_linear(b, tx, tw, None, ta, tb, None, plan))
+        dx, da, db = (interop.toTorch(b, v) for v in A.adapter_linear_grad(b, tdy, tx, tw, ta, tb, None, plan))
+        for rows, k in ((slice(T - tail, T), 1), (slice(0, 1000), 0), (slice(T - tail - 500, T - tail), None)):
+            xs, ds, w64 = x[rows].double(), dy[rows].double(), w.double()
+            wk = w64 if k is None else w64 + bt[k].double().t() @ a[k].double()
+            for got, want in ((y[rows], xs @ wk.t()), (dx[rows], ds @ wk)):
+                # bf16: one rounding; f32 sums of at most 8192 terms against the largest result
+                assert torch.all((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * want.abs().max() * 0.1)
+            if k is not None:
+                u, gr = xs @ a[k].double().t(), ds @ bt[k].double().t()
+                for got, want in ((da[k], gr.t() @ xs), (db[k], u.t() @ ds)):
+                    assert torch.all((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * want.abs().max() * 0.1)
+        plan.free()
+    finally:
+        torch.cuda.synchronize()
+        b.flush()
+        _lib.call("lc_set_stream", 0)
+        del x, dy
+        torch.cuda.empty_cache()
