@@ -31,7 +31,10 @@ __device__ __forceinline__ uint32_t idesc_rt(int n, bool a_mn, bool b_mn) {
   return (1u << 4) | (TcFmt<T>::ab << 7) | (TcFmt<T>::ab << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 }
+// The load is warp-wide (.aligned): the lanes meet first, since the code before
+// it treats rows of a warp differently.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  __syncwarp();
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
       T* Q = (T*)args.job[it.job].Q + (int64_t)row * args.ucols;
       for (int s = 0; s < it.segs.y && ok; s += args.nb) {
         const int n = min(args.nb, it.segs.y - s);
-        if (!mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err)) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err))) { ok = false; break; }
         tc_fence_after();
         for (int i = 0; i < n; i++) {
           const int4 g = __ldg(&args.segs[it.segs.x + s + i]);
@@ -255,22 +258,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
             uint32_t v[16];
             tmem_ld16(tb + c, v);
             tmem_wait_ld();
-            if (!mine) continue;
-            if (S > 1) {  // this CTA's share of the columns, added below
+            if (mine && S > 1) {  // this CTA's share of the columns, added below
               float4* p = (float4*)(sD + (quarter * 32 + lane) * args.R + c);
 #pragma unroll
               for (int j = 0; j < 4; j++)
                 p[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
-              continue;
-            }
-            alignas(16) T hi[16], lo[16];
+            } else if (mine) {
+              alignas(16) T hi[16], lo[16];
 #pragma unroll
-            for (int j = 0; j < 16; j++) split2<T>(c + j < args.rank ? sc * __uint_as_float(v[j]) : 0.f, hi[j], lo[j]);
-            uint4 *ph = (uint4*)(Q + c), *pl = (uint4*)(Q + half + c);
-            ph[0] = ((const uint4*)hi)[0];
-            ph[1] = ((const uint4*)hi)[1];
-            pl[0] = ((const uint4*)lo)[0];
-            pl[1] = ((const uint4*)lo)[1];
+              for (int j = 0; j < 16; j++) split2<T>(c + j < args.rank ? sc * __uint_as_float(v[j]) : 0.f, hi[j], lo[j]);
+              uint4 *ph = (uint4*)(Q + c), *pl = (uint4*)(Q + half + c);
+              ph[0] = ((const uint4*)hi)[0];
+              ph[1] = ((const uint4*)hi)[1];
+              pl[0] = ((const uint4*)lo)[0];
+              pl[1] = ((const uint4*)lo)[1];
+            }
           }
         }
         tc_fence_before();
@@ -541,7 +543,7 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
       const int col0 = t.c0 + quarter * 32 + lane, j0 = t.j0, halves = t.halves;
       T* dP = (T*)job.dP;
       f = min(hi, tile0 + p1);
-      if (!mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err))) break;
       tc_fence_after();
       for (int h = 0; h < halves; h++) {
         const int col = col0 + 128 * h;

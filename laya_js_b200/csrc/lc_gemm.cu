@@ -616,6 +616,7 @@ __device__ __forceinline__ void epilogue_tma(const GemmArgs& args, const CUtenso
       }
       const float2 bias2 = bias_pair(args, col, lane);
       uint32_t racc[64];
+      __syncwarp();  // the load is warp-wide, what precedes it was not
       tmem_ld64(tbase + u * 64, racc);
       tmem_wait_ld();
       // the last unit this warp reads: the loop ends after it, or the next unit (output block) is past the weight rows
@@ -1291,6 +1292,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
 #pragma unroll 1
       for (int u = half * (U / 2); u < (half + 1) * (U / 2); u++) {
         uint32_t ra[32], rb[32];
+        __syncwarp();  // the loads are warp-wide, the stores of the unit before were not
         tmem_ld32(tbase + u * 64, ra);
         tmem_ld32(tbase + u * 64 + 32, rb);
         tmem_wait_ld();
