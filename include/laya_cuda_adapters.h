@@ -42,10 +42,11 @@ int lc_adapter_plan_free(uint64_t plan);
  * that is computed elsewhere, such as a packed one); bias [N] or 0;
  * a [n, r, K], b [n, r, N] and scales f32 [n] (0 = every scale 1) with
  * n = the plan's n_adapters. x, w, a and b share a dtype: f32, f16 or bf16.
- * Sums are held in f32 and rounded once; with f16 and bf16 u is held as two
- * 16-bit parts, exact to 2^-22 and 2^-16 of each value (f16: to 2^-25, and up
- * to 131,008). No row's result depends on another row or on another request's
- * adapter, finite or not.
+ * Sums are held in f32 and rounded once, u as three bf16 parts that make up
+ * the f32 value (all of its bits and range). No row's result depends on
+ * another row or on another request's adapter, finite or not; a result that
+ * depends on an inf or a NaN is one of the two (NaN also where f32 arithmetic
+ * would keep an inf, since the parts of u meet it one by one).
  */
 int lc_adapter_linear(lc_tensor* out, lc_tensor x, lc_tensor w, lc_tensor bias, lc_tensor a, lc_tensor b, lc_tensor scales, uint64_t plan);
 
@@ -57,7 +58,9 @@ int lc_adapter_linear(lc_tensor* out, lc_tensor x, lc_tensor w, lc_tensor bias, 
  *   da_a = Σ_t g[t] ⊗ x[t]               [n, r, K]
  *   db_a = Σ_t u[t] ⊗ dy[t]              [n, r, N]
  * over the rows t of adapter a; an adapter without rows gets zeros. In the
- * inputs' dtype, summed in f32 in a fixed order (the same bits every run).
+ * inputs' dtype, summed in f32 in a fixed order (the same bits every run). u
+ * and g are held as for adapter_linear; in the sums da and db of f16, whose
+ * MMA takes f16 parts, exact to 2^-39 and up to 3.4e10 in magnitude.
  */
 int lc_adapter_linear_grad(lc_tensor* dx, lc_tensor* da, lc_tensor* db, lc_tensor dy, lc_tensor x, lc_tensor w, lc_tensor a, lc_tensor b,
                            lc_tensor scales, uint64_t plan);

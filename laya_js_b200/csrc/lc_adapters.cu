@@ -350,18 +350,23 @@ struct Rows {
 };
 
 // Copies rows of `cols` values into rows of `ld` (a multiple of 8), zeros after
-// them: up to five matrices a launch, eight values per thread step, the steps
-// of all matrices in one range. Bound by the latency of the 2-byte loads (1537
+// them, eight values per thread step, up to six matrices a launch, the steps
+// of all of them in one range. Bound by the latency of the 2-byte loads (1537
 // x 1001, 777 x 1001 and two banks: 3.9 us; matrix after matrix 4.4).
+// R > 0: an f16 bank [n, rank, cols] as bf16 values and remainders, [used
+// adapters, 2·R, ld] with zeros from the rank on: the 11 bits of an f16 as two
+// bf16, which the tensor cores multiply with the bf16 parts of u (lc_gemm.cu).
 struct PadJob {
   const uint16_t* src;
   uint16_t* dst;
   int64_t first, cols, ld;  // first: steps of the matrices before it
+  int rank, R, vec;         // vec: the source rows are 16-byte aligned
+  const int32_t* used;
 };
 struct PadJobs {
   int n;
   int64_t total;
-  PadJob j[5];
+  PadJob j[6];
 };
 __global__ void __launch_bounds__(256) k_pad_rows(const __grid_constant__ PadJobs jobs) {
   pdl_trigger();
@@ -371,24 +376,60 @@ __global__ void __launch_bounds__(256) k_pad_rows(const __grid_constant__ PadJob
     while (g < jobs.j[k].first) k--;
     const PadJob& j = jobs.j[k];
     const int64_t i = g - j.first, vecs = j.ld / 8, row = i / vecs, c = (i % vecs) * 8;
-    const uint16_t* s = j.src + row * j.cols + c;
-    uint16_t v[8];
+    int64_t from = row, to = row;
+    bool live = true;
+    if (j.R) {
+      const int64_t slot = row / j.R, r = row % j.R;
+      live = r < j.rank;
+      from = __ldg(j.used + slot) * (int64_t)j.rank + r;
+      to = slot * 2 * j.R + r;
+    }
+    const uint16_t* s = j.src + from * j.cols + c;
+    alignas(16) uint16_t v[8] = {};
+    if (live && j.vec) {
+      *(uint4*)v = __ldg((const uint4*)s);
+    } else if (live) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = c + e < j.cols ? s[e] : (uint16_t)0;
-    *(uint4*)(j.dst + row * j.ld + c) = *(const uint4*)v;
+      for (int e = 0; e < 8; e++) v[e] = c + e < j.cols ? s[e] : (uint16_t)0;
+    }
+    uint4* d = (uint4*)(j.dst + to * j.ld + c);
+    if (!j.R) {
+      *d = *(const uint4*)v;
+      continue;
+    }
+    alignas(16) __nv_bfloat16 high[8], low[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float f = __half2float(__ushort_as_half(v[e]));
+      high[e] = __float2bfloat16_rn(f);
+      low[e] = __float2bfloat16_rn(isfinite(f) ? f - __bfloat162float(high[e]) : 0.f);
+    }
+    *d = *(const uint4*)high;
+    d[j.R * j.ld / 8] = *(const uint4*)low;
   }
 }
 
 struct Padder {
   Held& held;
   PadJobs jobs{};
+  void add(const LcTensor* t, void* d, int64_t steps, int64_t cols, int64_t ld, int rank, int R, const int32_t* used) {
+    jobs.j[jobs.n++] = {(const uint16_t*)t->data(), (uint16_t*)d, jobs.total, cols, ld, rank, R, cols % 8 == 0 && ((uintptr_t)t->data() & 15) == 0, used};
+    jobs.total += steps;
+  }
   Rows of(const LcTensor* t, int64_t rows, int64_t cols) {
     if (!t) return {};
     if (cols % 8 == 0 && ((uintptr_t)t->data() & 15) == 0) return {t->data(), cols};
     const int64_t ld = (cols + 7) / 8 * 8;
     void* d = held.scratch((size_t)(rows * ld) * 2);
-    jobs.j[jobs.n++] = {(const uint16_t*)t->data(), (uint16_t*)d, jobs.total, cols, ld};
-    jobs.total += rows * ld / 8;
+    add(t, d, rows * ld / 8, cols, ld, 0, 0, nullptr);
+    return {d, ld};
+  }
+  // The bank beside a projection on the tensor cores: bf16 rows, or those of an f16 bank's used adapters in two parts.
+  Rows share(const LcTensor* bank, const AdapterPlan& p, int rank, int64_t cols) {
+    if (bank->dtype == LC_BF16) return of(bank, bank->shape[0] * rank, cols);
+    const int64_t ld = (cols + 7) / 8 * 8, rows = (int64_t)p.nused * adapter_rank_rows(rank);
+    void* d = held.scratch((size_t)(2 * rows * ld) * 2);
+    add(bank, d, rows * ld / 8, cols, ld, rank, adapter_rank_rows(rank), p.used);
     return {d, ld};
   }
   // true when a kernel was launched: the next one may start while it runs, and waits for it
@@ -411,9 +452,9 @@ struct Chained {
   }
 };
 
-// Bytes of a Q, and the product that fills it.
-size_t q_bytes(const Operands& o) { return ((size_t)o.T * adapter_u_cols(o.r) * 2 + 255) / 256 * 256; }
-AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_t C, void* Q) {
+// Room for u or g as Q and as H, and the product that fills them.
+size_t parts_bytes(const Operands& o, int parts) { return ((size_t)o.T * parts * adapter_rank_rows(o.r) * 2 + 255) / 256 * 256; }
+AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_t C, void* Q, void* H) {
   AdapterShrink c;
   c.X = X.p;
   c.P = P.p;
@@ -423,7 +464,8 @@ AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_
   c.n = o.n;
   c.rank = o.r;
   c.scales = o.scale_ptr();
-  c.Q = Q;
+  c.Q = (__nv_bfloat16*)Q;
+  c.H = (__half*)H;
   return c;
 }
 
@@ -432,7 +474,8 @@ void shrink(const AdapterShrink* c, int njobs, const Operands& o, bool padded) {
   if (!adapter_shrink_rows(c, njobs, *o.plan, o.dtype, stream())) adapter_shrink_tc(c, njobs, *o.plan, o.dtype, stream());
 }
 
-void expand_tc(const Operands& o, const Rows& X, const Rows& W, const Rows& P, const void* Q, bool transposed, LcTensor* Y) {
+// y, or dx (transposed). `few`: the dot-product form, whose bank is in the operands' type; otherwise `bank` is Padder::share's.
+void expand_16(const Operands& o, const Rows& X, const Rows& W, const Rows& bank, const void* Q, bool transposed, bool few, LcTensor* Y) {
   GemmAdaptedCall c;
   c.x = X.p;
   c.M = o.T;
@@ -449,15 +492,18 @@ void expand_tc(const Operands& o, const Rows& X, const Rows& W, const Rows& P, c
   c.y = Y->data();
   c.ldy = c.N;
   c.share.u = Q;
-  c.share.u_cols = adapter_u_cols(o.r);
-  c.share.bank = P.p;
-  c.share.n = o.n;
-  c.share.rank = o.r;
-  c.share.ld = P.ld;
+  c.share.R = adapter_rank_rows(o.r);
+  c.share.bank = bank.p;
+  c.share.ld = bank.ld;
+  c.share.parts = o.dtype == LC_F16 ? 2 : 1;
+  c.share.n = o.dtype == LC_F16 ? o.plan->nused : o.n;
+  c.share.rows = o.dtype == LC_F16 ? 2 * c.share.R : o.r;
+  c.share.nsegs = o.plan->nsegs;
   c.share.segs = o.plan->segs;
   c.share.tiles = o.plan->tiles;
   c.after_share = o.plan->nsegs > 0;
-  if (!adapter_linear_rows(c, *o.plan, o.dtype, stream())) gemm_adapted(c, o.dtype, stream());
+  if (few) adapter_linear_rows(c, *o.plan, o.r, o.dtype, stream());
+  else gemm_adapted(c, o.dtype, stream());
 }
 
 void linear(const Operands& o, LcTensor* y, Held& held) {
@@ -468,14 +514,15 @@ void linear(const Operands& o, LcTensor* y, Held& held) {
     expand_f32(o, o.x, o.b, u, false, y);
     return;
   }
+  const bool few = adapter_linear_rows_fit(o.T, o.N, o.K, *o.plan);
   Padder pad{held};
   const Rows x = pad.of(o.x, o.T, o.K), w = pad.of(o.w, o.N, o.K), a = pad.of(o.a, (int64_t)o.n * o.r, o.K),
-             b = pad.of(o.b, (int64_t)o.n * o.r, o.N);
+             b = few ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : pad.share(o.b, *o.plan, o.r, o.N);
   const bool padded = pad.run();
-  const AdapterShrink u = shrink_job(o, x, a, o.K, held.scratch(q_bytes(o)));
+  const AdapterShrink u = shrink_job(o, x, a, o.K, held.scratch(parts_bytes(o, kQParts)), nullptr);
   shrink(&u, 1, o, padded);
   const Chained chained(o);
-  expand_tc(o, x, w, b, u.Q, false, y);
+  expand_16(o, x, w, b, u.Q, false, few, y);
 }
 
 void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held& held) {
@@ -498,39 +545,48 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
     }
     return;
   }
+  const bool f16 = o.dtype == LC_F16;
   Padder pad{held};
   const Rows dy = pad.of(o.dy, o.T, o.N), x = da || db ? pad.of(o.x, o.T, o.K) : Rows{}, w = dx ? pad.of(o.w, o.N, o.K) : Rows{},
-             a = dx || db ? pad.of(o.a, (int64_t)o.n * o.r, o.K) : Rows{}, b = dx || da ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : Rows{};
+             a = db || (dx && !f16) ? pad.of(o.a, (int64_t)o.n * o.r, o.K) : Rows{},
+             b = dx || da ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : Rows{}, bank = dx && f16 ? pad.share(o.a, *o.plan, o.r, o.K) : a;
   const bool padded = pad.run();
   AdapterOuter out[2];
   int no = 0;
-  auto job = [&](const Rows& X, int64_t C, LcTensor* dP) -> AdapterOuter& {
+  auto job = [&](const Rows& X, int64_t C, LcTensor* dP) {
     AdapterOuter& c = out[no++];
     c.X = X.p;
     c.C = C;
     c.ld = X.ld;
     c.rank = o.r;
     c.dP = dP->data();
-    return c;
   };
-  AdapterOuter* of_u = db ? &job(dy, o.N, db) : nullptr;
-  AdapterOuter* of_g = da ? &job(x, o.K, da) : nullptr;
-  const int nq = (dx || da ? 1 : 0) + (db ? 1 : 0);
-  if (!nq) return;
-  char* scratch = (char*)held.scratch(nq * q_bytes(o) + (no ? adapter_part_bytes(out, no, *o.plan) : 0));
+  if (db) job(dy, o.N, db);
+  if (da) job(x, o.K, da);
+  // beside the projection g is read as Q; the outer sums read u and g in the type of the rows they meet
+  const size_t q_bytes = parts_bytes(o, kQParts), h_bytes = parts_bytes(o, kHParts);
+  const bool gq = dx || (da && !f16), gh = da && f16;
+  size_t at = 0;
+  auto place = [&](bool want, size_t bytes) {
+    const size_t here = at;
+    if (want) at += bytes;
+    return here;
+  };
+  const size_t u_at = place(db != nullptr, f16 ? h_bytes : q_bytes), gq_at = place(gq, q_bytes), gh_at = place(gh, h_bytes);
+  if (!at) return;
+  char* scratch = (char*)held.scratch(at + (no ? adapter_part_bytes(out, no, *o.plan) : 0));
   AdapterShrink q[2];
-  void* Q = scratch;
+  int nq = 0;
   if (db) {
-    q[0] = shrink_job(o, x, a, o.K, Q);
-    of_u->Q = Q;
-    Q = (char*)Q + q_bytes(o);
+    q[nq++] = shrink_job(o, x, a, o.K, f16 ? nullptr : scratch + u_at, f16 ? scratch + u_at : nullptr);
+    out[0].parts = scratch + u_at;
   }
-  if (dx || da) q[nq - 1] = shrink_job(o, dy, b, o.N, Q);
-  if (da) of_g->Q = Q;
+  if (dx || da) q[nq++] = shrink_job(o, dy, b, o.N, gq ? scratch + gq_at : nullptr, gh ? scratch + gh_at : nullptr);
+  if (da) out[no - 1].parts = scratch + (f16 ? gh_at : gq_at);
   shrink(q, nq, o, padded);
   const Chained chained(o);
-  if (no) adapter_outer_tc(out, no, scratch + nq * q_bytes(o), *o.plan, o.dtype, stream());
-  if (dx) expand_tc(o, dy, w, a, Q, true, dx);
+  if (no) adapter_outer_tc(out, no, scratch + at, *o.plan, o.dtype, stream());
+  if (dx) expand_16(o, dy, w, bank, scratch + gq_at, true, false, dx);
 }
 
 }  // namespace
@@ -579,7 +635,13 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
     spans[2 * k + 1] = s.hi;
   }
   std::vector<int32_t> seg4, tiles;
-  for (auto& g : segs) seg4.insert(seg4.end(), {g.lo, g.hi, g.a, 0});
+  std::vector<int32_t> empty, used, place(n_adapters);
+  for (int a = 0; a < n_adapters; a++) {
+    std::vector<int32_t>& list = span_ptr[a] == span_ptr[a + 1] ? empty : used;
+    place[a] = (int32_t)list.size();
+    list.push_back(a);
+  }
+  for (auto& g : segs) seg4.insert(seg4.end(), {g.lo, g.hi, g.a, place[g.a]});
   for (int64_t m0 = 0, k = 0; m0 < T; m0 += 128) {
     while (k < (int64_t)S && segs[k].hi <= m0) k++;
     int64_t e = k;
@@ -593,9 +655,7 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
         chunks.insert(chunks.end(), {(int32_t)t, (int32_t)std::min<int64_t>(64, spans[2 * k + 1] - t), a, 0});
     chunk_ptr[a + 1] = (int32_t)(chunks.size() / 4);
   }
-  std::vector<int32_t> empty, pieces;
-  for (int a = 0; a < n_adapters; a++)
-    if (span_ptr[a] == span_ptr[a + 1]) empty.push_back(a);
+  std::vector<int32_t> pieces;
   if (T <= kRowsMost)
     for (auto& g : segs)
       for (int t = g.lo; t < g.hi; t += 8) pieces.insert(pieces.end(), {t, std::min(8, g.hi - t), g.a, 0});
@@ -608,7 +668,7 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   };
   const size_t o_spans = put(spans), o_ptr = put(span_ptr), o_segs = put(seg4), o_tiles = put(tiles),
                o_chunks = put(chunks), o_chunk_ptr = put(chunk_ptr), o_empty = put(empty),
-               o_pieces = put(pieces);
+               o_used = put(used), o_pieces = put(pieces);
   struct Guard {
     AdapterPlan* p;
     ~Guard() { if (p) plan_release(p); }
@@ -633,6 +693,8 @@ int lc_adapter_plan_create(uint64_t* out, const int32_t* cu_rows, const int32_t*
   p->host_chunk_ptr = std::move(chunk_ptr);
   p->empty = p->dev + o_empty;
   p->nempty = (int)empty.size();
+  p->used = p->dev + o_used;
+  p->nused = (int)used.size();
   p->pieces = (int4*)(p->dev + o_pieces);
   p->npieces = (int)(pieces.size() / 4);
   plans().insert(p);

@@ -7,9 +7,9 @@ constexpr int kAdapterMaxRank = 256;
 
 // Rows and adapters of one batch on the device (lc_adapter_plan_create).
 struct AdapterPlan {
-  int rows = 0, n_adapters = 0, nsegs = 0, nchunks = 0, nempty = 0, npieces = 0;
+  int rows = 0, n_adapters = 0, nsegs = 0, nchunks = 0, nempty = 0, nused = 0, npieces = 0;
   int32_t* dev = nullptr;          // one allocation behind the arrays below
-  int4* segs = nullptr;            // [nsegs]: row ranges with an adapter, ascending: lo, hi, adapter
+  int4* segs = nullptr;            // [nsegs]: row ranges with an adapter, ascending: lo, hi, adapter, its place in `used`
   int2* tiles = nullptr;           // per 128 rows: the first segment that meets them, and how many do
   int2* spans = nullptr;           // [nsegs]: the row ranges adapter by adapter, ascending within one
   int32_t* span_ptr = nullptr;     // [n_adapters + 1]: where each adapter's spans start
@@ -17,6 +17,7 @@ struct AdapterPlan {
   int32_t* chunk_ptr = nullptr;    // [n_adapters + 1]: where each adapter's blocks start
   std::vector<int32_t> host_chunk_ptr;
   int32_t* empty = nullptr;        // [nempty]: the adapters without rows
+  int32_t* used = nullptr;         // [nused]: the adapters with rows, ascending
   int4* pieces = nullptr;          // [npieces]: the segments in pieces of at most 8 rows (up to kRowsMost rows): row, rows, adapter
   cudaStream_t built_on = nullptr;
   cudaEvent_t built = nullptr;     // the arrays are on the device
@@ -38,40 +39,52 @@ __device__ __forceinline__ int adapter_of_row(const int2* tiles, const int4* seg
   return t >= s.x && t < s.y ? s.z : -1;
 }
 
-// 16-bit columns of a row of Q (lc_adapters_tc.cu): two parts of the rank
-// rounded up to 16, or to 64 above 32, where a part fills whole 128-byte rows.
-inline int adapter_u_cols(int rank) { return 2 * (rank <= 32 ? (rank + 15) / 16 * 16 : (rank + 63) / 64 * 64); }
+// u and g pass from kernel to kernel as 16-bit parts whose sum is the f32 value,
+// R = adapter_rank_rows(rank) columns per part:
+//   Q  bf16 [rows, 3·R]  the value, its remainder and the remainder of that: 8 bits each make f32's 24, over f32's range.
+//                        Read beside the projection (lc_gemm.cu, lc_adapters_rows.cu) and, in bf16, by the outer sums.
+//   H  f16 [rows, 4·R]   parts in units of 2^19, 2^8, 2^-3 and 2^-14, read by the outer sums of f16: their other operand
+//                        is f16, which an MMA cannot mix with bf16. Each part takes 11 bits of what the ones before left:
+//                        exact to 2^-39 up to 3.4e10 (beyond: inf), so neither a loss gradient of 1e-6 a row nor one
+//                        scaled by 2^16 loses bits that f32 keeps. Two f16 parts without units held no more than 2^-25,
+//                        1e-2 of the gradients for a dy of 3e-6 over 4096 rows.
+constexpr int kQParts = 3, kHParts = 4;
+inline int adapter_rank_rows(int rank) { return rank <= 32 ? (rank + 15) / 16 * 16 : (rank + 63) / 64 * 64; }
 
-// A value as two 16-bit parts, high part and remainder (Q of lc_adapters_tc.cu).
-template <typename T> __device__ __forceinline__ T largest();
-template <> __device__ __forceinline__ __half largest<__half>() { return __ushort_as_half(0x7bff); }
-template <> __device__ __forceinline__ __nv_bfloat16 largest<__nv_bfloat16>() { return __ushort_as_bfloat16(0x7f7f); }
-template <typename T>
-__device__ __forceinline__ void split2(float v, T& hi, T& lo) {
-  hi = from_f<T>(v);
-  float h = to_f<T>(hi);
-  if (!isfinite(h)) {
-    if (!isfinite(v)) {  // the value itself: its remainder would be NaN
-      lo = from_f<T>(0.f);
-      return;
-    }
-    h = copysignf(to_f<T>(largest<T>()), v);
-    hi = from_f<T>(h);
+__device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 (&q)[kQParts]) {
+  q[0] = __float2bfloat16_rn(v);
+  q[1] = q[2] = __float2bfloat16_rn(0.f);
+  if (!isfinite(v)) return;  // the value itself: its remainder would be NaN
+  if (!isfinite(__bfloat162float(q[0]))) q[0] = __float2bfloat16_rn(copysignf(0x1.fep127f, v));
+  const float r = v - __bfloat162float(q[0]);
+  q[1] = __float2bfloat16_rn(r);
+  q[2] = __float2bfloat16_rn(r - __bfloat162float(q[1]));
+}
+__device__ __forceinline__ void split_f16(float v, __half (&h)[kHParts]) {
+  const bool in = fabsf(v) < 0x1.ffcp34f;
+  float r = in ? v : 0.f;
+  const float unit[kHParts] = {0x1p19f, 0x1p8f, 0x1p-3f, 0x1p-14f}, per[kHParts] = {0x1p-19f, 0x1p-8f, 0x1p3f, 0x1p14f};
+#pragma unroll
+  for (int i = 0; i < kHParts; i++) {
+    h[i] = __float2half_rn(r * per[i]);
+    r -= __half2float(h[i]) * unit[i];
   }
-  lo = from_f<T>(v - h);
+  if (!in) h[0] = __float2half_rn(isnan(v) ? v : copysignf(INFINITY, v));
 }
 
-// Q[t] = s_a·P_a·X[t] for X [rows, C] and P [n, rank, C] (row strides ld, ldp: multiples of 8; 16-byte aligned).
+// s_a·P_a·X[t] as Q and H (each may be null) for X [rows, C] and P [n, rank, C] (row strides ld, ldp: multiples of 8;
+// 16-byte aligned).
 struct AdapterShrink {
   const void *X = nullptr, *P = nullptr;
   int64_t C = 0, ld = 0, ldp = 0;
   int n = 0, rank = 0;
   const float* scales = nullptr;
-  void* Q = nullptr;
+  __nv_bfloat16* Q = nullptr;
+  __half* H = nullptr;
 };
-// dP[a] = Σ_{t in a} Q[t] ⊗ X[t], [n, rank, C] dense.
+// dP[a] = Σ_{t in a} q[t] ⊗ X[t], [n, rank, C] dense; `parts` holds q as Q (bf16) or H (f16).
 struct AdapterOuter {
-  const void *X = nullptr, *Q = nullptr;
+  const void *X = nullptr, *parts = nullptr;
   int64_t C = 0, ld = 0;
   int rank = 0;
   void* dP = nullptr;
@@ -91,7 +104,9 @@ void adapter_outer_tc(const AdapterOuter* c, int njobs, void* part, const Adapte
 constexpr int kRowsMost = 16384;
 constexpr int64_t kRowsShrinkMost = 3 << 24, kRowsLinearMost = 1 << 25;
 bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
-bool adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int dtype, cudaStream_t st);
+bool adapter_linear_rows_fit(int64_t M, int64_t N, int64_t K, const AdapterPlan& p);
+// The forward product for a call that fits; c.share.bank [n, rank, ld] is in `dtype` here.
+void adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int rank, int dtype, cudaStream_t st);
 }  // namespace lc
 
 void lc_adapters_destroy();

@@ -90,13 +90,14 @@ __device__ __forceinline__ float dot_piece(const T* X, int64_t ldx, int nx, cons
 
 struct RowsShrinkJob {
   const void *X, *P;
-  void* Q;
+  __nv_bfloat16* Q;
+  __half* H;
   int64_t ldx, ldp;
   int C;
 };
 struct RowsShrinkArgs {
   RowsShrinkJob job[2];
-  int rank, R, ucols;
+  int rank, R;
   const int4* pieces;  // up to 8 rows of one adapter
   const float* scales;
 };
@@ -117,18 +118,28 @@ __global__ void __launch_bounds__(THREADS, 1) k_shrink_rows(const __grid_constan
   const int i = lane & 7, j = j0 + warp * 4 + (lane >> 3);
   if (i >= pc.y || j >= args.R) return;
   const float s = args.scales ? __ldg(args.scales + pc.z) : 1.f;
-  T hi, lo;
-  split2<T>(j < args.rank ? s * v : 0.f, hi, lo);
-  T* q = (T*)job.Q + ((int64_t)pc.x + i) * args.ucols + j;
-  q[0] = hi;
-  q[args.R] = lo;
+  const float q = j < args.rank ? s * v : 0.f;
+  const int64_t t = (int64_t)pc.x + i;
+  if (job.Q) {
+    __nv_bfloat16 part[kQParts];
+    split_bf16(q, part);
+#pragma unroll
+    for (int k = 0; k < kQParts; k++) job.Q[(t * kQParts + k) * args.R + j] = part[k];
+  }
+  if (job.H) {
+    __half part[kHParts];
+    split_f16(q, part);
+#pragma unroll
+    for (int k = 0; k < kHParts; k++) job.H[(t * kHParts + k) * args.R + j] = part[k];
+  }
 }
 
 struct RowsLinearArgs {
-  const void *x, *w, *bank, *Q, *bias;
+  const void *x, *w, *bank, *bias;
+  const __nv_bfloat16* Q;
   void* y;
   int64_t M, ldx, ldw, ldb, ldy;
-  int N, K, rank, ucols, bias_dtype, defer, ngroups;  // ngroups: groups of 16 columns
+  int N, K, rank, R, bias_dtype, defer, ngroups;  // ngroups: groups of 16 columns
   const int2* tiles;
   const int4* segs;
 };
@@ -152,12 +163,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_rows(const __grid_constan
   if (args.bias) v += ld_as<float>((const char*)args.bias, args.bias_dtype, n);
   const int a = adapter_of_row(args.tiles, args.segs, t);
   if (a >= 0) {
-    const T* q = (const T*)args.Q + t * args.ucols;
+    const __nv_bfloat16* q = args.Q + t * kQParts * args.R;
     const T* p = (const T*)args.bank + (int64_t)a * args.rank * args.ldb + n;
-    const int half = args.ucols / 2;
     float d = 0.f;
 #pragma unroll 8
-    for (int j = 0; j < args.rank; j++) d = fmaf(to_f<T>(q[j]) + to_f<T>(q[half + j]), to_f<T>(p[j * args.ldb]), d);
+    for (int j = 0; j < args.rank; j++) {
+      const float u = __bfloat162float(q[j]) + (__bfloat162float(q[args.R + j]) + __bfloat162float(q[2 * args.R + j]));
+      d = fmaf(u, to_f<T>(p[j * args.ldb]), d);
+    }
     v += d;
   }
   ((T*)args.y)[t * args.ldy + n] = from_f<T>(v);
@@ -167,22 +180,21 @@ template <typename T>
 void shrink_rows_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStream_t st) {
   RowsShrinkArgs a{};
   a.rank = c[0].rank;
-  a.ucols = adapter_u_cols(a.rank);
-  a.R = a.ucols / 2;
+  a.R = adapter_rank_rows(a.rank);
   a.pieces = p.pieces;
   a.scales = c[0].scales;
-  for (int j = 0; j < njobs; j++) a.job[j] = {c[j].X, c[j].P, c[j].Q, c[j].ld, c[j].ldp, (int)c[j].ld};
+  for (int j = 0; j < njobs; j++) a.job[j] = {c[j].X, c[j].P, c[j].Q, c[j].H, c[j].ld, c[j].ldp, (int)c[j].ld};
   launch_chain(k_shrink_rows<T>, dim3((unsigned)p.npieces, (unsigned)((a.R + COLS - 1) / COLS), (unsigned)njobs), dim3(THREADS), 0, st, a);
   LC_LAUNCHED(1);
 }
 
 template <typename T>
-void linear_rows_t(const GemmAdaptedCall& c, const AdapterPlan& p, cudaStream_t st) {
+void linear_rows_t(const GemmAdaptedCall& c, const AdapterPlan& p, int rank, cudaStream_t st) {
   RowsLinearArgs a{};
   a.x = c.x;
   a.w = c.w;
   a.bank = c.share.bank;
-  a.Q = c.share.u;
+  a.Q = (const __nv_bfloat16*)c.share.u;
   a.bias = c.bias;
   a.bias_dtype = c.bias_dtype;
   a.y = c.y;
@@ -193,8 +205,8 @@ void linear_rows_t(const GemmAdaptedCall& c, const AdapterPlan& p, cudaStream_t 
   a.ldy = c.ldy;
   a.N = (int)c.N;
   a.K = (int)c.ldx;  // rows of padded operands end in zeros
-  a.rank = c.share.rank;
-  a.ucols = c.share.u_cols;
+  a.rank = rank;
+  a.R = c.share.R;
   a.defer = c.after_share ? 1 : 0;
   a.tiles = p.tiles;
   a.segs = p.segs;
@@ -213,15 +225,15 @@ static int short_requests(const AdapterPlan& p) { return (int64_t)p.nsegs * 16 >
 bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st) {
   int64_t C = 0;
   for (int j = 0; j < njobs; j++) C += c[j].ld;
-  if (!p.npieces || (int64_t)p.rows * (adapter_u_cols(c[0].rank) / 2) * C > kRowsShrinkMost * short_requests(p)) return false;
+  if (!p.npieces || (int64_t)p.rows * adapter_rank_rows(c[0].rank) * C > kRowsShrinkMost * short_requests(p)) return false;
   dtype == LC_F16 ? shrink_rows_t<__half>(c, njobs, p, st) : shrink_rows_t<__nv_bfloat16>(c, njobs, p, st);
   return true;
 }
 
-bool adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int dtype, cudaStream_t st) {
-  if (c.transposed || c.M * c.N * c.K > kRowsLinearMost * short_requests(p)) return false;
-  dtype == LC_F16 ? linear_rows_t<__half>(c, p, st) : linear_rows_t<__nv_bfloat16>(c, p, st);
-  return true;
+bool adapter_linear_rows_fit(int64_t M, int64_t N, int64_t K, const AdapterPlan& p) { return M * N * K <= kRowsLinearMost * short_requests(p); }
+
+void adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int rank, int dtype, cudaStream_t st) {
+  dtype == LC_F16 ? linear_rows_t<__half>(c, p, rank, st) : linear_rows_t<__nv_bfloat16>(c, p, rank, st);
 }
 
 }  // namespace lc

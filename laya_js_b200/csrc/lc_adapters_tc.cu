@@ -1,13 +1,6 @@
 // The narrow products of the adapter operators on the tensor cores (f16 and
 // bf16): the shrink Q[t, :] = s_a·P_a·X[t] and the outer sums
 // dP_a = Σ_{t in a} Q[t] ⊗ X[t]. The wide product is gemm_adapted (lc_gemm.cu).
-//
-// Q is held as two 16-bit parts per value, high part and remainder, so that
-// the tensor cores read it back as exactly as an f32 would be at the scale of
-// the result (2^-16 of each value in bf16, 2^-22 in f16, 2^-25 absolute):
-// [T, 2·R] with the high parts in columns [0, R), R = rank rounded up to 16
-// (to 64 above 32). An f16 value beyond 65504 keeps its excess in the
-// remainder, up to 131008.
 #include "lc_adapters.h"
 #include "lc_api.h"
 #include "lc_gemm.h"
@@ -73,12 +66,13 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 // shared memory and are added in rank order.
 struct ShrinkJob {
   CUtensorMap tmX, tmP;
-  void* Q;
+  __nv_bfloat16* Q;
+  __half* H;
   int C, blocks;  // blocks: tmX brings both 64-column blocks of a stage (a 3-D map)
 };
 struct ShrinkArgs {
   ShrinkJob job[2];  // the longer one first
-  int njobs, T, ntiles, R, rank, nb, stages, ucols, S;
+  int njobs, T, ntiles, R, rank, nb, stages, S;
   int extra, filled;  // the second job's tiles that even out the first's last round (ShrinkItems)
   uint32_t bank_bytes, tmem_cols;
   const int4* segs;
@@ -124,6 +118,44 @@ struct ShrinkItems {
     return true;
   }
 };
+
+// Columns c .. c + N - 1 of row t of a product, into its Q and H.
+template <int N>
+__device__ __forceinline__ void store_q(const ShrinkJob& job, int64_t t, int R, int c, const float (&v)[N]) {
+  auto put = [](auto* dst, const auto (&part)[N]) {
+    if constexpr (N % 8 == 0) {
+#pragma unroll
+      for (int i = 0; i < N / 8; i++) ((uint4*)dst)[i] = ((const uint4*)part)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) dst[i] = part[i];
+    }
+  };
+  if (job.Q) {
+    alignas(16) __nv_bfloat16 p[kQParts][N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      __nv_bfloat16 q[kQParts];
+      split_bf16(v[i], q);
+#pragma unroll
+      for (int k = 0; k < kQParts; k++) p[k][i] = q[k];
+    }
+#pragma unroll
+    for (int k = 0; k < kQParts; k++) put(job.Q + (t * kQParts + k) * R + c, p[k]);
+  }
+  if (job.H) {
+    alignas(16) __half p[kHParts][N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      __half q[kHParts];
+      split_f16(v[i], q);
+#pragma unroll
+      for (int k = 0; k < kHParts; k++) p[k][i] = q[k];
+    }
+#pragma unroll
+    for (int k = 0; k < kHParts; k++) put(job.H + (t * kHParts + k) * R + c, p[k]);
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_constant__ ShrinkArgs args) {
@@ -237,13 +269,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
       }
     }
   } else {
-    const int quarter = warp & 3, half = args.ucols / 2;
+    const int quarter = warp & 3;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     for (ShrinkItems it(args, first, step); ok && it.next();) {
       const int row = it.t * BM + quarter * 32 + lane;
-      T* Q = (T*)args.job[it.job].Q + (int64_t)row * args.ucols;
       for (int s = 0; s < it.segs.y && ok; s += args.nb) {
         const int n = min(args.nb, it.segs.y - s);
         if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, abort, &g_adapter_err))) { ok = false; break; }
@@ -264,14 +295,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
               for (int j = 0; j < 4; j++)
                 p[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
             } else if (mine) {
-              alignas(16) T hi[16], lo[16];
+              float q[16];
 #pragma unroll
-              for (int j = 0; j < 16; j++) split2<T>(c + j < args.rank ? sc * __uint_as_float(v[j]) : 0.f, hi[j], lo[j]);
-              uint4 *ph = (uint4*)(Q + c), *pl = (uint4*)(Q + half + c);
-              ph[0] = ((const uint4*)hi)[0];
-              ph[1] = ((const uint4*)hi)[1];
-              pl[0] = ((const uint4*)lo)[0];
-              pl[1] = ((const uint4*)lo)[1];
+              for (int j = 0; j < 16; j++) q[j] = c + j < args.rank ? sc * __uint_as_float(v[j]) : 0.f;
+              store_q(args.job[it.job], row, args.R, c, q);
             }
           }
         }
@@ -292,7 +319,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
     // one item per cluster: rank r adds rows [r·128/S, (r+1)·128/S) of all the CTAs' shares
     const int t = first >= args.ntiles ? first - args.ntiles : first, m0 = t * BM, rows = BM / S;
     const int2 segs = __ldg(args.tiles + t);
-    T* Q = (T*)args.job[first >= args.ntiles].Q;
+    const ShrinkJob& job = args.job[first >= args.ntiles];
     for (int lr = rank * rows + (int)threadIdx.x / 16; lr < (rank + 1) * rows; lr += TC_THREADS / 16) {
       const int row = m0 + lr;
       int a = -1;
@@ -306,10 +333,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
         const uint32_t at = smem_u32(sD + lr * args.R + c);
         float v = 0.f;
         for (int q = 0; q < S; q++) v += ld_cluster_f32(mapa_rank(at, (uint32_t)q));
-        T hi, lo;
-        split2<T>(c < args.rank ? sc * v : 0.f, hi, lo);
-        Q[(int64_t)row * args.ucols + c] = hi;
-        Q[(int64_t)row * args.ucols + args.ucols / 2 + c] = lo;
+        const float q[1] = {c < args.rank ? sc * v : 0.f};
+        store_q(job, row, args.R, c, q);
       }
     }
     cluster_sync();  // no CTA leaves while another reads its shared memory
@@ -327,8 +352,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
 // D [columns of X, N] += X-blockᵀ · Q-block over blocks of up to 64 rows of one
 // adapter and 256 columns (two M = 128 accumulators, so that Q and the steps of
 // a block are shared by twice the columns): both operands are read MN-major from the row-major blocks that
-// TMA brings (their rows are the contraction). N covers the high and the
-// remainder parts of up to 64 rank rows; the epilogue adds the two. A block
+// TMA brings (their rows are the contraction). N covers the three parts of Q
+// (bf16) or the four of H (f16) of up to 64 rank rows, side by side; the
+// epilogue adds them, each times its unit, smallest first. A block
 // that ends inside its adapter's rows is loaded up to the next multiple of 16
 // rows, which may be another request's: a warp of its own writes zeros over
 // those before the MMA reads them (a product with zero would let an inf or NaN
@@ -359,11 +385,11 @@ struct OuterJob {
 };
 struct OuterArgs {
   OuterJob job[2];
-  int rank, nchunks, ntiles, ucols, rgroups, nmma, stages;
+  int rank, nchunks, ntiles, qstep, rgroups, nmma, stages, naccs;  // qstep: columns from one box of Q to the next
   uint32_t q_bytes, tmem_cols;
   const int4* chunks;  // row0, rows, adapter
   const int32_t* chunk_ptr;
-  float* part;         // [runs, 2, nmma / 2, 256]
+  float* part;         // [runs, 2, rank rows of a tile, 256]
 };
 
 struct OuterTile {
@@ -377,6 +403,16 @@ struct OuterTile {
     xblocks = min(BC / 64, (args.job[job].C - c0 + 63) / 64);
     halves = xblocks > 2 ? 2 : 1;
   }
+};
+
+template <typename T> struct OuterParts;  // how Q is held beside an X of type T
+template <> struct OuterParts<__nv_bfloat16> {
+  static constexpr int n = kQParts;
+  __device__ static float unit(int) { return 1.f; }
+};
+template <> struct OuterParts<__half> {
+  static constexpr int n = kHParts;
+  __device__ static float unit(int k) { return k == 0 ? 0x1p19f : k == 1 ? 0x1p8f : k == 2 ? 0x1p-3f : 0x1p-14f; }
 };
 
 template <typename T>
@@ -440,7 +476,7 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
           }
 #pragma unroll 1
           for (int b = 0; b < qblocks; b++)
-            tma_load_2d(st + XC_BYTES + b * 8192 + i * 2048, mq, &full[stage], b * (args.ucols / 2) + j0, ch.x + 16 * i);
+            tma_load_2d(st + XC_BYTES + b * 8192 + i * 2048, mq, &full[stage], b * args.qstep + j0, ch.x + 16 * i);
         }
         used |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
@@ -491,7 +527,7 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
         tc_commit(&tfull[acc]);
         last = &tfull[acc];
         last_phase = acc_phase;
-        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        if (++acc == args.naccs) { acc = 0; acc_phase ^= 1; }
       }
       if (last) {
         const uint64_t t0 = gtimer();
@@ -529,7 +565,8 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
     __syncwarp();
   } else {
     const int quarter = warp & 3;
-    const int nh = args.nmma / 2;  // rank rows of a tile, rounded up
+    constexpr int NP = OuterParts<T>::n;
+    const int nh = args.nmma / NP;  // rank rows of a tile, rounded up
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int64_t f = lo; f < hi;) {
@@ -549,17 +586,19 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
         const int col = col0 + 128 * h;
         const uint32_t tb = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((acc * 2 + h) * args.nmma);
         for (int j = 0; j < nh; j += 16) {
-          uint32_t vh[16], vl[16];
-          tmem_ld16(tb + j, vh);
-          tmem_ld16(tb + nh + j, vl);
+          uint32_t v[NP][16];
+#pragma unroll
+          for (int k = 0; k < NP; k++) tmem_ld16(tb + k * nh + j, v[k]);
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             const int row = j0 + j + i;
             if (row < args.rank && col < job.C) {
-              const float v = __uint_as_float(vh[i]) + __uint_as_float(vl[i]);
-              if (whole) dP[a * size + (int64_t)row * job.C + col] = TcFmt<T>::cvt(v);
-              else part[(j + i) * BC + 128 * h] = v;
+              float sum = OuterParts<T>::unit(NP - 1) * __uint_as_float(v[NP - 1][i]);
+#pragma unroll
+              for (int k = NP - 2; k >= 0; k--) sum = fmaf(OuterParts<T>::unit(k), __uint_as_float(v[k][i]), sum);
+              if (whole) dP[a * size + (int64_t)row * job.C + col] = TcFmt<T>::cvt(sum);
+              else part[(j + i) * BC + 128 * h] = sum;
             }
           }
         }
@@ -567,7 +606,7 @@ __global__ void __launch_bounds__(OUTER_THREADS, 1) k_outer_tc(const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      if (++acc == args.naccs) { acc = 0; acc_phase ^= 1; }
     }
   }
   if (threadIdx.x == 0 && *abort) {
@@ -636,8 +675,7 @@ void shrink_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStrea
   a.T = p.rows;
   a.ntiles = (p.rows + BM - 1) / BM;
   a.rank = c[0].rank;
-  a.ucols = adapter_u_cols(a.rank);
-  a.R = a.ucols / 2;
+  a.R = adapter_rank_rows(a.rank);
   // adapters side by side: 128 columns of D, 192 for rank 64 (a ragged tile of
   // 128 rows meets two or three requests), which leaves five stages or more
   a.nb = a.R <= 32 ? 64 / a.R : a.R == 64 ? 2 : 1;
@@ -653,6 +691,7 @@ void shrink_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStrea
     a.job[j].tmX = a.job[j].blocks ? tensor_map_blocks(q.X, p.rows, q.C, q.ld, 2, BM, dtype) : tensor_map_2d(q.X, p.rows, q.C, q.ld, BK, BM, dtype);
     a.job[j].tmP = tensor_map_3d(q.P, q.n, q.rank, q.C, q.ldp, a.R, dtype);
     a.job[j].Q = q.Q;
+    a.job[j].H = q.H;
     a.job[j].C = (int)q.C;
     KB = std::min(KB, (a.job[j].C + SK - 1) / SK);
   }
@@ -703,7 +742,7 @@ struct OuterRuns {
   int ntiles = 0, runs = 0;
   int64_t total = 0;
   OuterRuns(const AdapterOuter* c, int njobs, const AdapterPlan& p) {
-    for (int j = 0; j < njobs; j++) ntiles += (int)((c[j].C + BC - 1) / BC) * std::max(1, adapter_u_cols(c[j].rank) / 128);
+    for (int j = 0; j < njobs; j++) ntiles += (int)((c[j].C + BC - 1) / BC) * std::max(1, adapter_rank_rows(c[j].rank) / 64);
     total = (int64_t)ntiles * p.nchunks;
     runs = (int)std::min<int64_t>(std::min(num_sms(), kMaxRuns), total);
   }
@@ -715,12 +754,16 @@ void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p
   OuterArgs a{};
   a.rank = c[0].rank;
   a.nchunks = p.nchunks;
-  a.ucols = adapter_u_cols(a.rank);
-  a.rgroups = std::max(1, a.ucols / 128);
-  a.nmma = std::min(a.ucols, 128);
-  a.q_bytes = a.ucols > 64 ? 16384 : 8192;
-  a.stages = a.q_bytes > 8192 ? 4 : 5;
-  a.tmem_cols = tmem_columns(4 * a.nmma);
+  constexpr int NP = OuterParts<T>::n;
+  const int R = adapter_rank_rows(a.rank), nh = std::min(R, 64), qcols = NP * R;
+  a.rgroups = std::max(1, R / 64);
+  a.nmma = NP * nh;
+  a.qstep = std::max(R, 64);
+  a.q_bytes = (uint32_t)((a.nmma + 63) / 64 * 8192);
+  a.stages = std::min(5, (int)((224u << 10) / (XC_BYTES + a.q_bytes)));
+  // two accumulators, each of two halves of the columns, where TMEM's 512 columns hold them (up to 32 rank rows)
+  a.naccs = 4 * a.nmma <= 512 ? 2 : 1;
+  a.tmem_cols = tmem_columns(2 * a.naccs * a.nmma);
   a.chunks = p.chunks;
   a.chunk_ptr = p.chunk_ptr;
   const OuterRuns runs(c, njobs, p);
@@ -734,10 +777,10 @@ void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p
     o.whole = c[j].C % 64 == 0 ? (int)std::min<int64_t>(BC, c[j].C) / 64 : 0;
     o.tmX = o.whole ? tensor_map_blocks(c[j].X, p.rows, c[j].C, c[j].ld, o.whole, 64, dtype)
                     : tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 64, dtype);
-    o.tmQ = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 64, dtype);
+    o.tmQ = tensor_map_2d(c[j].parts, p.rows, qcols, qcols, 64, 64, dtype);
     o.tmX16 = o.whole ? tensor_map_blocks(c[j].X, p.rows, c[j].C, c[j].ld, o.whole, 16, dtype)
                       : tensor_map_2d(c[j].X, p.rows, c[j].C, c[j].ld, 64, 16, dtype);
-    o.tmQ16 = tensor_map_2d(c[j].Q, p.rows, a.ucols, a.ucols, 64, 16, dtype);
+    o.tmQ16 = tensor_map_2d(c[j].parts, p.rows, qcols, qcols, 64, 16, dtype);
     o.dP = c[j].dP;
   }
   const size_t smem = (size_t)a.stages * (XC_BYTES + a.q_bytes) + 1024 + 512;
@@ -769,7 +812,7 @@ void outer_t(const AdapterOuter* c, int njobs, float* part, const AdapterPlan& p
   join.rgroups = a.rgroups;
   join.njobs = njobs;
   join.ctiles0 = a.job[0].ctiles;
-  join.nh = a.nmma / 2;
+  join.nh = nh;
   join.part = part;
   for (int j = 0; j < njobs; j++) {
     join.dP[j] = a.job[j].dP;
@@ -790,7 +833,7 @@ void adapter_shrink_tc(const AdapterShrink* c, int njobs, const AdapterPlan& p, 
 
 size_t adapter_part_bytes(const AdapterOuter* c, int njobs, const AdapterPlan& p) {
   const OuterRuns runs(c, njobs, p);
-  return (size_t)runs.runs * 2 * (std::min(adapter_u_cols(c[0].rank), 128) / 2) * BC * 4;
+  return (size_t)runs.runs * 2 * std::min(adapter_rank_rows(c[0].rank), 64) * BC * 4;
 }
 
 void adapter_outer_tc(const AdapterOuter* c, int njobs, void* part, const AdapterPlan& p, int dtype, cudaStream_t st) {

@@ -61,37 +61,47 @@ struct GemmPlain {
   static constexpr int kb_off = 0;
 };
 // The adapters' share of a projection: for each segment of rows [lo, hi) with
-// adapter a that meets the tile, D[rows] += U·P_a, U [M, 64·nchunks] and P_a
-// [r, N]. U rides as the A operand (the tile's rows, 64 columns per block of
-// the ring) and P_a, whose rows run along N, as an MN-major B operand; the MMA
-// leaves the rows outside the segment alone (TMEM lanes switched off), so a
-// row never meets another request's adapter, not even multiplied by zero.
-// U holds each value as a 16-bit high part and the 16-bit remainder, which
-// meet the same rows of P_a: the sum is as exact as an f32 u, for another two
-// MMA steps per request (rank 16) where one tile of 768 columns in takes 48.
+// adapter a that meets the tile, D[rows] += U·P_a, U [M, 3·R] and P_a [r, N].
+// U rides as the A operand (the tile's rows, 64 columns per block of the ring)
+// and P_a, whose rows run along N, as an MN-major B operand; the MMA leaves the
+// rows outside the segment alone (TMEM lanes switched off), so a row never
+// meets another request's adapter, not even multiplied by zero.
+// U holds each value as three bf16 parts (24 bits), which meet the same rows of
+// P_a: the sum is that of an f32 u, for three MMA steps per request (rank 16)
+// where one tile of 768 columns in takes 48. An f16 bank comes as two bf16
+// parts and the products that count are five (the third part of u times the
+// remainders of P is below f32's rounding); f16 parts of u would end at 2^-25
+// and at 131,008. The MMAs of both types accumulate in the same f32 columns.
 // Bound by the projection: 69,135 rows, 768 -> 2304 in f16 take 197 us without
-// adapters, 207 with those of 256 requests (U given); adding the share in a
-// kernel of its own would read and write y (318 MB) once more, ~95 us.
+// adapters; adding the share in a kernel of its own would read and write y
+// (318 MB) once more, ~95 us.
 // WT: the shared projection is read transposed, D = X·W for W [K, N] (the
 // gradient with respect to the input): an MN-major B operand as well.
 template <bool WT>
 struct GemmAdapted {
   static constexpr bool kOn = true, kWT = WT;
   CUtensorMap tmU, tmP;
-  const int4* segs;           // lo, hi, adapter
+  const int4* segs;           // lo, hi, adapter, its place among those used
   const int2* tiles;          // per 128 rows: the first segment that meets them, and how many do
-  int nchunks;                // 64-column blocks of U
-  int ksteps;                 // 16-column steps used per block
-  int half;                   // steps after which P's rows start over (high and low part in one block), else ksteps
-  int pgroups;                // 64-row blocks of P_a
+  int by_place;               // the bank holds the used adapters only
+  int R16, parts;             // R / 16; parts of P
+  int uchunks;                // 64-column blocks of U
+  int nchunks;                // pairs of a block of U and one of P per segment
+  int groups;                 // 64-row blocks of a part of P_a (1 below 64 rows, where one block holds all parts)
+  // MMA steps of the first pair and of the others: 4 bits each, 16 columns of the block of U | 16 rows of P's << 2
+  uint32_t steps[2];
+  int nsteps[2];
   int prows;                  // rows of P_a per block (box height of tmP)
-  int per;                    // segments whose blocks of P share a stage (64 / prows; 1 with several blocks of U)
+  int per;                    // segments whose blocks of P share a stage (64 / prows)
   int defer;                  // x, w and bias were complete when the previous kernel let this one start: only U waits for it
   // Single-CTA kernel: a tile's U (two blocks at most) stays in shared memory
-  // and stages hold blocks of P alone, 2·per requests to a stage: 500 rows in
-  // 250 requests, 768 -> 2304 in bf16, 77 -> 44 us at rank 40, 28 -> 25 at 16.
+  // and stages hold blocks of P alone, 2·per to a stage (500 rows in 250
+  // requests, 768 -> 2304 in bf16, rank 16: 28 -> 25 us).
   int resident;
   int kb_off;                 // added to the K block of the main loop's loads (past the operands' end: zeros)
+  __device__ int u_block(int c) const { return c % uchunks; }
+  __device__ int p_row(int c) const { return (c / uchunks * groups + c % groups) * 64; }
+  __device__ int place(const int4& seg) const { return by_place ? seg.w : seg.z; }
 };
 
 // The segments [x, y) that meet the tile of `rows` (128 or 256) rows from m0.
@@ -1090,8 +1100,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           const int2 sg = tile_segments(ex, m0, BM, args.M);
           if (ex.resident && sg.x < sg.y) {
             if (!mbar_wait(ufree, u_phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
-            mbar_arrive_expect_tx(ufull, ex.nchunks * A_BYTES);
-            for (int c = 0; c < ex.nchunks; c++) tma_load_2d(sU + c * A_BYTES, &ex.tmU, ufull, c * 64, m0);
+            mbar_arrive_expect_tx(ufull, ex.uchunks * A_BYTES);
+            for (int c = 0; c < ex.uchunks; c++) tma_load_2d(sU + c * A_BYTES, &ex.tmU, ufull, c * 64, m0);
             u_issued = true;
             u_phase ^= 1;
             for (int s = sg.x; s < sg.y; s += 2 * ex.per) {
@@ -1100,7 +1110,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
               mbar_arrive_expect_tx(&full[stage], n * (BN / 64) * ex.prows * 128);
 #pragma unroll 1
               for (int i = 0; i < n; i++) {
-                const int a = __ldg(&ex.segs[s + i].z);
+                const int a = ex.place(__ldg(ex.segs + s + i));
                 uint8_t* dst = i < ex.per ? sA + stage * A_BYTES : sB + stage * B_BYTES - ex.per * (BN / 64) * ex.prows * 128;
                 for (int h = 0; h < BN / 64; h++) tma_load_3d(dst + (i * (BN / 64) + h) * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, 0, a);
               }
@@ -1115,12 +1125,12 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
               const int n = min(ex.per, sg.y - s);
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
               mbar_arrive_expect_tx(&full[stage], A_BYTES + n * (BN / 64) * ex.prows * 128);
-              tma_load_2d(sA + stage * A_BYTES, &ex.tmU, &full[stage], c * 64, m0);
+              tma_load_2d(sA + stage * A_BYTES, &ex.tmU, &full[stage], ex.u_block(c) * 64, m0);
 #pragma unroll 1
               for (int i = 0; i < n; i++) {
-                const int a = __ldg(&ex.segs[s + i].z);
+                const int a = ex.place(__ldg(ex.segs + s + i));
                 for (int h = 0; h < BN / 64; h++)
-                  tma_load_3d(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, (c % ex.pgroups) * 64, a);
+                  tma_load_3d(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, ex.p_row(c), a);
               }
               issued[stage] = 1;
               iss_phase[stage] = phase;
@@ -1148,7 +1158,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
     // ---------------- MMA issuer
     if (lane == 0) {
       const uint32_t idesc = idesc_f16<T, BN>();
-      [[maybe_unused]] const uint32_t idesc_t = idesc_f16<T, BN, 128, true>();
+      [[maybe_unused]] const uint32_t idesc_t = idesc_f16<T, BN, 128, true>(), idesc_u = idesc_f16<__nv_bfloat16, BN, 128, true>();
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -1186,7 +1196,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           if (ex.resident && sg.x < sg.y) {
             if (!mbar_wait(ufull, u_phase, abort, &g_gemm_err)) { ok = false; break; }
             u_phase ^= 1;
-            const uint32_t high = smem_u32(sU), low = ex.nchunks == 1 ? high + ex.prows * 2 : high + A_BYTES;
+            const uint32_t u0 = smem_u32(sU);
             for (int s = sg.x; s < sg.y; s += 2 * ex.per) {
               const int n = min(2 * ex.per, sg.y - s);
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
@@ -1199,10 +1209,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
                 for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
                 const uint32_t p = (i < ex.per ? smem_u32(sA + stage * A_BYTES) : smem_u32(sB + stage * B_BYTES) - ex.per * (BN / 64) * ex.prows * 128) +
                                    i * (BN / 64) * ex.prows * 128;
-                for (int k = 0; k < ex.prows / 16; k++) {
+                for (int k = 0; k < ex.parts * ex.R16; k++) {  // 16 rows of P: values, then remainders
                   const uint64_t pd = sdesc_sw128_mn(p + k * 2048, ex.prows * 128);
-                  tc_mma_lanes(d, sdesc_sw128(high + k * 32), pd, idesc_t, 1u, off);
-                  tc_mma_lanes(d, sdesc_sw128(low + k * 32), pd, idesc_t, 1u, off);
+                  for (int b = k < ex.R16 ? k : k - ex.R16; b < (k < ex.R16 ? 3 : 2) * ex.R16; b += ex.R16)
+                    tc_mma_lanes(d, sdesc_sw128(u0 + (b >> 2) * A_BYTES + (b & 3) * 32), pd, idesc_u, 1u, off);
                 }
               }
               tc_commit(&empty[stage]);
@@ -1225,9 +1235,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
                 uint32_t off[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
-                for (int k = 0; k < ex.ksteps; k++)
-                  tc_mma_lanes(d, sdesc_sw128(a0 + k * 32), sdesc_sw128_mn(b0 + i * ex.prows * 128 + (k >= ex.half ? k - ex.half : k) * 2048, 8192),
-                               idesc_t, 1u, off);
+                uint32_t w = ex.steps[c > 0];
+                for (int k = ex.nsteps[c > 0]; k > 0; k--, w >>= 4)
+                  tc_mma_lanes(d, sdesc_sw128(a0 + (w & 3) * 32), sdesc_sw128_mn(b0 + i * ex.prows * 128 + (w >> 2 & 3) * 2048, 8192), idesc_u, 1u, off);
               }
               tc_commit(&empty[stage]);
               last = &empty[stage];
@@ -1504,13 +1514,13 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
               const int n = min(ex.per, sg.y - s);
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
               if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (A_BYTES + n * 2 * ex.prows * 128));
-              tma_load_2d_pair(sA + stage * A_BYTES, &ex.tmU, full0 + 8 * stage, c * 64, m0);
+              tma_load_2d_pair(sA + stage * A_BYTES, &ex.tmU, full0 + 8 * stage, ex.u_block(c) * 64, m0);
 #pragma unroll 1
               for (int i = 0; i < n; i++) {
-                const int a = __ldg(&ex.segs[s + i].z);
+                const int a = ex.place(__ldg(ex.segs + s + i));
                 for (int h = 0; h < 2; h++)
                   tma_load_3d_pair(sB + stage * B_BYTES + h * 8192 + i * ex.prows * 128, &ex.tmP, full0 + 8 * stage, n0 + 64 * h,
-                                   (c % ex.pgroups) * 64, a);
+                                   ex.p_row(c), a);
               }
               issued[stage] = 1;
               iss_phase[stage] = phase;
@@ -1532,7 +1542,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = idesc_f16<T, BN, 256>();
       const uint64_t dA0 = sdesc_sw128(smem_u32(sA)), dB0 = sdesc_sw128(smem_u32(sB));
-      [[maybe_unused]] const uint32_t idesc_t = idesc_f16<T, BN, 256, true>();
+      [[maybe_unused]] const uint32_t idesc_t = idesc_f16<T, BN, 256, true>(), idesc_u = idesc_f16<__nv_bfloat16, BN, 256, true>();
       [[maybe_unused]] const uint64_t dBt0 = sdesc_sw128_mn(smem_u32(sB), 8192);
       int stage = 0;
       uint32_t phase = 0;
@@ -1575,8 +1585,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
                 uint32_t off[8];
 #pragma unroll
                 for (int q = 0; q < 8; q++) off[q] = lanes_off(t0 + 32 * q, seg.x, seg.y);
-                for (int k = 0; k < ex.ksteps; k++)
-                  tc_mma_pair_lanes(d, da + k * 2, db + i * ex.prows * 8 + (k >= ex.half ? k - ex.half : k) * 128, idesc_t, 1u, off);
+                uint32_t w = ex.steps[c > 0];
+                for (int k = ex.nsteps[c > 0]; k > 0; k--, w >>= 4)
+                  tc_mma_pair_lanes(d, da + (w & 3) * 2, db + i * ex.prows * 8 + (w >> 2 & 3) * 128, idesc_u, 1u, off);
               }
               tc_commit_pair(&empty[stage]);
               last = &empty[stage];
@@ -1929,17 +1940,27 @@ void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
   a.ksplit = 1;
   GemmAdapted<WT> ex{};
   const AdapterShare& s = c.share;
-  ex.tmU = tensor_map(s.u, c.M, s.u_cols, s.u_cols, 64, BM, dtype);
-  ex.prows = std::min(64, s.u_cols / 2);  // rows past the rank arrive as zeros
-  ex.tmP = tensor_map_stack(s.bank, std::max(1, s.n), s.rank, c.N, s.ld, ex.prows, dtype);
+  const int R = s.R;
+  ex.tmU = tensor_map(s.u, c.M, 3 * R, 3 * R, 64, BM, LC_BF16);
+  ex.prows = std::min(64, s.parts * R);  // rows past the rank arrive as zeros
+  // (without segments no block of P is read, and there may be no bank)
+  ex.tmP = s.nsegs ? tensor_map_stack(s.bank, s.n, s.rows, c.N, s.ld, ex.prows, LC_BF16) : tensor_map_stack(s.u, 1, 1, 8, 8, ex.prows, LC_BF16);
   ex.segs = s.segs;
   ex.tiles = s.tiles;
-  ex.nchunks = (s.u_cols + 63) / 64;
-  ex.ksteps = std::min(4, s.u_cols / 16);
-  ex.half = s.u_cols <= 64 ? s.u_cols / 32 : 4;
-  ex.pgroups = std::max(1, s.u_cols / 128);
+  ex.by_place = s.parts == 2;
+  ex.R16 = R / 16;
+  ex.parts = s.parts;
+  ex.groups = std::max(1, R / 64);
+  ex.uchunks = (3 * R + 63) / 64;
+  ex.nchunks = R < 64 || s.parts == 1 ? ex.uchunks : 5 * ex.groups;
+  const uint32_t all = s.parts == 1 ? 0u : ~0u;  // (the second part's steps, if it is there)
+  if (R == 16) ex.steps[0] = 0x210 | (all & 0x54000), ex.nsteps[0] = s.parts == 1 ? 3 : 5;
+  else if (R == 32) ex.steps[0] = 0x7250 | (all & 0xfad80000), ex.nsteps[0] = s.parts == 1 ? 4 : 8;
+  else ex.steps[0] = 0xfa50, ex.nsteps[0] = 4;
+  ex.steps[1] = R == 32 ? 0x50 : 0xfa50;
+  ex.nsteps[1] = R == 32 ? 2 : 4;
   ex.per = 64 / ex.prows;
-  ex.resident = s.u_cols <= 128;
+  ex.resident = R <= 32;
   ex.defer = c.after_share ? 1 : 0;
   ex.kb_off = c.w ? 0 : 1;  // a block past the end of the stand-in maps below, which TMA fills with zeros
   const CUtensorMap ma = c.w ? tensor_map(c.x, c.M, c.K, c.ldx, BK, BM, dtype) : tensor_map(s.u, 1, 8, 8, BK, BM, dtype);

@@ -51,14 +51,18 @@ struct GemmQuantB {
   const float* gamma = nullptr;  // optional column scale [K] (a folded LayerNorm weight)
 };
 
-// The adapters' share that gemm_adapted adds to a projection.
+// The adapters' share that gemm_adapted adds to a projection: bf16 parts of u
+// against bf16 parts of the bank, whatever the projection's own type.
 struct AdapterShare {
-  const void* u = nullptr;     // [M, u_cols] 16-bit: high parts (u_cols / 2), then the remainders
-  int u_cols = 0;              // 32, 64 or a multiple of 128
-  const void* bank = nullptr;  // [n, rank, ld] 16-bit, ld % 8 == 0
-  int n = 0, rank = 0;
+  const void* u = nullptr;     // bf16 [M, 3·R]: values, remainders, remainders of those
+  int R = 0;                   // the rank rounded up: 16, 32 or a multiple of 64
+  const void* bank = nullptr;  // bf16 [n, rows, ld], ld % 8 == 0
+  int parts = 1;               // 1: rank rows, an adapter's place is its number; 2: R rows of values and R of remainders,
+                               // an adapter's place is the segment's fourth entry
+  int n = 0, rows = 0;
   int64_t ld = 0;
-  const int4* segs = nullptr;  // row ranges with an adapter, ascending: lo, hi, adapter
+  int nsegs = 0;
+  const int4* segs = nullptr;  // row ranges with an adapter, ascending: lo, hi, adapter, its place among those used
   const int2* tiles = nullptr;  // per 128 rows: the first segment that meets them, and how many do
 };
 // y[M, N] = x·wᵀ for w [N, K], or x·w for w [K, N] (transposed), plus bias and
