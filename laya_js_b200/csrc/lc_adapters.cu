@@ -350,92 +350,74 @@ struct Rows {
 };
 
 // Copies rows of `cols` values into rows of `ld` (a multiple of 8), zeros after
-// them, eight values per thread step, up to six matrices a launch, the steps
-// of all of them in one range. Bound by the latency of the 2-byte loads (1537
-// x 1001, 777 x 1001 and two banks: 3.9 us; matrix after matrix 4.4).
-// R > 0: an f16 bank [n, rank, cols] as bf16 values and remainders, [used
-// adapters, 2·R, ld] with zeros from the rank on: the 11 bits of an f16 as two
-// bf16, which the tensor cores multiply with the bf16 parts of u (lc_gemm.cu).
+// them, eight values per thread step, up to five matrices a launch, the steps
+// of all of them in one range, and after them those of a bank's split. Bound by
+// the latency of the 2-byte loads (1537 x 1001, 777 x 1001 and two banks: 3.9
+// us; matrix after matrix 4.4).
 struct PadJob {
   const uint16_t* src;
   uint16_t* dst;
   int64_t first, cols, ld;  // first: steps of the matrices before it
-  int rank, R, vec;         // vec: the source rows are 16-byte aligned
-  const int32_t* used;
 };
 struct PadJobs {
   int n;
   int64_t total;
-  PadJob j[6];
+  PadJob j[5];
+  BankSplit split;
 };
 __global__ void __launch_bounds__(256) k_pad_rows(const __grid_constant__ PadJobs jobs) {
   pdl_trigger();
   pdl_wait();
-  LC_GRID_STRIDE(g, jobs.total) {
+  LC_GRID_STRIDE(g, jobs.total + jobs.split.steps) {
+    if (g >= jobs.total) {
+      split_bank_step(jobs.split, g - jobs.total);
+      continue;
+    }
     int k = jobs.n - 1;
     while (g < jobs.j[k].first) k--;
     const PadJob& j = jobs.j[k];
     const int64_t i = g - j.first, vecs = j.ld / 8, row = i / vecs, c = (i % vecs) * 8;
-    int64_t from = row, to = row;
-    bool live = true;
-    if (j.R) {
-      const int64_t slot = row / j.R, r = row % j.R;
-      live = r < j.rank;
-      from = __ldg(j.used + slot) * (int64_t)j.rank + r;
-      to = slot * 2 * j.R + r;
-    }
-    const uint16_t* s = j.src + from * j.cols + c;
-    alignas(16) uint16_t v[8] = {};
-    if (live && j.vec) {
-      *(uint4*)v = __ldg((const uint4*)s);
-    } else if (live) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = c + e < j.cols ? s[e] : (uint16_t)0;
-    }
-    uint4* d = (uint4*)(j.dst + to * j.ld + c);
-    if (!j.R) {
-      *d = *(const uint4*)v;
-      continue;
-    }
-    alignas(16) __nv_bfloat16 high[8], low[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float f = __half2float(__ushort_as_half(v[e]));
-      high[e] = __float2bfloat16_rn(f);
-      low[e] = __float2bfloat16_rn(isfinite(f) ? f - __bfloat162float(high[e]) : 0.f);
-    }
-    *d = *(const uint4*)high;
-    d[j.R * j.ld / 8] = *(const uint4*)low;
+    *(uint4*)(j.dst + row * j.ld + c) = row_values8(j.src + row * j.cols, j.cols, c, false);
   }
 }
 
 struct Padder {
   Held& held;
   PadJobs jobs{};
-  void add(const LcTensor* t, void* d, int64_t steps, int64_t cols, int64_t ld, int rank, int R, const int32_t* used) {
-    jobs.j[jobs.n++] = {(const uint16_t*)t->data(), (uint16_t*)d, jobs.total, cols, ld, rank, R, cols % 8 == 0 && ((uintptr_t)t->data() & 15) == 0, used};
-    jobs.total += steps;
-  }
+  BankSplit split{};
+  static bool aligned(const LcTensor* t, int64_t cols) { return cols % 8 == 0 && ((uintptr_t)t->data() & 15) == 0; }
   Rows of(const LcTensor* t, int64_t rows, int64_t cols) {
     if (!t) return {};
-    if (cols % 8 == 0 && ((uintptr_t)t->data() & 15) == 0) return {t->data(), cols};
+    if (aligned(t, cols)) return {t->data(), cols};
     const int64_t ld = (cols + 7) / 8 * 8;
     void* d = held.scratch((size_t)(rows * ld) * 2);
-    add(t, d, rows * ld / 8, cols, ld, 0, 0, nullptr);
+    jobs.j[jobs.n++] = {(const uint16_t*)t->data(), (uint16_t*)d, jobs.total, cols, ld};
+    jobs.total += rows * ld / 8;
     return {d, ld};
   }
   // The bank beside a projection on the tensor cores: bf16 rows, or those of an f16 bank's used adapters in two parts.
   Rows share(const LcTensor* bank, const AdapterPlan& p, int rank, int64_t cols) {
     if (bank->dtype == LC_BF16) return of(bank, bank->shape[0] * rank, cols);
-    const int64_t ld = (cols + 7) / 8 * 8, rows = (int64_t)p.nused * adapter_rank_rows(rank);
-    void* d = held.scratch((size_t)(2 * rows * ld) * 2);
-    add(bank, d, rows * ld / 8, cols, ld, rank, adapter_rank_rows(rank), p.used);
-    return {d, ld};
+    split.ld = (cols + 7) / 8 * 8;
+    split.cols = cols;
+    split.rank = rank;
+    split.R = adapter_rank_rows(rank);
+    split.vec = aligned(bank, cols);
+    split.used = p.used;
+    split.src = (const uint16_t*)bank->data();
+    const int64_t rows = (int64_t)p.nused * split.R;
+    split.dst = (uint16_t*)held.scratch((size_t)(2 * rows * split.ld) * 2);
+    split.steps = rows * split.ld / 8;
+    return {split.dst, split.ld};
   }
-  // true when a kernel was launched: the next one may start while it runs, and waits for it
-  bool run() {
-    if (!jobs.total) return false;
-    launch_chain(k_pad_rows, dim3(blocks_for(jobs.total, 256)), dim3(256), 0, stream(), jobs);
+  // Launches the copies, with the split among them unless it may ride with the shrink and there is nothing else to do
+  // (128 rows of f16 through 768 -> 2304: 2.2 us for a launch of its own). True when a kernel was launched: the next one
+  // may start while it runs, and waits for it.
+  bool run(bool split_may_ride) {
+    if (!split_may_ride || jobs.total) std::swap(jobs.split, split);
+    const int64_t steps = jobs.total + jobs.split.steps;
+    if (!steps) return false;
+    launch_chain(k_pad_rows, dim3(blocks_for(steps, 256)), dim3(256), 0, stream(), jobs);
     LC_LAUNCHED(1);
     return true;
   }
@@ -469,9 +451,12 @@ AdapterShrink shrink_job(const Operands& o, const Rows& X, const Rows& P, int64_
   return c;
 }
 
-void shrink(const AdapterShrink* c, int njobs, const Operands& o, bool padded) {
-  std::unique_ptr<PdlScope> chained = padded ? std::make_unique<PdlScope>() : nullptr;
-  if (!adapter_shrink_rows(c, njobs, *o.plan, o.dtype, stream())) adapter_shrink_tc(c, njobs, *o.plan, o.dtype, stream());
+// The copies and the narrow products.
+void shrink(const AdapterShrink* c, int njobs, const Operands& o, Padder& pad) {
+  const bool few = adapter_shrink_rows_fit(c, njobs, *o.plan);
+  std::unique_ptr<PdlScope> chained = pad.run(few) ? std::make_unique<PdlScope>() : nullptr;
+  if (few) adapter_shrink_rows(c, njobs, pad.split, *o.plan, o.dtype, stream());
+  else adapter_shrink_tc(c, njobs, *o.plan, o.dtype, stream());
 }
 
 // y, or dx (transposed). `few`: the dot-product form, whose bank is in the operands' type; otherwise `bank` is Padder::share's.
@@ -518,9 +503,8 @@ void linear(const Operands& o, LcTensor* y, Held& held) {
   Padder pad{held};
   const Rows x = pad.of(o.x, o.T, o.K), w = pad.of(o.w, o.N, o.K), a = pad.of(o.a, (int64_t)o.n * o.r, o.K),
              b = few ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : pad.share(o.b, *o.plan, o.r, o.N);
-  const bool padded = pad.run();
   const AdapterShrink u = shrink_job(o, x, a, o.K, held.scratch(parts_bytes(o, kQParts)), nullptr);
-  shrink(&u, 1, o, padded);
+  shrink(&u, 1, o, pad);
   const Chained chained(o);
   expand_16(o, x, w, b, u.Q, false, few, y);
 }
@@ -550,7 +534,6 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
   const Rows dy = pad.of(o.dy, o.T, o.N), x = da || db ? pad.of(o.x, o.T, o.K) : Rows{}, w = dx ? pad.of(o.w, o.N, o.K) : Rows{},
              a = db || (dx && !f16) ? pad.of(o.a, (int64_t)o.n * o.r, o.K) : Rows{},
              b = dx || da ? pad.of(o.b, (int64_t)o.n * o.r, o.N) : Rows{}, bank = dx && f16 ? pad.share(o.a, *o.plan, o.r, o.K) : a;
-  const bool padded = pad.run();
   AdapterOuter out[2];
   int no = 0;
   auto job = [&](const Rows& X, int64_t C, LcTensor* dP) {
@@ -583,7 +566,7 @@ void gradients(const Operands& o, LcTensor* dx, LcTensor* da, LcTensor* db, Held
   }
   if (dx || da) q[nq++] = shrink_job(o, dy, b, o.N, gq ? scratch + gq_at : nullptr, gh ? scratch + gh_at : nullptr);
   if (da) out[no - 1].parts = scratch + (f16 ? gh_at : gq_at);
-  shrink(q, nq, o, padded);
+  shrink(q, nq, o, pad);
   const Chained chained(o);
   if (no) adapter_outer_tc(out, no, scratch + at, *o.plan, o.dtype, stream());
   if (dx) expand_16(o, dy, w, bank, scratch + gq_at, true, false, dx);

@@ -76,6 +76,40 @@ __device__ __forceinline__ void split_f16(float v, __half (&h)[kHParts]) {
   if (!in) h[0] = __float2half_rn(isnan(v) ? v : copysignf(INFINITY, v));
 }
 
+// The rows of an f16 bank [n, rank, cols] that a batch uses, as bf16 values and
+// remainders [used adapters, 2·R, ld] with zeros from the rank on: the 11 bits
+// of an f16 as two bf16, which the tensor cores multiply with the bf16 parts of
+// u (lc_gemm.cu). Eight values of a row per step.
+struct BankSplit {
+  const uint16_t* src = nullptr;
+  uint16_t* dst = nullptr;
+  const int32_t* used = nullptr;
+  int64_t cols = 0, ld = 0, steps = 0;
+  int rank = 0, R = 0, vec = 0;  // vec: the source rows are 16-byte aligned
+};
+// Values c .. c + 7 of a row of `cols`, zeros from its end on.
+__device__ __forceinline__ uint4 row_values8(const uint16_t* row, int64_t cols, int64_t c, bool vec) {
+  if (vec) return __ldg((const uint4*)(row + c));
+  alignas(16) uint16_t v[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = c + e < cols ? row[c + e] : (uint16_t)0;
+  return *(const uint4*)v;
+}
+__device__ __forceinline__ void split_bank_step(const BankSplit& b, int64_t i) {
+  const int64_t vecs = b.ld / 8, row = i / vecs, c = (i % vecs) * 8, slot = row / b.R, r = row % b.R;
+  const uint4 v = r < b.rank ? row_values8(b.src + (__ldg(b.used + slot) * (int64_t)b.rank + r) * b.cols, b.cols, c, b.vec) : make_uint4(0u, 0u, 0u, 0u);
+  alignas(16) __nv_bfloat16 high[8], low[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float f = __half2float(((const __half*)&v)[e]);
+    high[e] = __float2bfloat16_rn(f);
+    low[e] = __float2bfloat16_rn(isfinite(f) ? f - __bfloat162float(high[e]) : 0.f);
+  }
+  uint4* d = (uint4*)(b.dst + (slot * 2 * b.R + r) * b.ld + c);
+  *d = *(const uint4*)high;
+  d[b.R * vecs] = *(const uint4*)low;
+}
+
 // s_a·P_a·X[t] as Q and H (each may be null) for X [rows, C] and P [n, rank, C] (row strides ld, ldp: multiples of 8;
 // 16-byte aligned).
 struct AdapterShrink {
@@ -98,8 +132,8 @@ namespace lc {
 void adapter_shrink_tc(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
 size_t adapter_part_bytes(const AdapterOuter* c, int njobs, const AdapterPlan& p);  // f32 partial sums of adapter_outer_tc
 void adapter_outer_tc(const AdapterOuter* c, int njobs, void* part, const AdapterPlan& p, int dtype, cudaStream_t st);
-// The forms for few rows (lc_adapters_rows.cu): false, with nothing launched,
-// above so many multiplications. Measured (bf16, rank 16, 768 columns; dot
+// The forms for few rows (lc_adapters_rows.cu) fit up to so many
+// multiplications. Measured (bf16, rank 16, 768 columns; dot
 // products against tensor cores, one request / requests of 8 rows): shrink
 // 25 M 6.0 / 8.1 us against 8.3 / 16.4, 50 M 10.1 / 13.7 against 8.5 / 16.2;
 // linear 28 M 7.3 us against 9.4 / 9.7, 57 M 13.3 against 9.5 / 10.4. Twice
@@ -107,7 +141,9 @@ void adapter_outer_tc(const AdapterOuter* c, int njobs, void* part, const Adapte
 // rank 40 (66 M each) take 17 and 14 us against 25 and 44.
 constexpr int kRowsMost = 16384;
 constexpr int64_t kRowsShrinkMost = 3 << 24, kRowsLinearMost = 1 << 25;
-bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st);
+bool adapter_shrink_rows_fit(const AdapterShrink* c, int njobs, const AdapterPlan& p);
+// `split` (steps may be 0) rides along in blocks of its own.
+void adapter_shrink_rows(const AdapterShrink* c, int njobs, const BankSplit& split, const AdapterPlan& p, int dtype, cudaStream_t st);
 bool adapter_linear_rows_fit(int64_t M, int64_t N, int64_t K, const AdapterPlan& p);
 // The forward product for a call that fits; c.share.bank [n, rank, ld] is in `dtype` here.
 void adapter_linear_rows(const GemmAdaptedCall& c, const AdapterPlan& p, int rank, int dtype, cudaStream_t st);

@@ -97,17 +97,23 @@ struct RowsShrinkJob {
 };
 struct RowsShrinkArgs {
   RowsShrinkJob job[2];
-  int rank, R;
+  int rank, R, npieces;
   const int4* pieces;  // up to 8 rows of one adapter
   const float* scales;
+  BankSplit split;
 };
 
-// grid: (pieces, groups of 16 rank rows, jobs)
+// grid: (pieces and then blocks for the split, groups of 16 rank rows, jobs)
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1) k_shrink_rows(const __grid_constant__ RowsShrinkArgs args) {
   __shared__ float red[128];
   pdl_wait();
   pdl_trigger();  // after the wait: what runs before this kernel is done when the next one starts
+  if (blockIdx.x >= args.npieces) {  // the blocks beside the pieces, of every group and job, in one range
+    const int64_t nb = gridDim.x - args.npieces, b = blockIdx.x - args.npieces + nb * (blockIdx.y + (int64_t)gridDim.y * blockIdx.z);
+    for (int64_t i = b * THREADS + threadIdx.x; i < args.split.steps; i += nb * gridDim.y * gridDim.z * THREADS) split_bank_step(args.split, i);
+    return;
+  }
   const RowsShrinkJob& job = args.job[blockIdx.z];
   const int4 pc = __ldg(&args.pieces[blockIdx.x]);
   const int j0 = blockIdx.y * COLS;
@@ -177,14 +183,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_linear_rows(const __grid_constan
 }
 
 template <typename T>
-void shrink_rows_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStream_t st) {
+void shrink_rows_t(const AdapterShrink* c, int njobs, const BankSplit& split, const AdapterPlan& p, cudaStream_t st) {
   RowsShrinkArgs a{};
   a.rank = c[0].rank;
   a.R = adapter_rank_rows(a.rank);
+  a.npieces = p.npieces;
   a.pieces = p.pieces;
+  a.split = split;
   a.scales = c[0].scales;
   for (int j = 0; j < njobs; j++) a.job[j] = {c[j].X, c[j].P, c[j].Q, c[j].H, c[j].ld, c[j].ldp, (int)c[j].ld};
-  launch_chain(k_shrink_rows<T>, dim3((unsigned)p.npieces, (unsigned)((a.R + COLS - 1) / COLS), (unsigned)njobs), dim3(THREADS), 0, st, a);
+  const int groups = (a.R + COLS - 1) / COLS, per = THREADS * groups * njobs;
+  const unsigned beside = (unsigned)std::min<int64_t>((split.steps + per - 1) / per, 2 * num_sms());
+  launch_chain(k_shrink_rows<T>, dim3((unsigned)p.npieces + beside, (unsigned)groups, (unsigned)njobs), dim3(THREADS), 0, st, a);
   LC_LAUNCHED(1);
 }
 
@@ -222,12 +232,14 @@ namespace lc {
 // Requests of 16 rows or less on average cost the tensor-core forms a pass each.
 static int short_requests(const AdapterPlan& p) { return (int64_t)p.nsegs * 16 >= p.rows ? 2 : 1; }
 
-bool adapter_shrink_rows(const AdapterShrink* c, int njobs, const AdapterPlan& p, int dtype, cudaStream_t st) {
+bool adapter_shrink_rows_fit(const AdapterShrink* c, int njobs, const AdapterPlan& p) {
   int64_t C = 0;
   for (int j = 0; j < njobs; j++) C += c[j].ld;
-  if (!p.npieces || (int64_t)p.rows * adapter_rank_rows(c[0].rank) * C > kRowsShrinkMost * short_requests(p)) return false;
-  dtype == LC_F16 ? shrink_rows_t<__half>(c, njobs, p, st) : shrink_rows_t<__nv_bfloat16>(c, njobs, p, st);
-  return true;
+  return p.npieces && (int64_t)p.rows * adapter_rank_rows(c[0].rank) * C <= kRowsShrinkMost * short_requests(p);
+}
+
+void adapter_shrink_rows(const AdapterShrink* c, int njobs, const BankSplit& split, const AdapterPlan& p, int dtype, cudaStream_t st) {
+  dtype == LC_F16 ? shrink_rows_t<__half>(c, njobs, split, p, st) : shrink_rows_t<__nv_bfloat16>(c, njobs, split, p, st);
 }
 
 bool adapter_linear_rows_fit(int64_t M, int64_t N, int64_t K, const AdapterPlan& p) { return M * N * K <= kRowsLinearMost * short_requests(p); }
