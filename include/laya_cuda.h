@@ -52,6 +52,12 @@ int lc_stats(int64_t* live_tensors, int64_t* live_bytes, int64_t* launches);
 int lc_from_host(lc_tensor* out, int dtype, const int64_t* shape, int ndim, const void* data, size_t nbytes);
 /* Wraps device memory the caller owns as a dense tensor (never freed by the library). */
 int lc_from_device(lc_tensor* out, int dtype, const int64_t* shape, int ndim, void* dptr);
+/* The same for memory that `owner` keeps: on_release(owner, stream) is called
+   once, when the last tensor over it (a view and a DLPack export count) is
+   gone and no recorded graph needs it; work queued on `stream` until then may
+   still read it. Not called when this returns an error. */
+typedef void (*lc_release_fn)(void* owner, uint64_t stream);
+int lc_from_device_owned(lc_tensor* out, int dtype, const int64_t* shape, int ndim, void* dptr, lc_release_fn on_release, void* owner);
 /* index.ts:155-156 read: synchronises and copies the row-major values to `dst`. */
 int lc_read(lc_tensor t, void* dst, size_t nbytes);
 /* index.ts:157-158 dispose (idempotent at the TS layer; the C call rejects a dead handle). */

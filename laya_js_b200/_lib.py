@@ -29,6 +29,7 @@ _TYPES = {
     "lc_tensor*": C.POINTER(C.c_uint64), "constlc_tensor*": C.POINTER(C.c_uint64), "void": None,
     "constchar*": C.c_char_p, "float*": C.POINTER(C.c_float), "constfloat*": C.POINTER(C.c_float),
     "int32_t*": C.POINTER(C.c_int32), "constlc_encoder_config*": C.c_void_p, "double*": C.POINTER(C.c_double),
+    "lc_release_fn": C.c_void_p,
 }
 
 

@@ -30,12 +30,11 @@ _MODE = {"symmetric": 0, "affine": 1}
 class CudaTensor:
     """An opaque device tensor handle (index.ts:75-78 Tensor: shape + dtype)."""
 
-    __slots__ = ("handle", "shape", "dtype", "disposed", "keep", "_backend", "__weakref__")  # keep: what else the memory hangs on (interop)
+    __slots__ = ("handle", "shape", "dtype", "disposed", "_backend", "__weakref__")
 
     def __init__(self, backend: "CudaBackend", handle: int, dtype: Optional[str] = None, shape: Optional[tuple] = None):
         self._backend = backend
         self.handle = handle
-        self.keep = None
         if dtype is not None:  # the caller knows them: no call into the library
             self.shape, self.dtype, self.disposed = shape, dtype, False
             return

@@ -47,6 +47,9 @@ struct LcStorage {
   int64_t upload_mark = -1;
   uint64_t id = 0;       // unique per storage for the process's lifetime
   uint32_t version = 0;  // bumped whenever lc_copy_into writes it
+  // lc_from_device_owned: called once the last view is gone, with the stream whose work may still read the memory
+  void (*on_release)(void* owner, uint64_t stream) = nullptr;
+  void* owner = nullptr;
 };
 
 struct LcTensor {

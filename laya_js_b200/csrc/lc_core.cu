@@ -20,6 +20,10 @@
 static const uint64_t kMagic = 0x4c41594143554441ull;  // "LAYACUDA"
 
 namespace {
+struct ExternalOwner {
+  lc_release_fn on_release;
+  void* owner;
+};
 struct State {
   bool inited = false;
   int device = 0;
@@ -37,6 +41,7 @@ struct State {
   bool capturing = false;
   std::unordered_set<void*> cap_allocs;
   std::vector<void*> cap_deferred;
+  std::vector<ExternalOwner> cap_owners;  // of external memory released while capturing
   uint64_t next_storage_id = 0;
 };
 State& S() {
@@ -175,11 +180,14 @@ void release(LcTensor* t) {
   t->magic = 0;
   if (--t->st->refs == 0) {
     storage_released(t->st->id);
+    const ExternalOwner owner{t->st->on_release, t->st->owner};
     if (!t->st->external) {
       dfree(t->st->ptr);
       S().live_bytes -= (int64_t)t->st->bytes;
     }
     delete t->st;
+    if (owner.on_release && S().capturing) S().cap_owners.push_back(owner);  // the graph may read the memory
+    else if (owner.on_release) owner.on_release(owner.owner, reinterpret_cast<uint64_t>(S().cur));
   }
   delete t;
 }
@@ -555,17 +563,26 @@ int lc_from_host(lc_tensor* out, int dtype, const int64_t* shape, int ndim, cons
 }
 
 int lc_from_device(lc_tensor* out, int dtype, const int64_t* shape, int ndim, void* dptr) {
+  return lc_from_device_owned(out, dtype, shape, ndim, dptr, nullptr, nullptr);
+}
+
+int lc_from_device_owned(lc_tensor* out, int dtype, const int64_t* shape, int ndim, void* dptr, lc_release_fn on_release, void* owner) {
   LC_API_BEGIN
   LC_CHECK(dtype >= 0 && dtype < LC_NUM_DTYPES, "fromDevice: unknown dtype");
   LC_CHECK(ndim >= 0 && ndim <= LC_MAX_DIMS, "fromDevice: rank must be 0..8");
   std::vector<int64_t> sh(shape, shape + ndim);
-  LcStorage* st = new LcStorage();
+  for (auto d : sh) LC_CHECK(d >= 0, "fromDevice: negative dimension");
+  auto st = std::make_unique<LcStorage>();
   st->ptr = dptr;
   st->external = true;
   int64_t n = 1;
   for (auto d : sh) n *= d;
   st->bytes = n * dtype_size(dtype);
-  *out = handle(new_tensor(st, dtype, sh));
+  LcTensor* t = new_tensor(st.get(), dtype, sh);
+  st->on_release = on_release;  // from here on the storage's
+  st->owner = owner;
+  st.release();
+  *out = handle(t);
   LC_API_END
 }
 
@@ -827,18 +844,29 @@ struct LcGraph {
   cudaGraph_t graph = nullptr;
   cudaGraphExec_t exec = nullptr;
   std::vector<void*> deferred;  // freed with the graph
+  std::vector<ExternalOwner> owners;  // told with the graph
 };
 std::unordered_set<LcGraph*>& graphs() {
   static std::unordered_set<LcGraph*> g;
   return g;
 }
-void end_capture_state(std::vector<void*>* keep) {
+// Frees what was held back for a graph, on the current stream.
+void free_deferred(std::vector<void*>& mem, std::vector<ExternalOwner>& owners) {
+  for (void* p : mem) cudaFreeAsync(p, S().cur);
+  mem.clear();
+  std::vector<ExternalOwner> told;  // an owner may call back into the library
+  told.swap(owners);
+  for (auto& o : told) o.on_release(o.owner, reinterpret_cast<uint64_t>(S().cur));
+}
+void end_capture_state(LcGraph* keep) {
   State& s = S();
   s.capturing = false;
   s.cap_allocs.clear();
-  if (keep) keep->swap(s.cap_deferred);
-  for (void* p : s.cap_deferred) cudaFreeAsync(p, s.cur);
-  s.cap_deferred.clear();
+  if (keep) {
+    keep->deferred.swap(s.cap_deferred);
+    keep->owners.swap(s.cap_owners);
+  }
+  free_deferred(s.cap_deferred, s.cap_owners);
 }
 LcGraph* check_graph(uint64_t h) {
   LcGraph* g = reinterpret_cast<LcGraph*>(h);
@@ -869,11 +897,11 @@ int lc_graph_capture_end(uint64_t* out) {
   cudaError_t e = cudaStreamEndCapture(s.cur, &graph);
   const size_t unfreed = s.cap_allocs.size();
   auto g = std::make_unique<LcGraph>();
-  end_capture_state(&g->deferred);
+  end_capture_state(g.get());
   if (e != cudaSuccess || !graph || unfreed) {
     cudaGetLastError();
     if (graph) cudaGraphDestroy(graph);
-    for (void* p : g->deferred) cudaFreeAsync(p, s.cur);
+    free_deferred(g->deferred, g->owners);
     if (e != cudaSuccess || !graph)
       fail(std::string("graph capture failed: ") + cudaGetErrorString(e) +
            " (an op synchronised with the host or used another stream while capturing)");
@@ -884,7 +912,7 @@ int lc_graph_capture_end(uint64_t* out) {
   if (e != cudaSuccess) {
     cudaGetLastError();
     cudaGraphDestroy(graph);
-    for (void* p : g->deferred) cudaFreeAsync(p, s.cur);
+    free_deferred(g->deferred, g->owners);
     fail(std::string("graph instantiate failed: ") + cudaGetErrorString(e));
   }
   LcGraph* raw = g.release();
@@ -925,7 +953,7 @@ int lc_graph_destroy(uint64_t h) {
   // launches already queued on the stream finish before the stream-ordered frees
   if (g->exec) cudaGraphExecDestroy(g->exec);
   if (g->graph) cudaGraphDestroy(g->graph);
-  for (void* p : g->deferred) cudaFreeAsync(p, S().cur);
+  free_deferred(g->deferred, g->owners);
   g->magic = 0;
   delete g;
   LC_API_END

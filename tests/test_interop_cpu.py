@@ -1,0 +1,63 @@
+"""The exchange with torch, without a GPU: what the library is asked for, and
+what is kept until it answers."""
+from __future__ import annotations
+
+import gc
+import types
+import weakref
+
+import pytest
+import torch
+
+from laya_js_b200 import _lib, interop
+
+
+class _Cuda(torch.Tensor):
+    """A CPU tensor that says it is on the device."""
+
+    @property
+    def device(self):
+        return torch.device("cuda", 0)
+
+
+@pytest.fixture()
+def calls(monkeypatch):
+    made = []
+    monkeypatch.setattr(_lib, "call", lambda name, *a: made.append((name, a)))
+    monkeypatch.setattr(interop, "_torch_stream", lambda device: 1, raising=False)
+    return made
+
+
+def _backend():
+    return types.SimpleNamespace(device=0, _scopes=[], dispose=lambda t: None, _destroyed=False,
+                                 _wrap=lambda h, dtype, shape: types.SimpleNamespace(handle=h, dtype=dtype, shape=shape))
+
+
+def test_the_torch_tensor_outlives_the_handle_it_was_made_into(calls):
+    """Views share the library's storage, not the Python object: only the
+    storage knows when the memory is no longer read."""
+    t = torch.zeros(4, 3).as_subclass(_Cuda)
+    ref = weakref.ref(t)
+    x = interop.fromTorch(_backend(), t)
+    assert x.dtype == "f32" and x.shape == (4, 3)
+    del t, x
+    gc.collect()
+    assert ref() is not None
+    (name, args), = calls
+    assert name == "lc_from_device_owned"
+    interop._returned(args[-1], 1)  # as the library does when the last view is gone
+    gc.collect()
+    assert ref() is None
+
+
+def test_a_refused_tensor_is_not_kept(monkeypatch, calls):
+    def refuse(name, *a):
+        raise _lib.LayaCudaError("no")
+    monkeypatch.setattr(_lib, "call", refuse)
+    t = torch.zeros(4).as_subclass(_Cuda)
+    ref = weakref.ref(t)
+    with pytest.raises(_lib.LayaCudaError):
+        interop.fromTorch(_backend(), t)
+    del t
+    gc.collect()
+    assert ref() is None
