@@ -68,9 +68,11 @@ int lc_tensor_info(lc_tensor t, int* dtype, int* ndim, int64_t* shape /* [8] */)
    the library treats tensors as immutable (only lc_copy_into writes one). */
 int lc_tensor_data(lc_tensor t, uint64_t* dptr);
 /* A dense tensor as a DLPack managed tensor (DLManagedTensor*, for a capsule
-   named "dltensor"), which takes the handle over: its deleter frees the tensor
-   in the order of the library's stream at that time. The library treats the
-   memory as immutable; a strided view is an error. u16, u32 and u64 count. */
+   named "dltensor"), which takes the handle over: its deleter, which may run
+   on any thread, frees the tensor after the work that is then queued on the
+   stream that is the library's now (its consumer works there; the stream has
+   to outlive it). The library treats the memory as immutable; a strided view
+   is an error. u16, u32 and u64 count. */
 int lc_tensor_to_dlpack(lc_tensor t, uint64_t* managed);
 /* index.ts:163-164 flush: waits for queued work. */
 int lc_flush(void);

@@ -7,11 +7,22 @@
 namespace lc {
 void set_error(const std::string& m);
 void count_launch(int n);
+// Holds the library's state for one entry (again by the same thread, when an
+// entry calls back out of the library), and first frees the exported tensors
+// that other threads gave back meanwhile.
+struct ApiScope {
+  ApiScope();
+  ~ApiScope();
+  ApiScope(const ApiScope&) = delete;
+  ApiScope& operator=(const ApiScope&) = delete;
+};
 }  // namespace lc
 
 // Every exported entry point runs inside LC_API_BEGIN/END: exceptions become
 // a nonzero return code plus the message in lc_last_error().
-#define LC_API_BEGIN try {
+#define LC_API_BEGIN \
+  try {              \
+    ::lc::ApiScope api_scope;
 #define LC_API_END                                   \
   }                                                  \
   catch (const std::exception& e) {                  \

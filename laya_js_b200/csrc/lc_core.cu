@@ -9,6 +9,7 @@
 #include "lc_gemm.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <memory>
 #include <mutex>
@@ -43,12 +44,31 @@ struct State {
   std::vector<void*> cap_deferred;
   std::vector<ExternalOwner> cap_owners;  // of external memory released while capturing
   uint64_t next_storage_id = 0;
+  cudaEvent_t given_back = nullptr;  // orders the current stream behind one on which an exported tensor was used
 };
 State& S() {
   static State s;
   return s;
 }
 thread_local std::string g_err;
+
+// Tensors exported through DLPack. Their consumer drops one on any thread, at
+// any time, and its work on the stream of the export may not have run by then.
+struct ExportedTensor {
+  LcTensor* t;
+  uint64_t storage;
+  cudaStream_t stream;  // the library's when it was exported, on which the consumer works
+};
+struct Exports {
+  std::recursive_mutex api;  // the library's state
+  std::mutex m;              // `back`
+  std::vector<ExportedTensor> back;  // given back while another thread was in the library, or a capture went on
+  std::atomic<bool> any{false};
+};
+Exports& exports() {
+  static Exports* e = new Exports();  // a consumer may outlive the library's own objects
+  return *e;
+}
 }  // namespace
 
 const char* dtype_name(int d) {
@@ -191,6 +211,60 @@ void release(LcTensor* t) {
   }
   delete t;
 }
+
+// Frees an exported tensor: whatever takes its memory on the current stream
+// comes after the work queued on the stream of the export.
+static void release_exported(const ExportedTensor& x) {
+  State& s = S();
+  if (!s.live.count(x.t) || x.t->st->id != x.storage) return;  // lc_destroy freed it
+  // (cudaStreamPerThread is one name for a stream of every thread)
+  bool ordered = x.stream == s.cur && x.stream != cudaStreamPerThread;
+  if (!ordered && x.stream != cudaStreamPerThread)
+    ordered = cudaEventRecord(s.given_back, x.stream) == cudaSuccess && cudaStreamWaitEvent(s.cur, s.given_back, 0) == cudaSuccess;
+  if (!ordered) {
+    cudaGetLastError();
+    int before = s.device;
+    cudaGetDevice(&before);
+    cudaSetDevice(s.device);
+    cudaDeviceSynchronize();
+    cudaSetDevice(before);
+  }
+  release(x.t);
+}
+static void free_given_back() {
+  Exports& x = exports();
+  if (!x.any.load(std::memory_order_acquire) || S().capturing) return;
+  std::vector<ExportedTensor> back;
+  {
+    std::lock_guard<std::mutex> g(x.m);
+    back.swap(x.back);
+    x.any = false;
+  }
+  for (auto& e : back) release_exported(e);
+}
+// The consumer's deleter: at once when no other thread is in the library, else
+// with the next entry. It does not wait: it may hold what that thread waits for.
+static void give_back(const ExportedTensor& e) {
+  Exports& x = exports();
+  std::unique_lock<std::recursive_mutex> api(x.api, std::try_to_lock);
+  if (api && !S().capturing) {
+    release_exported(e);
+    return;
+  }
+  std::lock_guard<std::mutex> g(x.m);
+  x.back.push_back(e);
+  x.any.store(true, std::memory_order_release);
+}
+ApiScope::ApiScope() {
+  exports().api.lock();
+  try {
+    free_given_back();
+  } catch (...) {
+    exports().api.unlock();
+    throw;
+  }
+}
+ApiScope::~ApiScope() { exports().api.unlock(); }
 
 uint64_t handle(LcTensor* t) { return reinterpret_cast<uint64_t>(t); }
 
@@ -405,7 +479,7 @@ struct DLManagedTensor {
 struct DlpackTensor {
   DLManagedTensor managed{};  // first: the deleter gets its address
   int64_t shape[LC_MAX_DIMS];
-  uint64_t storage;
+  ExportedTensor exported;
 };
 }  // namespace
 
@@ -428,6 +502,7 @@ int lc_init(int device) {
   s.sms = prop.multiProcessorCount;
   CUDA_OK(cudaStreamCreateWithFlags(&s.own, cudaStreamNonBlocking));
   s.cur = s.own;
+  CUDA_OK(cudaEventCreateWithFlags(&s.given_back, cudaEventDisableTiming));
   // keep freed blocks cached in the stream-ordered pool
   cudaMemPool_t pool;
   CUDA_OK(cudaDeviceGetDefaultMemPool(&pool, device));
@@ -472,10 +547,11 @@ int lc_supports(int dtype, int* out) {
 }
 
 int lc_stats(int64_t* live_tensors, int64_t* live_bytes, int64_t* launches) {
+  LC_API_BEGIN
   if (live_tensors) *live_tensors = (int64_t)S().live.size();
   if (live_bytes) *live_bytes = S().live_bytes;
   if (launches) *launches = S().launches;
-  return 0;
+  LC_API_END
 }
 
 namespace {
@@ -635,11 +711,10 @@ int lc_tensor_to_dlpack(lc_tensor h, uint64_t* managed) {
   for (int i = 0; i < t->ndim; i++) m->shape[i] = t->shape[i];
   m->managed.dl_tensor.shape = m->shape;
   m->managed.manager_ctx = t;
-  m->storage = t->st->id;
+  m->exported = {t, t->st->id, stream()};
   m->managed.deleter = [](DLManagedTensor* d) {
     auto* m = reinterpret_cast<DlpackTensor*>(d);
-    auto* t = static_cast<LcTensor*>(d->manager_ctx);
-    if (S().live.count(t) && t->st->id == m->storage) release(t);  // unless lc_destroy freed it
+    give_back(m->exported);
     delete m;
   };
   *managed = reinterpret_cast<uint64_t>(&m->managed);

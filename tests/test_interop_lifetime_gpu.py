@@ -11,6 +11,7 @@ import pytest
 
 from gpu_util import backend
 from laya_js_b200 import _lib, interop
+from laya_js_b200.host import HostTensor
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +122,85 @@ def test_a_recorded_graph_keeps_it(b):
     _lib.call("lc_graph_destroy", g.value)
     gc.collect()
     assert ref() is None
+
+
+def test_memory_given_back_waits_for_the_stream_it_was_used_on(b):
+    """y is made and read on one stream, dropped while the library is on
+    another; what the library allocates there next must not take y's memory
+    before the read has run."""
+    import torch
+    n = 1 << 20
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    x = torch.arange(n, device="cuda", dtype=torch.float32)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        with torch.cuda.stream(first):
+            interop.useTorchStream(b)
+            lent = interop.fromTorch(b, x)
+            y = interop.toTorch(b, b.scale(lent, 1.0))
+            z = torch.empty_like(x)
+            torch.cuda._sleep(20_000_000)  # the read is queued behind some ten milliseconds of waiting
+            z.copy_(y)
+        with torch.cuda.stream(second):
+            interop.useTorchStream(b)
+            del y
+            others = [b.scale(lent, -2.0) for _ in range(4)]  # of y's size
+        torch.cuda.synchronize()
+        assert torch.equal(z, x)
+        for t in others:
+            b.dispose(t)
+
+
+def test_torch_tensors_dropped_by_another_thread(b):
+    """A consumer's thread drops exported tensors while this one calls the
+    library: every one is freed, once, and nothing else is."""
+    import queue
+    import threading
+
+    import torch
+    before = b.stats()
+    q: queue.Queue = queue.Queue()
+
+    def drop():
+        while (t := q.get()) is not None:
+            del t
+    threads = [threading.Thread(target=drop) for _ in range(3)]
+    for t in threads:
+        t.start()
+    x = interop.fromTorch(b, torch.arange(5000, device="cuda", dtype=torch.float32))
+    for i in range(1500):
+        y = b.scale(x, 1.0)
+        z = interop.toTorch(b, b.scale(y, 2.0))
+        q.put(z)
+        del z
+        b.dispose(y)
+    y = b.read(b.scale(x, 3.0)).data
+    for t in threads:
+        q.put(None)
+    for t in threads:
+        t.join()
+    assert np.array_equal(y, np.arange(5000, dtype=np.float32) * 3)
+    b.dispose(x)
+    after = b.stats()
+    assert after["live_tensors"] == before["live_tensors"] + 1 and after["live_bytes"] == before["live_bytes"] + 20000  # (the one that was read)
+
+
+def test_tensors_dropped_while_a_graph_is_recorded(b):
+    import torch
+    torch.cuda.synchronize()
+    _lib.call("lc_set_stream", 0)
+    x = b.fromHost(HostTensor("f32", (1000,), np.arange(1000, dtype=np.float32)))
+    y = interop.toTorch(b, b.scale(x, 2.0))
+    before = b.stats()["live_tensors"]
+    g = C.c_uint64()
+    _lib.call("lc_graph_capture_begin")
+    del y
+    t = b.add(x, x)
+    b.dispose(t)
+    assert b.stats()["live_tensors"] == before
+    _lib.call("lc_graph_capture_end", C.byref(g))
+    assert b.stats()["live_tensors"] == before - 1
+    _lib.call("lc_graph_launch", g.value)
+    _lib.call("lc_graph_destroy", g.value)
+    b.dispose(x)
+    b.flush()
