@@ -43,7 +43,8 @@ AdapterPlan* check_plan(uint64_t h) {
 // another stream waits for that copy.
 void plan_enter(AdapterPlan* p) {
   cudaStream_t st = stream();
-  if (st == p->built_on) return;
+  // (cudaStreamPerThread names another stream in every thread)
+  if (st == p->built_on && st != cudaStreamPerThread) return;
   p->shared = true;
   if (p->settled || (p->settled = cudaEventQuery(p->built) == cudaSuccess)) return;
   cudaGetLastError();
@@ -187,8 +188,8 @@ __global__ void __launch_bounds__(128) k_outer_f32(const float* __restrict__ Q, 
 
 // Scratch kept from call to call (padded operands, Q, partial sums): an
 // allocation and its release cost 1.2 us each call, a tenth of a small one.
-// It belongs to the stream of its first use (one that nobody can destroy: the
-// library's own or CUDA's default ones), whose order separates one call's
+// It belongs to the stream of its first use (the library's own or CUDA's legacy
+// default one, which nobody can destroy), whose order separates one call's
 // contents from the next; calls on other streams, in captures and beyond
 // kMost allocate theirs. It grows to what the calls before have asked for.
 struct Workspace {

@@ -101,7 +101,7 @@ void cuda_check(cudaError_t e, const char* what);
 #define CUDA_OK(x) ::lc::cuda_check((x), #x)
 
 cudaStream_t stream();
-bool permanent_stream();  // the current stream is one that no caller can destroy
+bool permanent_stream();  // the current stream is one stream for all threads, and no caller can destroy it
 int device();
 int num_sms();
 void* dmalloc(size_t bytes);

@@ -94,7 +94,7 @@ static void ensure_init() {
 cudaStream_t stream() { return S().cur; }
 bool permanent_stream() {
   const State& s = S();
-  return s.cur == s.own || s.cur == cudaStreamLegacy || s.cur == cudaStreamPerThread;
+  return s.cur == s.own || s.cur == cudaStreamLegacy;  // (cudaStreamPerThread names another stream in every thread)
 }
 int device() { return S().device; }
 int num_sms() { return S().sms; }

@@ -35,3 +35,14 @@ def test_gemm_epilogues_meet_before_warp_wide_loads():
         at = text.index(load, text.index("epilogue_tma(" if "64(" in load else "k_gemm_tc(const"))
         lines = text[:at].rstrip().splitlines()
         assert lines[-1].strip().startswith("__syncwarp()"), lines[-1]
+
+
+def test_the_per_thread_stream_is_not_taken_for_one_stream():
+    """cudaStreamPerThread is one handle value for a different stream in every
+    thread: nothing kept for a stream may be kept for it, and two uses of it
+    are not in order."""
+    core = (CSRC / "lc_core.cu").read_text()
+    body = re.sub(r"//.*", "", _body(core, core.index("bool permanent_stream()")))
+    assert "cudaStreamLegacy" in body and "cudaStreamPerThread" not in body
+    enter = (CSRC / "lc_adapters.cu").read_text()
+    assert "st != cudaStreamPerThread) return;" in _body(enter, enter.index("void plan_enter("))
