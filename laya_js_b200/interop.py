@@ -83,6 +83,10 @@ def fromTorch(b, t) -> CudaTensor:
         raise ValueError(f"fromTorch: tensor on {t.device}, backend on cuda:{b.device}")
     if not t.is_contiguous():
         raise ValueError("fromTorch: the tensor must be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("fromTorch: the tensor requires grad, which the backend's ops do not record; pass t.detach() (or use torch.no_grad())")
+    if t.is_neg():
+        raise ValueError("fromTorch: the tensor is a negated view; pass t.resolve_neg()")
     out, owner = C.c_uint64(), next(_owners)
     _lent[owner] = (t, _torch_stream(b.device))
     try:

@@ -61,3 +61,17 @@ def test_a_refused_tensor_is_not_kept(monkeypatch, calls):
     del t
     gc.collect()
     assert ref() is None
+
+
+def test_tensors_that_would_lose_something_are_refused(calls):
+    """Autograd would be cut without a word; a negated view's memory holds the
+    other sign."""
+    t = torch.zeros(4, requires_grad=True).as_subclass(_Cuda)
+    with pytest.raises(ValueError, match="requires grad"):
+        interop.fromTorch(_backend(), t)
+    with torch.no_grad():
+        interop.fromTorch(_backend(), t)
+    interop.fromTorch(_backend(), t.detach())
+    neg = torch._neg_view(torch.ones(4)).as_subclass(_Cuda)
+    with pytest.raises(ValueError, match="negated"):
+        interop.fromTorch(_backend(), neg)
