@@ -104,6 +104,12 @@ _capsule = C.pythonapi.PyCapsule_New
 _capsule.restype, _capsule.argtypes = C.py_object, [C.c_void_p, C.c_char_p, C.c_void_p]
 
 
+def _is_dense(t: CudaTensor) -> bool:
+    p = C.c_uint64()
+    _lib.call("lc_tensor_data", t.handle, C.byref(p))
+    return p.value != 0
+
+
 def toTorch(b, t: CudaTensor):
     """``t`` as a torch tensor over the same memory (DLPack). The handle now
     belongs to the torch tensor, which frees it in the order of the library's
@@ -112,8 +118,8 @@ def toTorch(b, t: CudaTensor):
     out = C.c_uint64()
     try:
         _lib.call("lc_tensor_to_dlpack", b._h(t, "toTorch"), C.byref(out))
-    except _lib.LayaCudaError as e:
-        if "dense" not in str(e):
+    except _lib.LayaCudaError:
+        if t.disposed or _is_dense(t):
             raise
         d = b.cast(t, t.dtype)
         b.dispose(t)

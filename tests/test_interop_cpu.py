@@ -75,3 +75,20 @@ def test_tensors_that_would_lose_something_are_refused(calls):
     neg = torch._neg_view(torch.ones(4)).as_subclass(_Cuda)
     with pytest.raises(ValueError, match="negated"):
         interop.fromTorch(_backend(), neg)
+
+
+def test_a_strided_view_is_known_by_asking(monkeypatch):
+    """Not by the words of an error message: any other refusal is passed on."""
+    asked = []
+
+    def call(name, *a):
+        asked.append(name)
+        if name == "lc_tensor_to_dlpack":
+            raise _lib.LayaCudaError("the device is dense with errors")
+        a[1]._obj.value = 64  # lc_tensor_data: a dense tensor's address
+    monkeypatch.setattr(_lib, "call", call)
+    b = types.SimpleNamespace(device=0, _h=lambda t, what: t.handle, cast=lambda *a: pytest.fail("copied a dense tensor"))
+    t = types.SimpleNamespace(handle=5, disposed=False, dtype="f32")
+    with pytest.raises(_lib.LayaCudaError, match="device"):
+        interop.toTorch(b, t)
+    assert asked == ["lc_tensor_to_dlpack", "lc_tensor_data"]
