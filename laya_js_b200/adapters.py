@@ -26,13 +26,21 @@ from . import compose as Cm
 from .host import HostTensor, f32_to_bf16_bits
 
 
+def _int32(what: str, v) -> np.ndarray:
+    v = np.asarray(v)
+    if v.size and v.dtype.kind not in "iu":
+        raise TypeError(f"AdapterPlan: {what} must be whole numbers, got {v.dtype}")
+    if v.size and (v.max() > np.iinfo(np.int32).max or v.min() < np.iinfo(np.int32).min):
+        raise ValueError(f"AdapterPlan: {what} must fit 32 bits")
+    return np.ascontiguousarray(v, np.int32)
+
+
 class AdapterPlan:
     """The rows of one batch: request i owns rows cu_rows[i]:cu_rows[i + 1] and
     uses adapter ``adapters[i]`` (-1: none). One plan serves every layer."""
 
     def __init__(self, backend, cu_rows, adapters, n_adapters: int):
-        cu = np.ascontiguousarray(cu_rows, np.int32)
-        ad = np.ascontiguousarray(adapters, np.int32)
+        cu, ad = _int32("cu_rows", cu_rows), _int32("adapters", adapters)
         if cu.ndim != 1 or ad.ndim != 1 or len(cu) != len(ad) + 1:
             raise ValueError(f"AdapterPlan: cu_rows has {cu.shape} entries, adapters {ad.shape}: one more than the requests is expected")
         h = C.c_uint64()
