@@ -94,15 +94,20 @@ struct GemmAdapted {
   int prows;                  // rows of P_a per block (box height of tmP)
   int per;                    // segments whose blocks of P share a stage (64 / prows)
   int defer;                  // x, w and bias were complete when the previous kernel let this one start: only U waits for it
-  // Single-CTA kernel: a tile's U (two blocks at most) stays in shared memory
-  // and stages hold blocks of P alone, 2·per to a stage (500 rows in 250
-  // requests, 768 -> 2304 in bf16, rank 16: 28 -> 25 us).
-  int resident;
+  // Single-CTA kernel, up to 64 rank rows: a tile's U (three blocks at most)
+  // stays in shared memory and stages hold blocks of P alone, 2·per to a stage,
+  // pblocks (1 or 2) to a segment. Bound by the MMAs, each over all 128 rows
+  // for the few of a request: 500 rows in 250 requests, 768 -> 2304, rank 16
+  // take 37 us in bf16 and 51 in f16, rank 40 80 and 139 (131 and 208 with U
+  // loaded again for every request).
+  int resident, pblocks;
   int kb_off;                 // added to the K block of the main loop's loads (past the operands' end: zeros)
   __device__ int u_block(int c) const { return c % uchunks; }
   __device__ int p_row(int c) const { return (c / uchunks * groups + c % groups) * 64; }
   __device__ int place(const int4& seg) const { return by_place ? seg.w : seg.z; }
 };
+
+constexpr int kUBlocks = 3;  // 64-column blocks of U that stay in shared memory
 
 // The segments [x, y) that meet the tile of `rows` (128 or 256) rows from m0.
 template <bool WT>
@@ -947,7 +952,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
   uint8_t* sPk = sB + STAGES * B_BYTES;
   uint8_t* sE = sPk + STAGES * PK_BYTES;  // epilogue staging (TMAE, or EX with rows TMA cannot store), 1024-aligned
   float* sP = (float*)(sE + (TMAE || EX::kOn ? STG_BYTES : 0));  // split-K partial tile (KS only)
-  uint64_t* full = (uint64_t*)((uint8_t*)sP + (KS ? part_bytes<BN>() : 0) + (EX::kOn ? 2 * A_BYTES : 0));
+  uint64_t* full = (uint64_t*)((uint8_t*)sP + (KS ? part_bytes<BN>() : 0) + (EX::kOn ? kUBlocks * A_BYTES : 0));
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;
@@ -959,7 +964,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
   uint64_t* ufree = ufull + 1;                 // EX: it has been multiplied
   uint32_t* tmem_slot = (uint32_t*)(ufree + 1);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
-  uint8_t* sU = sE + STG_BYTES;  // EX: two blocks of U
+  uint8_t* sU = sE + STG_BYTES;  // EX: blocks of U
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int KB = (args.K + BK - 1) / BK;
@@ -1104,15 +1109,15 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
             for (int c = 0; c < ex.uchunks; c++) tma_load_2d(sU + c * A_BYTES, &ex.tmU, ufull, c * 64, m0);
             u_issued = true;
             u_phase ^= 1;
-            for (int s = sg.x; s < sg.y; s += 2 * ex.per) {
-              const int n = min(2 * ex.per, sg.y - s);
+            for (int s = sg.x; s < sg.y; s += 2 * ex.per / ex.pblocks) {
+              const int n = min(2 * ex.per, (sg.y - s) * ex.pblocks);
               if (!mbar_wait(&empty[stage], phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
               mbar_arrive_expect_tx(&full[stage], n * (BN / 64) * ex.prows * 128);
 #pragma unroll 1
               for (int i = 0; i < n; i++) {
-                const int a = ex.place(__ldg(ex.segs + s + i));
+                const int a = ex.place(__ldg(ex.segs + s + (ex.pblocks == 2 ? i >> 1 : i))), row = ex.pblocks == 2 ? (i & 1) * 64 : 0;
                 uint8_t* dst = i < ex.per ? sA + stage * A_BYTES : sB + stage * B_BYTES - ex.per * (BN / 64) * ex.prows * 128;
-                for (int h = 0; h < BN / 64; h++) tma_load_3d(dst + (i * (BN / 64) + h) * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, 0, a);
+                for (int h = 0; h < BN / 64; h++) tma_load_3d(dst + (i * (BN / 64) + h) * ex.prows * 128, &ex.tmP, &full[stage], n0 + 64 * h, row, a);
               }
               issued[stage] = 1;
               iss_phase[stage] = phase;
@@ -1196,23 +1201,33 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           if (ex.resident && sg.x < sg.y) {
             if (!mbar_wait(ufull, u_phase, abort, &g_gemm_err)) { ok = false; break; }
             u_phase ^= 1;
-            const uint32_t u0 = smem_u32(sU);
-            for (int s = sg.x; s < sg.y; s += 2 * ex.per) {
-              const int n = min(2 * ex.per, sg.y - s);
+            // (one thread issues up to a thousand MMAs a tile here: descriptors by addition, the next segment loaded ahead)
+            const uint64_t du = sdesc_sw128(smem_u32(sU)), dp0 = sdesc_sw128_mn(smem_u32(sA), ex.prows * 128);
+            const uint32_t unit = (uint32_t)(BN / 64) * ex.prows * 8, low = (smem_u32(sB) - smem_u32(sA)) / 16;  // in 16 bytes
+            const int second = ex.pblocks - 1, R16 = ex.R16, k16 = ex.prows / 16;
+            auto u_part = [&](int b) { return du + (uint32_t)((b >> 2) * (A_BYTES / 16) + (b & 3) * 2); };
+            int4 ahead = __ldg(ex.segs + sg.x);
+            for (int s = sg.x; s < sg.y; s += 2 * ex.per / ex.pblocks) {
+              const int n = min(2 * ex.per, (sg.y - s) * ex.pblocks);
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
               tc_fence_after();
+              uint32_t off[4];
 #pragma unroll 1
               for (int i = 0; i < n; i++) {
-                const int4 seg = __ldg(ex.segs + s + i);
-                uint32_t off[4];
+                if (!(i & second)) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
-                const uint32_t p = (i < ex.per ? smem_u32(sA + stage * A_BYTES) : smem_u32(sB + stage * B_BYTES) - ex.per * (BN / 64) * ex.prows * 128) +
-                                   i * (BN / 64) * ex.prows * 128;
-                for (int k = 0; k < ex.parts * ex.R16; k++) {  // 16 rows of P: values, then remainders
-                  const uint64_t pd = sdesc_sw128_mn(p + k * 2048, ex.prows * 128);
-                  for (int b = k < ex.R16 ? k : k - ex.R16; b < (k < ex.R16 ? 3 : 2) * ex.R16; b += ex.R16)
-                    tc_mma_lanes(d, sdesc_sw128(u0 + (b >> 2) * A_BYTES + (b & 3) * 32), pd, idesc_u, 1u, off);
+                  for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, ahead.x, ahead.y);
+                  const int next = s + (i >> second) + 1;
+                  if (next < sg.y) ahead = __ldg(ex.segs + next);
+                }
+                uint64_t pd = dp0 + (i < ex.per ? stage * (A_BYTES / 16) + i * unit : low + stage * (B_BYTES / 16) + (i - ex.per) * unit);
+                const int r0 = (i & second) * 4;
+#pragma unroll 1
+                for (int r = r0; r < r0 + k16; r++, pd += 128) {  // 16 rows of P: values, then remainders
+                  const int b = r < R16 ? r : r - R16;
+                  tc_mma_lanes(d, u_part(b), pd, idesc_u, 1u, off);
+                  tc_mma_lanes(d, u_part(b + R16), pd, idesc_u, 1u, off);
+                  if (r < R16) tc_mma_lanes(d, u_part(b + 2 * R16), pd, idesc_u, 1u, off);
                 }
               }
               tc_commit(&empty[stage]);
@@ -1687,7 +1702,7 @@ CUtensorMap tensor_map_u8(const void* ptr, int64_t rows, int64_t cols, int box_c
 template <typename T, int BN, int STAGES, bool TMAE, typename EX = GemmPlain>
 void launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& my, const CUtensorMap& mr, const GemmArgs& a,
                  cudaStream_t st, const EX& ex = EX()) {
-  constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(TMAE || EX::kOn) + (EX::kOn ? 2 * BM * BK * 2 : 0);
+  constexpr size_t smem = gemm_smem_bytes<STAGES, BN>(TMAE || EX::kOn) + (EX::kOn ? kUBlocks * BM * BK * 2 : 0);
   static_assert(smem <= 232448, "GEMM shared memory above the 227 KB per-CTA limit");
   static bool attr = false;
   if (!attr) {
@@ -1960,7 +1975,8 @@ void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
   ex.steps[1] = R == 32 ? 0x50 : 0xfa50;
   ex.nsteps[1] = R == 32 ? 2 : 4;
   ex.per = 64 / ex.prows;
-  ex.resident = R <= 32;
+  ex.resident = ex.uchunks <= kUBlocks;
+  ex.pblocks = std::max(1, s.parts * R / ex.prows);
   ex.defer = c.after_share ? 1 : 0;
   ex.kb_off = c.w ? 0 : 1;  // a block past the end of the stand-in maps below, which TMA fills with zeros
   const CUtensorMap ma = c.w ? tensor_map(c.x, c.M, c.K, c.ldx, BK, BM, dtype) : tensor_map(s.u, 1, 8, 8, BK, BM, dtype);
@@ -1993,9 +2009,9 @@ void launch_adapted(const GemmAdaptedCall& c, cudaStream_t st) {
     shape(128);
     if (tmae) {
       const CUtensorMap my = tensor_map(c.y, c.M, c.N, c.ldy, 64, 32, dtype);
-      launch_gemm<T, 128, 5, true, GemmAdapted<WT>>(ma, weight_map(128), my, my, a, st, ex);
+      launch_gemm<T, 128, 4, true, GemmAdapted<WT>>(ma, weight_map(128), my, my, a, st, ex);
     } else {
-      launch_gemm<T, 128, 5, false, GemmAdapted<WT>>(ma, weight_map(128), ma, ma, a, st, ex);
+      launch_gemm<T, 128, 4, false, GemmAdapted<WT>>(ma, weight_map(128), ma, ma, a, st, ex);
     }
   }
   LC_LAUNCHED(1);
