@@ -109,6 +109,33 @@ struct GemmAdapted {
 
 constexpr int kUBlocks = 3;  // 64-column blocks of U that stay in shared memory
 
+__device__ __forceinline__ const int4* seg_list(const GemmPlain&) { return nullptr; }
+template <bool WT>
+__device__ __forceinline__ const int4* seg_list(const GemmAdapted<WT>& ex) { return ex.segs; }
+
+// The rows of a tile (32·Q from m0) that a segment leaves alone, for the thread
+// that issues the MMAs: computed once while the segment stays the same, and the
+// next one is loaded ahead (a load and the masks take as long as an MMA).
+template <int Q>
+struct SegmentRows {
+  const int4* segs;
+  int end, m0, at = -1, next;
+  int4 ahead = {};
+  uint32_t off[Q];
+  __device__ SegmentRows(const int4* s, int2 range, int m0_) : segs(s), end(range.y), m0(m0_), next(range.x) {
+    if (next < end) ahead = __ldg(segs + next);
+  }
+  __device__ void take(int i) {
+    if (i == at) return;
+    const int4 seg = i == next ? ahead : __ldg(segs + i);
+    at = i;
+    next = i + 1;
+    if (next < end) ahead = __ldg(segs + next);
+#pragma unroll
+    for (int q = 0; q < Q; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
+  }
+};
+
 // The segments [x, y) that meet the tile of `rows` (128 or 256) rows from m0.
 template <bool WT>
 __device__ __forceinline__ int2 tile_segments(const GemmAdapted<WT>& ex, int m0, int rows, int M) {
@@ -1176,7 +1203,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
       for (int w = blockIdx.x; w < args.ntiles * S && ok; w += gridDim.x) {
         const int kb0 = (w % S) * KB / S, kb1 = (w % S + 1) * KB / S;
         [[maybe_unused]] int2 sg = make_int2(0, 0);
-        if constexpr (EX::kOn) sg = tile_segments(ex, (w / args.ntile_n) * BM, BM, args.M);  // in flight during the main loop
+        if constexpr (EX::kOn) sg = tile_segments(ex, (w / args.ntile_n) * BM, BM, args.M);
+        [[maybe_unused]] SegmentRows<4> rows(EX::kOn ? seg_list(ex) : nullptr, sg, (w / args.ntile_n) * BM);  // in flight during the main loop
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * BN);
@@ -1201,33 +1229,26 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
           if (ex.resident && sg.x < sg.y) {
             if (!mbar_wait(ufull, u_phase, abort, &g_gemm_err)) { ok = false; break; }
             u_phase ^= 1;
-            // (one thread issues up to a thousand MMAs a tile here: descriptors by addition, the next segment loaded ahead)
+            // (one thread issues up to a thousand MMAs a tile here: descriptors by addition)
             const uint64_t du = sdesc_sw128(smem_u32(sU)), dp0 = sdesc_sw128_mn(smem_u32(sA), ex.prows * 128);
             const uint32_t unit = (uint32_t)(BN / 64) * ex.prows * 8, low = (smem_u32(sB) - smem_u32(sA)) / 16;  // in 16 bytes
             const int second = ex.pblocks - 1, R16 = ex.R16, k16 = ex.prows / 16;
             auto u_part = [&](int b) { return du + (uint32_t)((b >> 2) * (A_BYTES / 16) + (b & 3) * 2); };
-            int4 ahead = __ldg(ex.segs + sg.x);
             for (int s = sg.x; s < sg.y; s += 2 * ex.per / ex.pblocks) {
               const int n = min(2 * ex.per, (sg.y - s) * ex.pblocks);
               if (!mbar_wait(&full[stage], phase, abort, &g_gemm_err)) { ok = false; break; }
               tc_fence_after();
-              uint32_t off[4];
 #pragma unroll 1
               for (int i = 0; i < n; i++) {
-                if (!(i & second)) {
-#pragma unroll
-                  for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, ahead.x, ahead.y);
-                  const int next = s + (i >> second) + 1;
-                  if (next < sg.y) ahead = __ldg(ex.segs + next);
-                }
+                rows.take(s + (i >> second));
                 uint64_t pd = dp0 + (i < ex.per ? stage * (A_BYTES / 16) + i * unit : low + stage * (B_BYTES / 16) + (i - ex.per) * unit);
                 const int r0 = (i & second) * 4;
 #pragma unroll 1
                 for (int r = r0; r < r0 + k16; r++, pd += 128) {  // 16 rows of P: values, then remainders
                   const int b = r < R16 ? r : r - R16;
-                  tc_mma_lanes(d, u_part(b), pd, idesc_u, 1u, off);
-                  tc_mma_lanes(d, u_part(b + R16), pd, idesc_u, 1u, off);
-                  if (r < R16) tc_mma_lanes(d, u_part(b + 2 * R16), pd, idesc_u, 1u, off);
+                  tc_mma_lanes(d, u_part(b), pd, idesc_u, 1u, rows.off);
+                  tc_mma_lanes(d, u_part(b + R16), pd, idesc_u, 1u, rows.off);
+                  if (r < R16) tc_mma_lanes(d, u_part(b + 2 * R16), pd, idesc_u, 1u, rows.off);
                 }
               }
               tc_commit(&empty[stage]);
@@ -1246,13 +1267,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) k_gemm_tc(const __grid_consta
               const uint32_t a0 = smem_u32(sA + stage * A_BYTES), b0 = smem_u32(sB + stage * B_BYTES);
 #pragma unroll 1
               for (int i = 0; i < n; i++) {
-                const int4 seg = __ldg(ex.segs + s + i);
-                uint32_t off[4];
-#pragma unroll
-                for (int q = 0; q < 4; q++) off[q] = lanes_off(m0 + 32 * q, seg.x, seg.y);
+                rows.take(s + i);
                 uint32_t w = ex.steps[c > 0];
                 for (int k = ex.nsteps[c > 0]; k > 0; k--, w >>= 4)
-                  tc_mma_lanes(d, sdesc_sw128(a0 + (w & 3) * 32), sdesc_sw128_mn(b0 + i * ex.prows * 128 + (w >> 2 & 3) * 2048, 8192), idesc_u, 1u, off);
+                  tc_mma_lanes(d, sdesc_sw128(a0 + (w & 3) * 32), sdesc_sw128_mn(b0 + i * ex.prows * 128 + (w >> 2 & 3) * 2048, 8192), idesc_u, 1u, rows.off);
               }
               tc_commit(&empty[stage]);
               last = &empty[stage];
@@ -1568,7 +1586,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
       uint32_t last_phase = 0;
       for (int t = pair; t < args.ntiles && ok; t += npairs) {
         [[maybe_unused]] int2 sg = make_int2(0, 0);
-        if constexpr (EX::kOn) sg = tile_segments(ex, (t / args.ntile_n) * (2 * BM), 2 * BM, args.M);  // in flight during the main loop
+        if constexpr (EX::kOn) sg = tile_segments(ex, (t / args.ntile_n) * (2 * BM), 2 * BM, args.M);
+        [[maybe_unused]] SegmentRows<8> rows(EX::kOn ? seg_list(ex) : nullptr, sg, (t / args.ntile_n) * (2 * BM));  // in flight during the main loop
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort, &g_gemm_err)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * BN);
@@ -1596,13 +1615,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) k_gemm_pair(const __grid_cons
               const uint64_t da = dA0 + ((stage * A_BYTES) >> 4), db = dBt0 + ((stage * B_BYTES) >> 4);
 #pragma unroll 1
               for (int i = 0; i < n; i++) {
-                const int4 seg = __ldg(ex.segs + s + i);
-                uint32_t off[8];
-#pragma unroll
-                for (int q = 0; q < 8; q++) off[q] = lanes_off(t0 + 32 * q, seg.x, seg.y);
+                rows.take(s + i);
                 uint32_t w = ex.steps[c > 0];
                 for (int k = ex.nsteps[c > 0]; k > 0; k--, w >>= 4)
-                  tc_mma_pair_lanes(d, da + (w & 3) * 2, db + i * ex.prows * 8 + (w >> 2 & 3) * 128, idesc_u, 1u, off);
+                  tc_mma_pair_lanes(d, da + (w & 3) * 2, db + i * ex.prows * 8 + (w >> 2 & 3) * 128, idesc_u, 1u, rows.off);
               }
               tc_commit_pair(&empty[stage]);
               last = &empty[stage];
