@@ -11,10 +11,10 @@
 //   linear  8 rows of the batch against 16 rows of W, plus bias and each row's
 //           own Q · P_a
 // Bound by latency and, with few rows, the read of W (or the bank) from L2: 8
-// rows of 8 tenants, 768 -> 2304 in bf16, rank 16, take 2.9 + 4.5 us (3.5 MB
+// rows of 8 tenants, 768 -> 2304 in bf16, rank 16, take 3.2 + 5.1 us (3.5 MB
 // of W); one launch instead of two, with u shared over a cluster, took 12.8.
-// 175 and 250 registers keep one block on an SM: held to 128 they spill, and
-// the pair takes 4.8 + 5.6.
+// 234 and 252 registers keep one block on an SM: held to 128 they spill, and
+// the pair took 3 us more.
 #include "lc_adapters.h"
 #include "lc_api.h"
 #include "lc_gemm.h"

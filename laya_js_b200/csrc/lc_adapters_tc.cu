@@ -60,8 +60,8 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 // tile's columns are streamed again. D is double-buffered in TMEM.
 //
 // Bound by the read of X: 69,135 rows of 2304 and of 768 columns in f16 (424 MB),
-// rank 16, take 77 us with one request and 79 with 256 (5.4 TB/s, 0.83 of the
-// measured copy); stages of 64 columns instead of 128 took 79 and 85. With few
+// rank 16, take 78 us with 256 requests (5.4 TB/s, 0.83 of the measured copy);
+// stages of 64 columns instead of 128 took 85. With few
 // tiles the columns are split over clusters of S CTAs, whose partial D meet in
 // shared memory and are added in rank order.
 struct ShrinkJob {
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
               tma_load_2d(st, &job.tmX, &full[stage], kb * SK, it.t * BM);
               tma_load_2d(st + X_BYTES / 2, &job.tmX, &full[stage], kb * SK + 64, it.t * BM);
             }
-            // (a rolled loop: unrolled over the possible eight with the loads predicated, the kernel took 103 us instead of 83)
+            // (a rolled loop: unrolled over all that fit with the loads predicated, the kernel took 103 us instead of 83)
 #pragma unroll 1
             for (int i = 0; i < n; i++) {
               const int a = __ldg(&args.segs[it.segs.x + s + i].z);
@@ -371,9 +371,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_shrink_tc(const __grid_consta
 // over 24 runs.)
 //
 // Bound by the read of X: 69,135 rows of 2304 and of 768 columns in f16 (424
-// MB), rank 16, take 79 us with one request and 88 with 256 (5.4 and 4.8 TB/s);
-// 40,000 of 5248 and of 1024 in bf16, rank 32, 115 us. Equal runs: with a whole
-// number of runs per tile (125 of 148 SMs) that was 123.
+// MB), rank 16, take 82 us with 256 requests (5.2 TB/s); 40,000 of 5248 and of
+// 1024 in bf16, rank 32, 123 us. Equal runs: with a whole number of runs per
+// tile (125 of 148 SMs) the latter took 8 us more.
 constexpr int OUTER_THREADS = TC_THREADS + 32;  // and the warp that clears rows
 constexpr int BC = 256;                         // columns of X per CTA
 constexpr uint32_t XC_BYTES = 64 * BC * 2;
@@ -676,8 +676,11 @@ void shrink_t(const AdapterShrink* c, int njobs, const AdapterPlan& p, cudaStrea
   a.ntiles = (p.rows + BM - 1) / BM;
   a.rank = c[0].rank;
   a.R = adapter_rank_rows(a.rank);
-  // adapters side by side: 128 columns of D, 192 for rank 64 (a ragged tile of
-  // 128 rows meets two or three requests), which leaves five stages or more
+  // adapters side by side: four of 16 rank rows, two of 32 or 64 (a ragged tile
+  // of 128 rows meets two or three requests), one above. The ring then has four
+  // stages up to 32 rank rows, three up to 128 and two above (40,000 rows of
+  // 1024 columns, both directions, bf16 / f16: rank 16 42 / 44 us, 64 54 / 64,
+  // 128 81 / 96, 256 141 / 172)
   a.nb = a.R <= 32 ? 64 / a.R : a.R == 64 ? 2 : 1;
   a.bank_bytes = (uint32_t)(a.nb * a.R * 256);
   a.tmem_cols = tmem_columns(2 * a.nb * a.R);

@@ -73,8 +73,9 @@ struct GemmPlain {
 // remainders of P is below f32's rounding); f16 parts of u would end at 2^-25
 // and at 131,008. The MMAs of both types accumulate in the same f32 columns.
 // Bound by the projection: 69,135 rows, 768 -> 2304 in f16 take 197 us without
-// adapters; adding the share in a kernel of its own would read and write y
-// (318 MB) once more, ~95 us.
+// adapters, 237 with those of 256 requests (U and the split bank given);
+// adding the share in a kernel of its own would read and write y (318 MB) once
+// more, ~95 us.
 // WT: the shared projection is read transposed, D = X·W for W [K, N] (the
 // gradient with respect to the input): an MN-major B operand as well.
 template <bool WT>
