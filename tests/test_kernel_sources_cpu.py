@@ -46,3 +46,13 @@ def test_the_per_thread_stream_is_not_taken_for_one_stream():
     assert "cudaStreamLegacy" in body and "cudaStreamPerThread" not in body
     enter = (CSRC / "lc_adapters.cu").read_text()
     assert "st != cudaStreamPerThread) return;" in _body(enter, enter.index("void plan_enter("))
+
+
+def test_a_flush_reads_the_adapters_error_word_only_after_their_kernels():
+    """Every flush and every host-to-host forward takes the device errors; a
+    word of kernels that did not run would cost each a blocking copy."""
+    text = (CSRC / "lc_adapters_tc.cu").read_text()
+    body = _body(text, text.index("std::string take_adapter_errors()"))
+    assert body.index('if (!launched) return "";') < body.index("cudaMemcpyFromSymbol")
+    for entry in ("void adapter_shrink_tc(", "void adapter_outer_tc("):
+        assert "launched = true;" in _body(text, text.index(entry))
